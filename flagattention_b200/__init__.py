@@ -7,6 +7,7 @@ Public operators (no CPU path: every call runs CUDA kernels of the in-tree
 * ``paged_attention``            -- flag_attn.paged_attention drop-in
 * ``flash_attention_split_kv``   -- flag_attn.flash_attention_split_kv drop-in
 * ``flash_attention``            -- forward / LSE of flag_attn.flash_attention
+* ``prompt_attention``           -- attention over whole prompts, packed sequences
 * ``get_mla_metadata``, ``flash_mla_with_kvcache`` -- MLA metadata + decode
 * ``shard``                      -- multi-GPU sharding (sequence / KV pages)
 """
@@ -14,6 +15,7 @@ Public operators (no CPU path: every call runs CUDA kernels of the in-tree
 from flagattention_b200._lib import CudaError, InvalidArgument, Unsupported  # noqa: F401
 from flagattention_b200.mla import append_kv_rows, flash_mla_with_kvcache, get_mla_metadata  # noqa: F401
 from flagattention_b200.paged import paged_attention  # noqa: F401
+from flagattention_b200.prompt import prompt_attention  # noqa: F401
 from flagattention_b200.split_kv import flash_attention, flash_attention_split_kv  # noqa: F401
 
 __version__ = "0.1.0"

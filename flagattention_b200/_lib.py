@@ -72,6 +72,20 @@ class MlaArgs(ctypes.Structure):
     ]
 
 
+class PromptArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_stride_t", _i64), ("q_stride_h", _i64),
+        ("k", _vp), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("v", _vp), ("v_stride_t", _i64), ("v_stride_h", _i64),
+        ("cu_q", _vp), ("cu_k", _vp),
+        ("batch", _i32), ("total_q", _i32), ("total_k", _i32),
+        ("num_q_heads", _i32), ("num_kv_heads", _i32), ("d_qk", _i32), ("d_v", _i32),
+        ("causal", _i32), ("dtype", _i32), ("scale", _f32),
+        ("o", _vp), ("o_stride_t", _i64), ("o_stride_h", _i64),
+        ("lse", _vp), ("status", _vp),
+    ]
+
+
 # (name, restype, argtypes) of every exported entry point
 SIGNATURES = [
     ("fa_version", _i32, []),
@@ -89,6 +103,7 @@ SIGNATURES = [
                                         ctypes.POINTER(ctypes.c_size_t)]),
     ("fa_paged_attention", _i32, [ctypes.POINTER(DecodeArgs), _vp]),
     ("fa_split_kv_attention", _i32, [ctypes.POINTER(DecodeArgs), _vp]),
+    ("fa_prompt_attention", _i32, [ctypes.POINTER(PromptArgs), _vp]),
     ("fa_lse_combine", _i32, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp]),
     ("fa_lse_combine_strided", _i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _i32, _vp,
                                       _vp]),

@@ -35,6 +35,9 @@ int gqa_box_rows(const fa_decode_args *, int pair);
 bool gqa_pairs_heads(const fa_decode_args *);
 cudaError_t launch_mla_sv(const CUtensorMap &, const CUtensorMap &, const CUtensorMap &,
                           const CUtensorMap &, const fa_mla_args *, int, cudaStream_t);
+int prompt_tile_tokens(const fa_prompt_args *);
+cudaError_t launch_prompt(const CUtensorMap &, const CUtensorMap &, const CUtensorMap &,
+                          const fa_prompt_args *, cudaStream_t);
 }  // namespace fa
 
 namespace {
@@ -163,6 +166,33 @@ int encode_gather_map(CUtensorMap *map, const void *base, int dtype, uint64_t ro
     return fail(FA_ERR_INVALID_ARGUMENT, "gather map rejected (code %d): rows %llu stride %llu B",
                 static_cast<int>(r), (unsigned long long)rows,
                 (unsigned long long)strides[0]);
+  return FA_OK;
+}
+
+// 3-D map {d, heads, tokens} of a packed query tensor with a {64, group,
+// box_tokens} box (128-byte swizzle): one box is a Q tile's 64-dim chunk, its
+// rows ordered token by token, the group's heads inside.
+int encode_query_map(CUtensorMap *map, const void *base, int dtype, uint64_t d, uint64_t heads,
+                     uint64_t tokens, int64_t head_stride, int64_t token_stride, uint32_t group,
+                     uint32_t box_tokens) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(FA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {d, heads, tokens};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2,
+                           static_cast<cuuint64_t>(token_stride) * 2};
+  cuuint32_t box[3] = {64, group, box_tokens};
+  cuuint32_t es[3] = {1, 1, 1};
+  CUresult r = enc(map, dtype == FA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                   3, const_cast<void *>(base), dims, strides, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FA_ERR_INVALID_ARGUMENT,
+                "query map rejected (code %d): dims {%llu,%llu,%llu} strides {%llu,%llu} B",
+                static_cast<int>(r), (unsigned long long)d, (unsigned long long)heads,
+                (unsigned long long)tokens, (unsigned long long)strides[0],
+                (unsigned long long)strides[1]);
   return FA_OK;
 }
 
@@ -363,6 +393,36 @@ int validate_mla(const fa_mla_args *a) {
   return FA_OK;
 }
 
+int validate_prompt(const fa_prompt_args *a) {
+  if (!a) return fail(FA_ERR_INVALID_ARGUMENT, "null args");
+  if (a->batch < 0 || a->total_q < 0 || a->total_k < 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "prompt: negative batch or token count");
+  if (a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->num_q_heads % a->num_kv_heads != 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "number of heads in q must be a multiple of that in k & v");
+  if (a->num_q_heads / a->num_kv_heads > 128)
+    return fail(FA_ERR_UNSUPPORTED, "prompt: at most 128 query heads per kv head");
+  if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F16)
+    return fail(FA_ERR_UNSUPPORTED, "prompt attention computes in bf16 or f16");
+  if (a->d_qk <= 0 || a->d_v <= 0 || a->d_qk % 8 || a->d_v % 8 || a->d_qk > 192 || a->d_v > 128)
+    return fail(FA_ERR_UNSUPPORTED,
+                "prompt: head sizes must be multiples of 8, d_qk <= 192, d_v <= 128 (got %d/%d)",
+                a->d_qk, a->d_v);
+  if (!(a->scale > 0.f) || std::isinf(a->scale))
+    return fail(FA_ERR_INVALID_ARGUMENT, "prompt: scale must be positive and finite");
+  if (a->batch == 0 || a->total_q == 0) return FA_OK;
+  if (!a->q || !a->o || !a->cu_q || !a->cu_k || (a->total_k > 0 && (!a->k || !a->v)))
+    return fail(FA_ERR_INVALID_ARGUMENT, "null tensor");
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o))
+    return fail(FA_ERR_INVALID_ARGUMENT, "prompt: q / k / v / o must be 16-byte aligned");
+  const int64_t strides[] = {a->q_stride_t, a->q_stride_h, a->k_stride_t, a->k_stride_h,
+                             a->v_stride_t, a->v_stride_h, a->o_stride_t, a->o_stride_h};
+  for (int64_t x : strides)
+    if (x % 8 || x < 0)
+      return fail(FA_ERR_INVALID_ARGUMENT,
+                  "prompt: strides must be non-negative multiples of 8 elements (16 bytes)");
+  return FA_OK;
+}
+
 }  // namespace
 
 namespace fa {
@@ -508,6 +568,29 @@ int fa_paged_attention(const fa_decode_args *a, void *stream) {
 int fa_split_kv_attention(const fa_decode_args *a, void *stream) {
   if (a && a->block_table) return fail(FA_ERR_INVALID_ARGUMENT, "split-KV attention takes contiguous keys");
   return run_decode(a, stream);
+}
+
+int fa_prompt_attention(const fa_prompt_args *a, void *stream) {
+  int st = validate_prompt(a);
+  if (st != FA_OK) return st;
+  if (a->batch == 0 || a->total_q == 0) return FA_OK;
+  CUtensorMap qm, km, vm;
+  const uint32_t group = static_cast<uint32_t>(a->num_q_heads / a->num_kv_heads);
+  st = encode_query_map(&qm, a->q, a->dtype, a->d_qk, a->num_q_heads, a->total_q, a->q_stride_h,
+                        a->q_stride_t, group, fa::prompt_tile_tokens(a));
+  if (st != FA_OK) return st;
+  if (a->total_k > 0) {
+    st = encode_map(&km, a->k, a->dtype, a->d_qk, a->total_k, a->num_kv_heads, a->k_stride_t,
+                    a->k_stride_h, 128);
+    if (st != FA_OK) return st;
+    st = encode_map(&vm, a->v, a->dtype, a->d_v, a->total_k, a->num_kv_heads, a->v_stride_t,
+                    a->v_stride_h, 128);
+    if (st != FA_OK) return st;
+  } else {
+    km = vm = qm;  // no key exists, so no key tile is ever loaded
+  }
+  const cudaError_t e = fa::launch_prompt(qm, km, vm, a, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FA_OK : cuda_fail(e, "prompt attention launch");
 }
 
 int fa_lse_combine(const float *part_o, const float *part_lse, int num_parts, int64_t rows,

@@ -32,6 +32,9 @@
  *   fa_mla_append_rows        no reference function: writes new tokens'
  *                             latent rows into the paged pool read by the
  *                             decode (the cache layout of paged.py:22-23)
+ *   fa_prompt_attention       flash.py:269 forward (_fwd_kernel), for packed
+ *                             sequences of different lengths (the reference
+ *                             takes one length per call)
  *   fa_mla_combine_push,      paged.py:366-449 / split_kv.py:198-228 merges
  *   fa_lse_merge_wait         carried across GPUs (the reference has no
  *                             multi-GPU code); fa_ipc_* map peer memory
@@ -156,6 +159,39 @@ int fa_decode_workspace_size(const fa_decode_args *args, size_t *part_o_bytes,
                              size_t *part_lse_bytes, size_t *sched_bytes);
 int fa_paged_attention(const fa_decode_args *args, void *stream);
 int fa_split_kv_attention(const fa_decode_args *args, void *stream);
+
+/* ---- attention over whole prompts ----------------------------------------
+ * Packed sequences: tokens cu_q[b] .. cu_q[b+1]-1 of q / o and cu_k[b] ..
+ * cu_k[b+1]-1 of k / v belong to sequence b (int32 [batch + 1] on the device,
+ * starting at 0, non-decreasing).  Token t, head h of q lives at
+ * q + t*q_stride_t + h*q_stride_h (k, v, o likewise), last dims dense.  Query
+ * head h reads kv head h / (num_q_heads / num_kv_heads).  Causal: query i of
+ * lq sees keys [0, lk - lq + i] of lk (bottom-right).  A row that sees no key
+ * gets o = 0 and lse = -inf.  Tokens from cu_q[batch] on belong to no sequence
+ * and are not written.
+ * bf16 / f16, head sizes multiples of 8: d_qk <= 192, d_v <= 128; at most 128
+ * query heads per kv head; scale > 0; pointers 16-byte aligned, strides
+ * multiples of 8 elements.  lse (nullable): f32 [num_q_heads][total_q].
+ * total_q / total_k: rows of the packed tensors (bounds for every access). */
+typedef struct fa_prompt_args {
+  const void *q;
+  int64_t q_stride_t, q_stride_h;
+  const void *k;
+  int64_t k_stride_t, k_stride_h;
+  const void *v;
+  int64_t v_stride_t, v_stride_h;
+  const int32_t *cu_q, *cu_k;
+  int32_t batch, total_q, total_k;
+  int32_t num_q_heads, num_kv_heads, d_qk, d_v;
+  int32_t causal;
+  int32_t dtype;
+  float scale;
+  void *o;
+  int64_t o_stride_t, o_stride_h;
+  float *lse;
+  int *status; /* nullable device status word (kernel time-outs) */
+} fa_prompt_args;
+int fa_prompt_attention(const fa_prompt_args *args, void *stream);
 
 /* Merge `num_parts` partial results by log-sum-exp:
  *   lse = log(sum_s exp(lse_s)),  o = sum_s exp(lse_s - lse) * o_s
