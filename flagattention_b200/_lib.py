@@ -86,6 +86,23 @@ class PromptArgs(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp), ("num_blocks", _i32), ("num_kv_heads", _i32), ("block_size", _i32),
+        ("head_size", _i32), ("group_size", _i32), ("dtype", _i32),
+    ]
+
+
+class Kv4AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_stride_b", _i64), ("q_stride_h", _i64), ("cache", Kv4Cache),
+        ("block_table", _vp), ("bt_stride", _i64), ("bt_width", _i32), ("seq_lens", _vp),
+        ("batch", _i32), ("num_q_heads", _i32), ("scale", _f32),
+        ("o", _vp), ("o_stride_b", _i64), ("o_stride_h", _i64),
+        ("lse", _vp), ("part_o", _vp), ("part_lse", _vp), ("merge", _vp), ("status", _vp),
+    ]
+
+
 # (name, restype, argtypes) of every exported entry point
 SIGNATURES = [
     ("fa_version", _i32, []),
@@ -104,6 +121,16 @@ SIGNATURES = [
     ("fa_paged_attention", _i32, [ctypes.POINTER(DecodeArgs), _vp]),
     ("fa_split_kv_attention", _i32, [ctypes.POINTER(DecodeArgs), _vp]),
     ("fa_prompt_attention", _i32, [ctypes.POINTER(PromptArgs), _vp]),
+    ("fa_kv4_cache_bytes", _i32, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(_i64)]),
+    ("fa_kv4_append", _i32, [ctypes.POINTER(Kv4Cache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                             _vp]),
+    ("fa_kv4_read", _i32, [ctypes.POINTER(Kv4Cache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                           _vp]),
+    ("fa_kv4_attention_workspace_size", _i32, [ctypes.POINTER(Kv4AttentionArgs),
+                                               ctypes.POINTER(ctypes.c_size_t),
+                                               ctypes.POINTER(ctypes.c_size_t),
+                                               ctypes.POINTER(ctypes.c_size_t)]),
+    ("fa_kv4_attention", _i32, [ctypes.POINTER(Kv4AttentionArgs), _vp]),
     ("fa_lse_combine", _i32, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp]),
     ("fa_lse_combine_strided", _i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _i32, _vp,
                                       _vp]),

@@ -1,0 +1,68 @@
+// kv4.cuh -- layout of the 4-bit key / value cache, shared by the kernels that
+// write it (kv4_cache.cu) and the attention that reads it (kv4_decode.cu).
+//
+// A pool is [num_blocks][num_kv_heads][block_size / 16] tiles; a tile holds 16
+// consecutive tokens of one kv head:
+//   key codes    16 * D / 2 bytes
+//   value codes  16 * D / 2 bytes
+//   scales       16 tokens x [keys: D / G x (lo, scale) | values: the same],
+//                two 16-bit numbers (bf16 or f16, the type of the rows) each
+// so any run of tokens is a run of whole tiles, fetched by one bulk copy each.
+// A code c of a group of G dims stands for lo + scale * c.
+//
+// Codes are packed eight to a 32-bit word, and words are ordered so that
+// a lane of a warp reads what it feeds to mma.m16n8k16 with 16-byte loads and
+// without bank conflicts.  Lane l = 4 r + q (r = l / 4, q = l % 4):
+//   keys (A operand, rows = tokens r and r + 8): lane q of row t owns the
+//     words j = 4 i + q (dims 8 j .. 8 j + 7, in order, nibble n = dim 8 j +
+//     n), adjacent in memory; rows of more than 128 dims are cut into planes
+//     of 128.
+//   values (A operand of V^T P, columns = tokens 2q, 2q + 1, 2q + 8, 2q + 9):
+//     lane (r, q) owns word (u, r) of each of its four tokens; the nibbles of
+//     word (u, r) are dims 64 u + 32 p + 4 r + i with p = (n >> 1) & 1, i =
+//     (n & 1) + 2 * (n >> 2), which keeps every m16 tile of dims inside one
+//     group of 32.  16-byte planes of [r][q][4 words].
+#pragma once
+
+#include "common.cuh"
+
+namespace fa {
+namespace kv4 {
+
+constexpr int kTileTokens = 16;
+
+__host__ __device__ constexpr int code_bytes(int d) { return kTileTokens * d / 2; }  // keys or values
+__host__ __device__ constexpr int scale_bytes(int groups) { return kTileTokens * groups * 8; }
+__host__ __device__ constexpr int tile_bytes(int d, int groups) {
+  return 2 * code_bytes(d) + scale_bytes(groups);
+}
+
+// Byte offset of key word j of token t (inside the tile's key codes).
+template <int kD>
+__host__ __device__ constexpr int key_word(int t, int j) {
+  constexpr int kPlaneDims = kD < 128 ? kD : 128;
+  constexpr int kW = kPlaneDims / 32;  // words of a lane in a plane's row
+  const int plane = j / (kPlaneDims / 8), jj = j % (kPlaneDims / 8);
+  return plane * (kTileTokens * kPlaneDims / 2) + t * (kPlaneDims / 2) + ((jj % 4) * kW + jj / 4) * 4;
+}
+// Byte offset of value word (u, r) of token t (inside the tile's value codes).
+template <int kD>
+__host__ __device__ constexpr int value_word(int t, int u, int r) {
+  constexpr int kU = kD / 64;
+  const int q = (t % 8) / 2, slot = (t % 2) + 2 * (t / 8);
+  const int idx = slot * kU + u;
+  return (idx / 4) * 512 + (r * 4 + q) * 16 + (idx % 4) * 4;
+}
+
+// Where a pool slot (block * block_size + offset) lives.
+struct Pool {
+  uint8_t *data;
+  int64_t slots;  // num_blocks * block_size
+  int block_size, heads, tile_bytes;
+  __device__ __forceinline__ uint8_t *tile(int64_t block, int head, int tile_in_block) const {
+    return data + ((block * heads + head) * (block_size / kTileTokens) + tile_in_block) * tile_bytes;
+  }
+};
+
+}  // namespace kv4
+}  // namespace fa

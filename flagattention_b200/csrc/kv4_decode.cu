@@ -1,0 +1,799 @@
+// kv4_decode.cu -- one-token attention over the paged 4-bit cache (kv4.cuh).
+//
+// For sequence b, query head h of kv head g's group, over the cached tokens t
+// with codes c, group minima lo and scales s (G dims each, group index i):
+//   q . k_t = sum_i  ks_ti * (sum_{d in i} kc_td q_d) + klo_ti * (sum_{d in i} q_d)
+//   o_d     = sum_t (p_t vs_ti) vc_td  +  sum_t p_t vlo_ti
+// so codes go to the tensor cores as whole numbers, scales stay f32 factors
+// of small tiles, and nothing is expanded to 16-bit rows in memory.
+//
+// Byte-bound: a token and kv head is D + 8 D / G bytes (144 at D = 128, G =
+// 64; 512 in 16 bits).  At the measured copy rate an SM takes about 23 bytes a
+// cycle, one 16-token tile of 2304 bytes per 100 cycles, in which its four
+// schedulers issue 400 warp instructions: the instruction count per tile is
+// the second bound.  mma.sync m16n8k16 fits that: tokens (S = K Q^T) or dims
+// (O^T = V^T P) are the 16 rows, up to 8 heads the columns, codes come straight
+// from 16-byte shared-memory loads into A fragments (a shift and a three-input
+// logic operation make two 16-bit floats 16 + c from two codes), and P moves
+// between the two products in registers (movmatrix).  tcgen05 would need the
+// expanded operand written to shared memory first, 4x the bytes of the codes.
+//
+// The "16 +" is taken out exactly where it is cheap: with q_i = sum_{d in i}
+// q_d,  sum (16 + c) q = sum c q + 16 q_i (folded into the lo term), and for
+// the values 16 * sum_t P'_t, accumulated in f32 next to the lo term.
+//
+// Four warps of a CTA share a piece (a run of 64-token blocks of one entry),
+// one 16-token tile each per block; a warp has its own ring of tiles filled by
+// bulk copies.  The pieces are equal shares of all entries' blocks, cut from
+// the sequence lengths by every CTA; split entries are merged by a second
+// kernel launched as a programmatic dependent.
+#include "kv4.cuh"
+#include "flagattn_b200.h"
+#include "merge.cuh"
+
+namespace fa {
+int record_error(int status, const char *msg);
+
+namespace kv4 {
+int validate_cache(const fa_kv4_cache *c);
+Pool pool_of(const fa_kv4_cache *c);
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kBlockTokens = kWarps * kTileTokens;  // schedule unit: one tile per warp
+constexpr float kRescaleThreshold = 8.0f;           // log2 units (factor 256)
+
+struct Params {
+  const void *q;
+  int64_t q_sb, q_sh;
+  Pool pool;
+  int32_t num_blocks;
+  const int32_t *block_table;
+  int64_t bt_stride;
+  int32_t bt_width;
+  const int32_t *seq_lens;
+  int32_t batch, hq, hkv, group;
+  int32_t head_tiles;  // entries per kv head: runs of 8 * kNT query heads
+  float scale_log2;
+  void *o;
+  int64_t o_sb, o_sh;
+  float *lse;       // nullable [batch][hq]
+  float *part_o;    // [slot][8 * kNT][kD]
+  float *part_lse;  // [slot][8 * kNT]
+  int4 *merge;      // per entry: {first slot or -1, first later slot, later slots, 0}
+  int *status;
+};
+
+template <int kD, int kGroups, int kNT>
+struct Plan {
+  static constexpr int kTileB = tile_bytes(kD, kGroups);
+  static constexpr int kHeads = 8 * kNT;
+  static constexpr int kORow = kD + 4;  // f32 row pitch of the merge buffer (bank spread)
+  static constexpr int kMergeBytes = kWarps * kHeads * kORow * 4;
+  static constexpr int kMinBytes = kMergeBytes > 46080 ? kMergeBytes : 46080;
+  static constexpr int kStagesFit = kMinBytes / (kWarps * kTileB);
+  static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
+  static constexpr int kRing = kWarps * kStages * kTileB;
+  static constexpr int kBuf = kRing > kMergeBytes ? kRing : kMergeBytes;
+  static_assert(kStages >= 2, "ring");
+};
+
+struct Share {
+  long long a0, a1, x_lo, total;
+  int e_lo, e_hi, parts;
+};
+
+struct Control {
+  uint64_t full[kWarps][8];
+  int valid[kWarps][8];  // the stage holds a tile of the pool
+  long long warp_sum[kWarps];
+  Share share;
+  float m[kWarps][16], l[kWarps][16];
+  int abort_flag;
+};
+
+__device__ __forceinline__ int seq_len_of(const Params &p, int b) {
+  const int cap = static_cast<int>(
+      min(static_cast<long long>(p.bt_width) * p.pool.block_size, 0x7fffff00ll));
+  return min(max(__ldg(p.seq_lens + b), 0), cap);
+}
+__device__ __forceinline__ int blocks_of(int len) { return (len + kBlockTokens - 1) / kBlockTokens; }
+
+// The CTA's share of the work: entry costs 1 + blocks, in entry order, cut in
+// `parts` equal runs (the unit before an entry's blocks stands for its
+// per-piece overhead).  scan: batch + 1 int64 of shared memory.
+__device__ __noinline__ void compute_share(const Params &p, long long *scan, Control *ctl) {
+  const int B = p.batch, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (B + kThreads - 1) / kThreads;
+  const int b0 = min(B, tid * per), b1 = min(B, b0 + per);
+  long long local = 0;
+  for (int b = b0; b < b1; ++b) local += 1 + blocks_of(seq_len_of(p, b));
+  long long incl = local;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) ctl->warp_sum[warp] = incl;
+  __syncthreads();
+  long long run = incl - local;
+  for (int w = 0; w < warp; ++w) run += ctl->warp_sum[w];
+  for (int b = b0; b < b1; ++b) {
+    scan[b] = run;
+    run += 1 + blocks_of(seq_len_of(p, b));
+  }
+  if (b1 == B && b0 < b1) scan[B] = run;
+  __syncthreads();
+  if (tid == 0) {
+    Share sh;
+    const long long per_seq = static_cast<long long>(p.hkv) * p.head_tiles;
+    sh.total = per_seq * scan[B];
+    sh.parts = static_cast<int>(min(static_cast<long long>(gridDim.x), sh.total));
+    sh.e_lo = 0;
+    sh.e_hi = -1;
+    sh.x_lo = sh.a0 = sh.a1 = 0;
+    if (static_cast<int>(blockIdx.x) < sh.parts) {
+      sh.a0 = blockIdx.x * sh.total / sh.parts;
+      sh.a1 = (blockIdx.x + 1) * sh.total / sh.parts;
+      auto locate = [&](long long u, int &e, long long &x) {
+        int lo = 0, hi = B - 1;  // last sequence with per_seq * scan[b] <= u
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (per_seq * scan[mid] <= u) lo = mid; else hi = mid - 1;
+        }
+        const long long c = scan[lo + 1] - scan[lo];
+        const long long h = (u - per_seq * scan[lo]) / c;
+        e = static_cast<int>(lo * per_seq + h);
+        x = per_seq * scan[lo] + h * c;
+      };
+      long long x_hi;
+      locate(sh.a0, sh.e_lo, sh.x_lo);
+      locate(sh.a1 - 1, sh.e_hi, x_hi);
+    }
+    ctl->share = sh;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  return __byte_perm(a, b, sel);
+}
+// Nibbles k (0..3) of both 16-bit halves of w as two floats 16 + c: the codes
+// land in the top mantissa bits under the exponent of 16.
+template <typename T>
+__device__ __forceinline__ uint32_t codes16(uint32_t w, int k) {
+  constexpr int kTop = std::is_same<T, __half>::value ? 6 : 3;  // mantissa bits below the code
+  constexpr uint32_t kMask = 0x000f000fu << kTop;
+  constexpr uint32_t kSixteen = std::is_same<T, __half>::value ? 0x4c004c00u : 0x41804180u;
+  const int sh = kTop - 4 * k;
+  return ((sh >= 0 ? w << sh : w >> -sh) & kMask) | kSixteen;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8x8 transpose across the warp: lane l held row l / 4, columns 2 (l % 4), +1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <int kWords>
+__device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[kWords]) {
+  static_assert(kWords == 1 || kWords == 2 || kWords % 4 == 0, "vector width");
+  if constexpr (kWords == 1)
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  else if constexpr (kWords == 2)
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  else
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                   : "r"(addr + 16 * i));
+}
+// A (lo, scale) pair of the cache.
+template <typename T>
+__device__ __forceinline__ void pair_of(uint32_t w, float &lo, float &scale) {
+  const T *e = reinterpret_cast<const T *>(&w);
+  lo = Elem<T>::to_f(e[0]);
+  scale = Elem<T>::to_f(e[1]);
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+template <typename T, int kD, int kGroups, int kNT>
+__global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
+    kv4_decode_kernel(const __grid_constant__ Params p) {
+  using PL = Plan<kD, kGroups, kNT>;
+  constexpr int kG = kD / kGroups;
+  constexpr int kW = kD / 32;   // key words of a lane and token
+  constexpr int kU = kD / 64;   // value words of a lane and token
+  constexpr int kStages = PL::kStages, kTileB = PL::kTileB, kHeads = PL::kHeads;
+  constexpr bool kSplitP = std::is_same<T, __half>::value;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Control ctl;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kWarps; ++w)
+      for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&ctl.full[w][s]), 1);
+    ctl.abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  compute_share(p, reinterpret_cast<long long *>(smem), &ctl);
+  fence_proxy_async_smem();  // the ring overlays the scan
+  __syncthreads();
+  const Share &sh = ctl.share;
+  volatile int *abort_flag = &ctl.abort_flag;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * kTileB;
+  uint32_t filled = 0, used = 0;  // tiles of this warp's ring so far
+  float *obuf = reinterpret_cast<float *>(smem);
+
+  long long x = sh.x_lo;
+  for (int e = sh.e_lo; e <= sh.e_hi; ++e) {
+    // ------------------------------------------------------------ the piece
+    const int per_seq = p.hkv * p.head_tiles;
+    const int b = e / per_seq, kvh = (e % per_seq) / p.head_tiles, ht = e % p.head_tiles;
+    const int len = seq_len_of(p, b), nb = blocks_of(len);
+    const long long j0l = min(max(sh.a0 - x - 1, 0ll), static_cast<long long>(nb));
+    const long long j1l = min(max(sh.a1 - x - 1, 0ll), static_cast<long long>(nb));
+    const long long x_e = x;
+    x += 1 + nb;
+    if (nb > 0 ? j1l <= j0l : x_e < sh.a0) continue;  // the entry's unit alone: no piece here
+    const int j0 = static_cast<int>(j0l), j1 = static_cast<int>(j1l);
+    auto part_of = [&](long long u) {
+      return static_cast<int>(min(static_cast<long long>(sh.parts - 1),
+                                  ((u + 1) * sh.parts + sh.total - 1) / sh.total - 1));
+    };
+    const int p_lo = nb > 0 ? part_of(x_e + 1) : static_cast<int>(blockIdx.x);
+    const int p_hi = nb > 0 ? part_of(x_e + nb) : static_cast<int>(blockIdx.x);
+    const bool final_out = p_lo == p_hi;
+    if (j0 == 0 && threadIdx.x == 0)
+      p.merge[e] = make_int4(final_out ? -1 : sh.parts + p_lo, p_lo + 1, p_hi - p_lo, 0);
+    const int slot = j0 == 0 ? sh.parts + static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
+    const int h0 = ht * kHeads;                      // first head inside the group
+    const int heads = min(kHeads, p.group - h0);
+    // this warp's tiles: block j holds its tile j * 4 + warp
+    const int tiles_end = (len + kTileTokens - 1) / kTileTokens;
+    int n = j1 - j0;
+    while (n > 0 && (j0 + n - 1) * kWarps + warp >= tiles_end) --n;
+
+    // tiles are issued kStages ahead; lane i keeps the page of tile page0 + i
+    const int tiles_per_page = p.pool.block_size / kTileTokens;
+    int page0 = -32, my_page = -1;
+    auto issue = [&](int i) {  // i-th tile of the piece
+      const int tile = (j0 + i) * kWarps + warp;
+      if (i >= page0 + 32) {
+        page0 = i;
+        const int mine = (j0 + i + lane) * kWarps + warp;
+        my_page = mine < tiles_end
+                      ? __ldg(p.block_table + b * p.bt_stride + mine / tiles_per_page) : -1;
+      }
+      const int page = __shfl_sync(0xffffffffu, my_page, i - page0);
+      const uint32_t st = filled % kStages;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&ctl.full[warp][st]);
+        const bool ok = page >= 0 && page < p.num_blocks;  // others hold no token
+        ctl.valid[warp][st] = ok;
+        if (ok) {
+          mbar_arrive_expect_tx(bar, kTileB);
+          bulk_load(ring + st * kTileB, p.pool.tile(page, kvh, tile % tiles_per_page), kTileB, bar);
+        } else {
+          mbar_arrive(bar);
+        }
+      }
+      ++filled;
+    };
+    for (int i = 0; i < min(n, kStages); ++i) issue(i);
+
+    // Q as the B operand: pair k of word i holds dims 32 i + 8 q + {k, k + 4}
+    // of head r of each 8-head tile
+    uint32_t qf[kNT][kW][4];
+    float qs[kNT][kGroups][2];  // sum of q over a group, heads 2 q and 2 q + 1
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+      const bool live = t * 8 + r < heads;
+      const uint4 *src = reinterpret_cast<const uint4 *>(
+          static_cast<const T *>(p.q) + b * p.q_sb +
+          static_cast<int64_t>(kvh * p.group + h0 + (live ? t * 8 + r : 0)) * p.q_sh);
+      float sum[kGroups];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) sum[g] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        const uint4 v = live ? __ldg(src + 4 * i + q) : make_uint4(0u, 0u, 0u, 0u);
+        qf[t][i][0] = prmt(v.x, v.z, 0x5410);
+        qf[t][i][1] = prmt(v.x, v.z, 0x7632);
+        qf[t][i][2] = prmt(v.y, v.w, 0x5410);
+        qf[t][i][3] = prmt(v.y, v.w, 0x7632);
+        const T *el = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) sum[32 * i / kG] += Elem<T>::to_f(el[d]);
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+        qs[t][g][0] = __shfl_sync(0xffffffffu, sum[g], 8 * q);
+        qs[t][g][1] = __shfl_sync(0xffffffffu, sum[g], 8 * q + 4);
+      }
+    }
+
+    // running state; lanes of equal q agree on m; l and extra are partial sums
+    // over the lane's tokens
+    float m[kNT][2], l[kNT][2], extra[kNT][kGroups][2], o[kNT][kD / 16][4];
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        m[t][h] = -INFINITY;
+        l[t][h] = 0.f;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) extra[t][g][h] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kD / 16; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[t][i][c] = 0.f;
+    }
+
+    for (int i = 0; i < n; ++i) {
+      const uint32_t st = used % kStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.full[warp][st]), (used / kStages) & 1u,
+                                             abort_flag, p.status, kDevTimeoutProducer)))
+        break;  // the abort flag is set: copies in flight are waited for at the end
+      ++used;
+      const uint32_t tile = ring + st * kTileB;
+      const int left = len - ((j0 + i) * kWarps + warp) * kTileTokens;  // live tokens from row 0
+      const bool valid = *const_cast<volatile int *>(&ctl.valid[warp][st]) != 0;
+      if (valid) {
+        // ---------------------------------------------------------- scores
+        uint32_t ka[kW], kb[kW];
+        constexpr int kLaneWords = kW < 4 ? kW : 4;
+        constexpr int kRowBytes = 16 * kLaneWords;
+#pragma unroll
+        for (int pl = 0; pl < kW / kLaneWords; ++pl) {
+          uint32_t w[kLaneWords];
+          lds(tile + pl * (kTileTokens * kRowBytes) + r * kRowBytes + q * 4 * kLaneWords, w);
+#pragma unroll
+          for (int c = 0; c < kLaneWords; ++c) ka[pl * kLaneWords + c] = w[c];
+          lds(tile + pl * (kTileTokens * kRowBytes) + (r + 8) * kRowBytes + q * 4 * kLaneWords, w);
+#pragma unroll
+          for (int c = 0; c < kLaneWords; ++c) kb[pl * kLaneWords + c] = w[c];
+        }
+        uint32_t sca[2 * kGroups], scb[2 * kGroups];  // scale pairs of tokens r, r + 8
+        lds(tile + 2 * code_bytes(kD) + r * 8 * kGroups, sca);
+        lds(tile + 2 * code_bytes(kD) + (r + 8) * 8 * kGroups, scb);
+        float s[kNT][4];
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[t][c] = 0.f;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float acc[kNT][4];
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[t][c] = 0.f;
+#pragma unroll
+          for (int i2 = g * kW / kGroups; i2 < (g + 1) * kW / kGroups; ++i2)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              const uint32_t a0 = codes16<T>(ka[i2], 2 * ks), a1 = codes16<T>(kb[i2], 2 * ks),
+                             a2 = codes16<T>(ka[i2], 2 * ks + 1),
+                             a3 = codes16<T>(kb[i2], 2 * ks + 1);
+#pragma unroll
+              for (int t = 0; t < kNT; ++t)
+                mma16816<T>(acc[t], a0, a1, a2, a3, qf[t][i2][2 * ks], qf[t][i2][2 * ks + 1]);
+            }
+          float loa, sa, lob, sb;
+          pair_of<T>(sca[g], loa, sa);
+          pair_of<T>(scb[g], lob, sb);
+          const float ca = fmaf(-16.f, sa, loa), cb = fmaf(-16.f, sb, lob);
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+            s[t][0] += fmaf(sa, acc[t][0], ca * qs[t][g][0]);
+            s[t][1] += fmaf(sa, acc[t][1], ca * qs[t][g][1]);
+            s[t][2] += fmaf(sb, acc[t][2], cb * qs[t][g][0]);
+            s[t][3] += fmaf(sb, acc[t][3], cb * qs[t][g][1]);
+          }
+        }
+        // ------------------------------------------------- running softmax
+        const bool la = r < left, lb = r + 8 < left;  // tokens past the end: any bits
+        float top = -INFINITY;  // largest excess over the running maximum
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          s[t][0] = la ? s[t][0] * p.scale_log2 : -INFINITY;
+          s[t][1] = la ? s[t][1] * p.scale_log2 : -INFINITY;
+          s[t][2] = lb ? s[t][2] * p.scale_log2 : -INFINITY;
+          s[t][3] = lb ? s[t][3] * p.scale_log2 : -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float mx = fmaxf(s[t][h], s[t][h + 2]);
+            top = fmaxf(top, m[t][h] == -INFINITY ? (mx == -INFINITY ? -INFINITY : INFINITY)
+                                                  : mx - m[t][h]);
+          }
+        }
+        if (__any_sync(0xffffffffu, top > kRescaleThreshold)) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float mx = fmaxf(s[t][h], s[t][h + 2]);
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1)
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              const float mn = fmaxf(m[t][h], mx);
+              const float alpha = m[t][h] == -INFINITY ? 0.f : fast_exp2(m[t][h] - mn);
+              m[t][h] = mn;
+              l[t][h] *= alpha;
+#pragma unroll
+              for (int g = 0; g < kGroups; ++g) extra[t][g][h] *= alpha;
+#pragma unroll
+              for (int i2 = 0; i2 < kD / 16; ++i2) {
+                o[t][i2][h] *= alpha;
+                o[t][i2][h + 2] *= alpha;
+              }
+            }
+        }
+        // -------------------------------------------------------- P and P V
+        uint32_t pf[kNT][kGroups][kSplitP ? 4 : 2];  // B operands (hi, then lo parts)
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          const float ma = m[t][0] == -INFINITY ? 0.f : m[t][0];
+          const float mb = m[t][1] == -INFINITY ? 0.f : m[t][1];
+          const float p0 = fast_exp2(s[t][0] - ma), p1 = fast_exp2(s[t][1] - mb);
+          const float p2 = fast_exp2(s[t][2] - ma), p3 = fast_exp2(s[t][3] - mb);
+          l[t][0] += p0 + p2;
+          l[t][1] += p1 + p3;
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            float loa, sa, lob, sb;
+            pair_of<T>(sca[kGroups + g], loa, sa);
+            pair_of<T>(scb[kGroups + g], lob, sb);
+            loa = la ? loa : 0.f;  // select: scales past the end may be NaN
+            sa = la ? sa : 0.f;
+            lob = lb ? lob : 0.f;
+            sb = lb ? sb : 0.f;
+            const float x0 = p0 * sa, x1 = p1 * sa, x2 = p2 * sb, x3 = p3 * sb;
+            const uint32_t wa = Elem<__nv_bfloat16>::pack2(x0, x1);
+            const uint32_t wb = Elem<__nv_bfloat16>::pack2(x2, x3);
+            float y0 = __uint_as_float(wa << 16), y1 = __uint_as_float(wa & 0xffff0000u);
+            float y2 = __uint_as_float(wb << 16), y3 = __uint_as_float(wb & 0xffff0000u);
+            pf[t][g][0] = transpose8(wa);
+            pf[t][g][1] = transpose8(wb);
+            if constexpr (kSplitP) {
+              const uint32_t va = Elem<__nv_bfloat16>::pack2(x0 - y0, x1 - y1);
+              const uint32_t vb = Elem<__nv_bfloat16>::pack2(x2 - y2, x3 - y3);
+              pf[t][g][2] = transpose8(va);
+              pf[t][g][3] = transpose8(vb);
+              y0 += __uint_as_float(va << 16);
+              y1 += __uint_as_float(va & 0xffff0000u);
+              y2 += __uint_as_float(vb << 16);
+              y3 += __uint_as_float(vb & 0xffff0000u);
+            }
+            // the lo term, and the 16 that every code carries
+            extra[t][g][0] += fmaf(p0, loa, p2 * lob) - 16.f * (y0 + y2);
+            extra[t][g][1] += fmaf(p1, loa, p3 * lob) - 16.f * (y1 + y3);
+          }
+        }
+        uint32_t vw[4 * kU];  // [token slot][u]
+#pragma unroll
+        for (int pl = 0; pl < kU; ++pl) {
+          uint32_t w[4];
+          lds(tile + code_bytes(kD) + pl * 512 + lane * 16, w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) vw[4 * pl + c] = w[c];
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const uint32_t lo01 = prmt(vw[u], vw[kU + u], 0x5410);
+          const uint32_t hi01 = prmt(vw[u], vw[kU + u], 0x7632);
+          const uint32_t lo23 = prmt(vw[2 * kU + u], vw[3 * kU + u], 0x5410);
+          const uint32_t hi23 = prmt(vw[2 * kU + u], vw[3 * kU + u], 0x7632);
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            const int g = (64 * u + 32 * (e4 >> 1)) / kG;
+            using B = __nv_bfloat16;
+            const uint32_t a0 = codes16<B>(lo01, e4), a1 = codes16<B>(hi01, e4),
+                           a2 = codes16<B>(lo23, e4), a3 = codes16<B>(hi23, e4);
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) {
+              mma16816<B>(o[t][4 * u + e4], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
+              if constexpr (kSplitP)
+                mma16816<B>(o[t][4 * u + e4], a0, a1, a2, a3, pf[t][g][2], pf[t][g][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      if (i + kStages < n) issue(i + kStages);
+    }
+
+    // ------------------------------------------------ the warps' states meet
+    __syncthreads();  // every ring is drained: its space becomes the buffer
+    if (*abort_flag) break;  // set before the barrier: all warps leave together
+#pragma unroll
+    for (int t = 0; t < kNT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], off);
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+            extra[t][g][h] += __shfl_xor_sync(0xffffffffu, extra[t][g][h], off);
+        }
+        if (r == 0) {
+          ctl.m[warp][t * 8 + 2 * q + h] = m[t][h];
+          ctl.l[warp][t * 8 + 2 * q + h] = l[t][h];
+        }
+        float *row = obuf + (warp * kHeads + t * 8 + 2 * q + h) * PL::kORow;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int pp = 0; pp < 2; ++pp) {
+            const float ex = extra[t][(64 * u + 32 * pp) / kG][h];
+            const float *oa = o[t][4 * u + 2 * pp], *ob = o[t][4 * u + 2 * pp + 1];
+            // nibbles 2 pp and 2 pp + 1 of rows m < 8, then of rows m >= 8
+            *reinterpret_cast<float4 *>(row + 64 * u + 32 * pp + 4 * r) =
+                make_float4(oa[h] + ex, ob[h] + ex, oa[h + 2] + ex, ob[h + 2] + ex);
+          }
+      }
+    __syncthreads();
+    constexpr int kPer = kThreads / kHeads;       // threads of one head's row
+    const int hh = threadIdx.x / kPer, part = threadIdx.x % kPer;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ctl.m[w][hh]);
+    float L = 0.f, f[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      f[w] = ctl.m[w][hh] == -INFINITY ? 0.f : fast_exp2(ctl.m[w][hh] - M);
+      L += ctl.l[w][hh] * f[w];
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // a NaN stays one
+    const float lse = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+    if (hh < heads) {
+      const int h = kvh * p.group + h0 + hh;
+      for (int d = part * 4; d < kD; d += kPer * 4) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 v = *reinterpret_cast<const float4 *>(obuf + (w * kHeads + hh) * PL::kORow + d);
+          const float k = f[w] * inv;
+          acc.x = fmaf(v.x, k, acc.x);
+          acc.y = fmaf(v.y, k, acc.y);
+          acc.z = fmaf(v.z, k, acc.z);
+          acc.w = fmaf(v.w, k, acc.w);
+        }
+        if (final_out)
+          store4<T>(static_cast<T *>(p.o) + b * p.o_sb + h * p.o_sh + d, acc);
+        else
+          store4<float>(p.part_o + (static_cast<int64_t>(slot) * kHeads + hh) * kD + d, acc);
+      }
+      if (part == 0) {
+        if (!final_out)
+          p.part_lse[static_cast<int64_t>(slot) * kHeads + hh] = lse;
+        else if (p.lse)
+          p.lse[static_cast<int64_t>(b) * p.hq + h] = lse;
+      }
+    }
+    __syncthreads();          // the buffer becomes rings again
+    fence_proxy_async_smem();
+  }
+  // after a time-out copies may still be in flight: they must land before
+  // the CTA's shared memory is given back
+  if (*abort_flag) {
+    volatile int never = 0;
+    for (; used < filled; ++used)
+      mbar_wait(smem_u32(&ctl.full[warp][used % kStages]), (used / kStages) & 1u, &never, nullptr, 0);
+  }
+}
+
+// Merge of split entries: entry e = (sequence, kv head, run of head tiles),
+// one warp per row; partials f32 [slot][rows][kD].
+template <typename T>
+__global__ void __launch_bounds__(128)
+    kv4_combine_kernel(const float *__restrict__ part_o, const float *__restrict__ part_lse,
+                       const int4 *__restrict__ merge, int rows, int group, int head_tiles,
+                       int hkv, int hq, int d, T *__restrict__ out, int64_t o_sb, int64_t o_sh,
+                       float *__restrict__ lse) {
+  __shared__ MergeState states[4][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // one block per row, its four warps take every fourth partial
+  const int e = blockIdx.x / rows, row = blockIdx.x % rows;
+  const int4 mg = merge[e];
+  if (mg.x < 0) return;
+  const int ht = e % head_tiles, kvh = (e / head_tiles) % hkv, b = e / (head_tiles * hkv);
+  const int in_group = ht * rows + row;
+  if (in_group >= group) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t os = static_cast<int64_t>(rows) * d, off = static_cast<int64_t>(row) * d;
+  MergeState st;
+  st.init();
+  if (warp == 0)
+    fold_parts<false, 1>(st, part_o, part_lse, mg.x, 0, 1, 1, os, rows, off, row, d, lane);
+  fold_parts<false, 2>(st, part_o, part_lse, mg.y, warp, 4, mg.z, os, rows, off, row, d, lane);
+  states[warp][lane] = st;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) fold_state(st, states[w][lane]);
+  const int h = kvh * group + in_group;
+  const float l = finish_row<T>(st, d, out + b * o_sb + h * o_sh, lane);
+  if (lse && lane == 0) lse[static_cast<int64_t>(b) * hq + h] = l;
+}
+
+// Run of query heads one entry serves, as 8-head tiles: two where a group has
+// more than eight heads (the codes are expanded once for both), one for 256
+// dims (two would not fit the registers).
+int head_tiles_per_entry(int group, int d) { return group > 8 && d < 256 ? 2 : 1; }
+
+template <typename T, int kD, int kGroups, int kNT>
+int launch_t(const Params &p, int sms, cudaStream_t stream, int *grid_out, bool query) {
+  using PL = Plan<kD, kGroups, kNT>;
+  auto kern = kv4_decode_kernel<T, kD, kGroups, kNT>;
+  constexpr int per_sm = kD * kNT <= 128 ? 4 : 2;
+  *grid_out = sms * per_sm;
+  if (query) return FA_OK;
+  if (static_cast<int64_t>(p.batch + 1) * 8 > PL::kBuf)
+    return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many sequences per call");
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PL::kBuf);
+  if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(*grid_out);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = PL::kBuf;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
+  const int64_t blocks =
+      static_cast<int64_t>(p.batch) * p.hkv * p.head_tiles * PL::kHeads;
+  if (blocks > INT32_MAX) return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many rows");
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T>, static_cast<const float *>(p.part_o),
+                         static_cast<const float *>(p.part_lse),
+                         static_cast<const int4 *>(p.merge), PL::kHeads, p.group, p.head_tiles,
+                         p.hkv, p.hq, kD, static_cast<T *>(p.o), p.o_sb, p.o_sh, p.lse);
+  if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
+  return FA_OK;
+}
+
+template <typename T>
+int launch_d(const fa_kv4_cache *c, const Params &p, int nt, int sms, cudaStream_t s, int *grid,
+             bool query) {
+  const int key = c->head_size * 10 + c->head_size / c->group_size;
+  switch (key) {
+    case 641: return nt == 2 ? launch_t<T, 64, 1, 2>(p, sms, s, grid, query) : launch_t<T, 64, 1, 1>(p, sms, s, grid, query);
+    case 642: return nt == 2 ? launch_t<T, 64, 2, 2>(p, sms, s, grid, query) : launch_t<T, 64, 2, 1>(p, sms, s, grid, query);
+    case 1281: return nt == 2 ? launch_t<T, 128, 1, 2>(p, sms, s, grid, query) : launch_t<T, 128, 1, 1>(p, sms, s, grid, query);
+    case 1282: return nt == 2 ? launch_t<T, 128, 2, 2>(p, sms, s, grid, query) : launch_t<T, 128, 2, 1>(p, sms, s, grid, query);
+    case 1284: return nt == 2 ? launch_t<T, 128, 4, 2>(p, sms, s, grid, query) : launch_t<T, 128, 4, 1>(p, sms, s, grid, query);
+    case 2562: return launch_t<T, 256, 2, 1>(p, sms, s, grid, query);
+    default: return launch_t<T, 256, 4, 1>(p, sms, s, grid, query);
+  }
+}
+
+int validate_attention(const fa_kv4_attention_args *a) {
+  if (!a) return record_error(FA_ERR_INVALID_ARGUMENT, "null args");
+  const int st = validate_cache(&a->cache);
+  if (st != FA_OK) return st;
+  if (a->batch < 0 || a->num_q_heads <= 0 || a->num_q_heads % a->cache.num_kv_heads)
+    return record_error(FA_ERR_INVALID_ARGUMENT,
+                        "kv4 attention: query heads must be a multiple of the cache's kv heads");
+  if (a->bt_width < 0 || a->bt_stride < 0)
+    return record_error(FA_ERR_INVALID_ARGUMENT, "kv4 attention: block table shape");
+  if (!(a->scale > 0.f) || std::isinf(a->scale))
+    return record_error(FA_ERR_INVALID_ARGUMENT, "kv4 attention: scale must be positive and finite");
+  return FA_OK;
+}
+
+// Kernel parameters and grid; `query` leaves out the pointers' checks.
+int run(const fa_kv4_attention_args *a, cudaStream_t stream, bool query, int *grid, int *entries,
+        int *rows) {
+  const int group = a->num_q_heads / a->cache.num_kv_heads;
+  const int nt = head_tiles_per_entry(group, a->cache.head_size);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
+  Params p;
+  p.q = a->q;
+  p.q_sb = a->q_stride_b;
+  p.q_sh = a->q_stride_h;
+  p.pool = pool_of(&a->cache);
+  p.num_blocks = a->cache.num_blocks;
+  p.block_table = a->block_table;
+  p.bt_stride = a->bt_stride;
+  p.bt_width = a->bt_width;
+  p.seq_lens = a->seq_lens;
+  p.batch = a->batch;
+  p.hq = a->num_q_heads;
+  p.hkv = a->cache.num_kv_heads;
+  p.group = group;
+  p.head_tiles = (group + 8 * nt - 1) / (8 * nt);
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.o = a->o;
+  p.o_sb = a->o_stride_b;
+  p.o_sh = a->o_stride_h;
+  p.lse = a->lse;
+  p.part_o = a->part_o;
+  p.part_lse = a->part_lse;
+  p.merge = reinterpret_cast<int4 *>(a->merge);
+  p.status = a->status;
+  *rows = 8 * nt;
+  const int64_t n = static_cast<int64_t>(a->batch) * p.hkv * p.head_tiles;
+  if (n > INT32_MAX / 16) return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many rows");
+  *entries = static_cast<int>(n);
+  return a->cache.dtype == FA_DTYPE_F16
+             ? launch_d<__half>(&a->cache, p, nt, sms, stream, grid, query)
+             : launch_d<__nv_bfloat16>(&a->cache, p, nt, sms, stream, grid, query);
+}
+
+}  // namespace kv4
+}  // namespace fa
+
+extern "C" int fa_kv4_attention_workspace_size(const fa_kv4_attention_args *a, size_t *part_o_bytes,
+                                               size_t *part_lse_bytes, size_t *merge_bytes) {
+  using namespace fa::kv4;
+  if (!part_o_bytes || !part_lse_bytes || !merge_bytes)
+    return fa::record_error(FA_ERR_INVALID_ARGUMENT, "null out");
+  int st = validate_attention(a);
+  if (st != FA_OK) return st;
+  int grid = 0, entries = 0, rows = 0;
+  st = run(a, nullptr, true, &grid, &entries, &rows);
+  if (st != FA_OK) return st;
+  // two slots per CTA: its first and its last piece
+  const size_t cells = 2 * static_cast<size_t>(grid) * rows;
+  *part_o_bytes = cells * a->cache.head_size * sizeof(float);
+  *part_lse_bytes = (cells * sizeof(float) + 15) / 16 * 16;
+  *merge_bytes = static_cast<size_t>(entries) * 16;
+  return FA_OK;
+}
+
+extern "C" int fa_kv4_attention(const fa_kv4_attention_args *a, void *stream) {
+  using namespace fa::kv4;
+  int st = validate_attention(a);
+  if (st != FA_OK) return st;
+  if (a->batch == 0) return FA_OK;
+  auto al16 = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+  if (!a->q || !a->o || !a->seq_lens || (!a->block_table && a->bt_width > 0) || !a->part_o ||
+      !a->part_lse || !a->merge || (!a->cache.data && a->cache.num_blocks > 0))
+    return fa::record_error(FA_ERR_INVALID_ARGUMENT, "kv4 attention: null tensor");
+  if (!al16(a->q) || !al16(a->o) || !al16(a->part_o) || !al16(a->merge) || a->q_stride_b % 8 ||
+      a->q_stride_h % 8 || a->o_stride_b % 8 || a->o_stride_h % 8)
+    return fa::record_error(FA_ERR_INVALID_ARGUMENT,
+                            "kv4 attention: q / o / workspace must be 16-byte aligned, strides "
+                            "multiples of 8 elements");
+  int grid = 0, entries = 0, rows = 0;
+  return run(a, static_cast<cudaStream_t>(stream), false, &grid, &entries, &rows);
+}

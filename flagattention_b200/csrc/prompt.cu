@@ -269,7 +269,7 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
     ok = warp_wait(smem_u32(&bars->o_full[x]), 0, abort_flag, p.status, kDevTimeoutSoftmax);
   if (!ok) return;
   tc_fence_after();
-  const float f = l > 0.f ? 1.f / l : 0.f;
+  const float f = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
   T *orow = static_cast<T *>(p.o) + static_cast<int64_t>(it.q0 + tok) * p.o_st + head * p.o_sh;
 #pragma unroll 1
   for (int c = 0; c < kDv / 32; ++c) {
@@ -297,7 +297,7 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
   }
   if (live && p.lse)
     p.lse[static_cast<int64_t>(head) * p.total_q + it.q0 + tok] =
-        l > 0.f ? (m_use + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+        l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.6931471805599453f;
 }
 
 template <typename T, int kDqk, int kDv>

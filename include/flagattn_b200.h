@@ -35,6 +35,9 @@
  *   fa_prompt_attention       flash.py:269 forward (_fwd_kernel), for packed
  *                             sequences of different lengths (the reference
  *                             takes one length per call)
+ *   fa_kv4_append / _read,    no reference function: a paged cache of 4-bit
+ *   fa_kv4_attention          codes and its decode, which generalises
+ *                             paged.py:208-363 to that cache
  *   fa_mla_combine_push,      paged.py:366-449 / split_kv.py:198-228 merges
  *   fa_lse_merge_wait         carried across GPUs (the reference has no
  *                             multi-GPU code); fa_ipc_* map peer memory
@@ -192,6 +195,62 @@ typedef struct fa_prompt_args {
   int *status; /* nullable device status word (kernel time-outs) */
 } fa_prompt_args;
 int fa_prompt_attention(const fa_prompt_args *args, void *stream);
+
+/* ---- 4-bit key / value cache ----------------------------------------------
+ * A paged pool [num_blocks][num_kv_heads][block_size / 16] of 16-token tiles;
+ * a group of group_size dims of a key or value row is held as lo (its
+ * minimum), scale ((max - lo) / 15 rounded to dtype) and codes c =
+ * rint((x - lo) / scale) in 0 .. 15, and stands for lo + scale * c.  A group
+ * with a NaN or an infinity reads back as NaN.  fa_kv4_cache_bytes: the size
+ * of `data`, 2 * (head_size / 2 + 4 * head_size / group_size) bytes per token
+ * and kv head.  dtype (bf16 / f16) is the type of rows, queries and outputs;
+ * head_size 64, 128 or 256; group_size 32, 64 or 128 with 1 to 4 groups per
+ * head; block_size a multiple of 16; data 16-byte aligned. */
+typedef struct fa_kv4_cache {
+  void *data;
+  int32_t num_blocks, num_kv_heads, block_size, head_size, group_size, dtype;
+} fa_kv4_cache;
+int fa_kv4_cache_bytes(const fa_kv4_cache *cache, int64_t *bytes);
+/* Write rows t < n of k and v (row t, head h at k + t*k_stride_t +
+ * h*k_stride_h elements, 16-byte aligned, last dim dense) to pool slot
+ * slots[t] = block * block_size + offset.  A slot outside the pool (negative:
+ * padding) skips its row; slots must be distinct. */
+int fa_kv4_append(const fa_kv4_cache *cache, const void *k, int64_t k_stride_t,
+                  int64_t k_stride_h, const void *v, int64_t v_stride_t, int64_t v_stride_h,
+                  const int64_t *slots, int64_t n, void *stream);
+/* The values the cache stands for, rounded to dtype; a slot outside the pool
+ * gives a row of zeros. */
+int fa_kv4_read(const fa_kv4_cache *cache, void *k, int64_t k_stride_t, int64_t k_stride_h,
+                void *v, int64_t v_stride_t, int64_t v_stride_h, const int64_t *slots, int64_t n,
+                void *stream);
+/* One query token per sequence (q[b][h] at q + b*q_stride_b + h*q_stride_h)
+ * over the first seq_lens[b] tokens that block_table[b][0 .. bt_width) names.
+ * Tokens past the table and tokens of blocks outside the pool count as absent;
+ * a sequence without tokens gets o = 0, lse = -inf.  lse (nullable): f32
+ * [batch][num_q_heads].  part_o / part_lse / merge: scratch of the sizes
+ * fa_kv4_attention_workspace_size returns (split pieces, f32; merge records).
+ * Two launches: the decode, and the merge as its programmatic dependent. */
+typedef struct fa_kv4_attention_args {
+  const void *q;
+  int64_t q_stride_b, q_stride_h;
+  fa_kv4_cache cache;
+  const int32_t *block_table;
+  int64_t bt_stride;
+  int32_t bt_width;
+  const int32_t *seq_lens;
+  int32_t batch, num_q_heads;
+  float scale;
+  void *o;
+  int64_t o_stride_b, o_stride_h;
+  float *lse;
+  float *part_o;
+  float *part_lse;
+  int32_t *merge;
+  int *status;
+} fa_kv4_attention_args;
+int fa_kv4_attention_workspace_size(const fa_kv4_attention_args *args, size_t *part_o_bytes,
+                                    size_t *part_lse_bytes, size_t *merge_bytes);
+int fa_kv4_attention(const fa_kv4_attention_args *args, void *stream);
 
 /* Merge `num_parts` partial results by log-sum-exp:
  *   lse = log(sum_s exp(lse_s)),  o = sum_s exp(lse_s - lse) * o_s

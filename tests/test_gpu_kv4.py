@@ -1,0 +1,322 @@
+"""The 4-bit cache: writes and reads bit for bit, the decode against 64 bits.
+
+Quantisation is defined in f32 with IEEE division, so append + read is compared
+for equality with the same formula in torch.  The attention's bound is derived:
+with p the softmax weights, c / lo / s the codes, minima and scales, u the unit
+roundoff of the output type (2^-8 bf16, 2^-11 f16):
+  * p * s is rounded to bf16 before the value product (f16 caches: to two bf16
+    parts, 2^-16): u_p * sum p s c, u_p = 2^-8 or 2^-16;
+  * the output is rounded: u |o|;
+  * f32 accumulation of codes with their offset 16: 2^-20 sum p (|lo| + 47 s);
+  * scores are off by at most e = 2^-21 (3 S + 2), S = scale * sum_d |q_d| (47 s
+    + |lo|): a weight by 2 e.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import flagattention_b200 as fa
+from flagattention_b200._torch import read_status
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+UP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16}
+SHAPES = [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32), (256, 128), (256, 64)]
+
+
+def quantise(x, group):
+    """(codes, lo, scale) in f32, groups of the last dim."""
+    y = x.float().unflatten(-1, (-1, group))
+    lo, hi = y.amin(-1), y.amax(-1)
+    scale = ((hi - lo) / 15).to(x.dtype).float()
+    c = ((y - lo[..., None]) / scale[..., None]).round().clamp(0, 15)
+    return torch.where(scale[..., None] == 0, torch.zeros_like(c), c), lo, scale
+
+
+def values(x, group):
+    c, lo, scale = quantise(x, group)
+    return (lo[..., None] + c * scale[..., None]).flatten(-2)
+
+
+def rows(n, heads, d, dtype, seed, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    k = torch.randn(n, heads, d, generator=g, device="cuda") + \
+        2 * torch.randn(heads, d, generator=g, device="cuda")
+    v = torch.randn(n, heads, d, generator=g, device="cuda") * size
+    return k.to(dtype), v.to(dtype)
+
+
+def same(a, b):
+    return torch.equal(a.nan_to_num(12345.0), b.nan_to_num(12345.0)) and \
+        torch.equal(a.isnan(), b.isnan())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d, group", SHAPES)
+@pytest.mark.parametrize("heads, block, n", [(1, 16, 1), (3, 48, 200), (8, 64, 1000)])
+def test_append_then_read_is_exact(d, group, heads, block, n, dtype):
+    blocks = -(-n // block) + 2
+    cache = fa.Int4KVCache(blocks, heads, block, d, dtype=dtype, group_size=group)
+    k, v = rows(n, heads, d, dtype, 1)
+    slots = torch.randperm(blocks * block, device="cuda")[:n]
+    assert fa.append_kv_int4(k, v, cache, slots) is cache
+    for got, x in zip(fa.read_kv_int4(cache, slots), (k, v)):
+        assert same(got, values(x, group).to(dtype))
+    # the other slots were not touched
+    rest = torch.ones(blocks * block, dtype=torch.bool, device="cuda")
+    rest[slots] = False
+    for got in fa.read_kv_int4(cache, rest.nonzero()[:, 0]):
+        assert not got.any()
+
+
+def test_skipped_slots_overwrites_and_strides():
+    cache = fa.Int4KVCache(4, 2, 32, 128)
+    qkv = torch.randn(50, 8, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    qkv = qkv.to(torch.bfloat16)
+    k, v = qkv[:, 4:6], qkv[:, 6:]                       # views of a fused projection
+    slots = torch.arange(50, device="cuda") + 7
+    slots[[3, 20]] = torch.tensor([-1, 4 * 32], device="cuda")   # padding; past the pool
+    fa.append_kv_int4(k, v, cache, slots)
+    gk, gv = fa.read_kv_int4(cache, slots)
+    wk, wv = values(k, 64).to(k.dtype), values(v, 64).to(v.dtype)
+    for w in (wk, wv):
+        w[[3, 20]] = 0
+    assert same(gk, wk) and same(gv, wv)
+    fa.append_kv_int4(v, k, cache, slots)                # every bit of a row is replaced
+    gk, gv = fa.read_kv_int4(cache, slots)
+    assert same(gk, wv) and same(gv, wk)
+    odd = torch.randn(51 * 2 * 128 + 1, device="cuda").to(torch.bfloat16)[1:]
+    x = odd[:50 * 256].view(50, 2, 128)                  # off 16-byte alignment
+    fa.append_kv_int4(x, x, cache, slots)
+    assert same(fa.read_kv_int4(cache, slots)[0][:3], values(x, 64).to(x.dtype)[:3])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_constant_extreme_and_non_finite_groups(dtype):
+    cache = fa.Int4KVCache(1, 1, 16, 128, dtype=dtype)
+    top = torch.finfo(dtype).max
+    x = torch.randn(8, 1, 128, device="cuda").to(dtype)
+    x[0] = 3.25                                          # one value: scale 0, exact
+    x[1] = 0
+    x[2, 0, ::2], x[2, 0, 1::2] = top, -top              # max - min passes the type's range
+    x[3, 0, 5] = float("nan")
+    x[4, 0, 70] = float("inf")
+    x[5, 0, 7] = -float("inf")
+    x[6] = torch.finfo(dtype).tiny                       # smallest normal
+    x[7, 0, ::2], x[7, 0, 1::2] = 100, 101               # narrow range far from 0
+    slots = torch.arange(8, device="cuda")
+    fa.append_kv_int4(x, x, cache, slots)
+    for got in fa.read_kv_int4(cache, slots):
+        assert same(got[0], x[0]) and same(got[1], x[1]) and same(got[6], x[6])
+        # 15 * scale reaches the top within the rounding of the scale
+        err = (got[2].float() / top - x[2].float() / top).abs().max()
+        assert got[2].isfinite().all() and err <= 2.0 ** -6
+        assert got[3, 0, :64].isnan().all() and got[3, 0, 64:].isfinite().all()
+        assert got[4, 0, 64:].isnan().all() and got[4, 0, :64].isfinite().all()
+        assert got[5, 0, :64].isnan().all() and got[5, 0, 64:].isfinite().all()
+        assert (got[7].float() - x[7].float()).abs().max() <= 1 / 30 + 0.5 * (dtype == torch.bfloat16)
+
+
+def build(lens, hq, hk, d, group, block, dtype, seed=0, size=1.0, pool_extra=3):
+    """Cache with shuffled pages whose unused slots hold NaN scales and any
+    codes, the query, and the rows of each sequence."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    per = [-(-n // block) for n in lens]
+    blocks = sum(per) + pool_extra
+    cache = fa.Int4KVCache(blocks, hk, block, d, dtype=dtype, group_size=group)
+    cache.data.fill_(0xff)                               # bf16 / f16 0xffff is a NaN
+    perm = torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)
+    table = torch.zeros(len(lens), max(per + [1]), dtype=torch.int32, device="cuda")
+    data, a = [], 0
+    for b, n in enumerate(lens):
+        table[b, :per[b]] = perm[a:a + per[b]]
+        a += per[b]
+        k, v = rows(n, hk, d, dtype, seed * 1000 + b, size)
+        t = torch.arange(n, device="cuda")
+        fa.append_kv_int4(k, v, cache, table[b].long()[t // block] * block + t % block)
+        data.append((k, v))
+    q = torch.randn(len(lens), hq, d, generator=g, device="cuda").to(dtype)
+    return cache, table, q, data, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def check(cache, table, q, data, lens, scale=None, live=None):
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    out, lse = fa.paged_attention_int4(q, cache, lens, table, scale, return_lse=True)
+    torch.cuda.synchronize()
+    assert read_status(torch.device("cuda")) == 0
+    hq, hk, group = q.shape[1], cache.num_kv_heads, cache.group_size
+    for b, (k, v) in enumerate(data):
+        if live is not None:                              # tokens that count
+            k, v = k[live[b]], v[live[b]]
+        if k.shape[0] == 0:
+            assert not out[b].any() and (lse[b] == -np.inf).all()
+            continue
+        (ck, lk, sk), (cv, lv, sv) = ([t.double() for t in quantise(x, group)] for x in (k, v))
+        wide = lambda t: t[..., None].expand(*t.shape, group).flatten(-2)  # noqa: E731
+        heads = lambda t: t.transpose(0, 1).repeat_interleave(hq // hk, 0)  # noqa: E731
+        ck, cv = ck.flatten(-2), cv.flatten(-2)
+        kk, vv = (heads(wide(lo) + c * wide(s)) for c, lo, s in ((ck, lk, sk), (cv, lv, sv)))
+        q64 = q[b].double()[:, None]                      # [hq, 1, d]
+        s = scale * q64 @ kk.transpose(1, 2)              # [hq, 1, n]
+        p, want_l = torch.softmax(s, -1), torch.logsumexp(s, -1)
+        want = (p @ vv)[:, 0]
+        size = scale * q64.abs() @ heads(47 * wide(sk) + wide(lk).abs()).transpose(1, 2)
+        err = 2.0 ** -21 * (3 * size.amax(-1, keepdim=True) + 2)
+        mag = (p @ heads(wide(lv).abs() + 47 * wide(sv)))[:, 0]
+        tol = 1.01 * (UP[q.dtype] * (p @ heads(cv * wide(sv)))[:, 0] + U[q.dtype] * want.abs()) + \
+            (2 * err[:, 0] + 2.0 ** -20) * mag + 1e-7
+        off = (out[b].double() - want).abs()
+        assert (off <= tol).all(), f"sequence {b}: {(off / tol).max():.2f} of the bound"
+        off_l = (lse[b].double() - want_l[:, 0]).abs()
+        assert (off_l <= err[:, 0, 0] + 2.0 ** -21 * want_l[:, 0].abs()).all(), off_l.max()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d, group", SHAPES)
+@pytest.mark.parametrize("hq, hk", [(8, 1), (3, 3), (40, 2)])
+def test_decode_shapes(d, group, hq, hk, dtype):
+    lens = [1, 15, 16, 17, 63, 64, 65, 0, 200, 513]
+    check(*build(lens, hq, hk, d, group, 16, dtype, seed=1))
+
+
+@pytest.mark.parametrize("group_heads", [1, 2, 7, 8, 9, 16, 17, 64])
+def test_decode_group_sizes(group_heads):
+    check(*build([5, 300, 77], 2 * group_heads, 2, 128, 64, 32, torch.bfloat16, seed=2))
+
+
+@pytest.mark.parametrize("block", [16, 32, 48, 64, 256])
+def test_decode_pages(block):
+    check(*build([1, 31, 255, 700, 1500], 16, 2, 128, 64, block, torch.bfloat16, seed=3))
+
+
+@pytest.mark.parametrize("lens", [[20000], [9000, 1, 0, 12000], [0, 0, 0], [0, 5, 0, 0],
+                                  [1 + (i * 53) % 300 for i in range(400)]])
+def test_decode_long_split_and_many(lens):
+    check(*build(lens, 8, 2, 64, 32, 16, torch.bfloat16, seed=4))
+
+
+def test_decode_sharp_scores():
+    """Scores spread over hundreds, rising and falling along the context."""
+    cache, table, q, data, lens = build([900, 640], 8, 2, 128, 64, 16, torch.bfloat16, seed=5)
+    check(cache, table, q * 30, data, lens)
+    for b, (k, v) in enumerate(data):
+        n = k.shape[0]
+        ramp = torch.linspace(8, 0.1, n, device="cuda")[:, None, None]
+        data[b] = ((k * ramp).to(k.dtype), v)
+        t = torch.arange(n, device="cuda")
+        fa.append_kv_int4(*data[b], cache, table[b].long()[t // 16] * 16 + t % 16)
+    check(cache, table, q * 4, data, lens)
+
+
+@pytest.mark.parametrize("size", [1e-4, 1e4])
+def test_decode_f16_range(size):
+    """Value scales far below and above 1 in f16 (products p * s leave f16's
+    accurate range)."""
+    check(*build([400, 33], 8, 1, 128, 64, 16, torch.float16, seed=6, size=size))
+
+
+def test_decode_nan_stays_and_does_not_spread():
+    lens = [50, 70]
+    cache, table, q, data, n = build(lens, 4, 2, 128, 64, 16, torch.bfloat16, seed=7)
+    k = data[0][0].clone()
+    k[20, 0, 3] = float("nan")
+    fa.append_kv_int4(k[20:21], data[0][1][20:21], cache,
+                      (table[0, 1].long() * 16 + 4).reshape(1))
+    out, lse = fa.paged_attention_int4(q, cache, n, table, return_lse=True)
+    assert out[0, :2].isnan().all() and lse[0, :2].isnan().all()     # kv head 0
+    assert out[0, 2:].isfinite().all() and out[1].isfinite().all() and lse[1].isfinite().all()
+
+
+def test_decode_table_entries_outside_the_pool_and_short_tables():
+    cache, table, q, data, lens = build([100, 64, 40], 4, 2, 64, 32, 16, torch.bfloat16, seed=8)
+    live = [torch.ones(n, dtype=torch.bool, device="cuda") for n in (100, 64, 40)]
+    table[0, 2], table[1, 0] = -1, cache.num_blocks
+    live[0][32:48] = False
+    live[1][:16] = False
+    check(cache, table, q, data, lens, live=live)
+    lens[0] = 1000                                        # more tokens than the table names
+    live[0][:] = True
+    table, lens = table[:1, :2].contiguous(), lens[:1]
+    check(cache, table, q[:1], [(data[0][0][:32], data[0][1][:32])], lens)
+    lens[0] = -5
+    check(cache, table, q[:1], [(data[0][0][:0], data[0][1][:0])], lens)
+
+
+def test_decode_views_streams_and_graph():
+    cache, table, q, data, lens = build([300, 45], 8, 2, 128, 64, 16, torch.bfloat16, seed=9)
+    first = check(cache, table, q, data, lens)
+    fused = torch.zeros(2, 12, 128, dtype=q.dtype, device="cuda")
+    fused[:, 2:10] = q
+    wide = torch.zeros(2, 50, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(first, fa.paged_attention_int4(fused[:, 2:10], cache, lens,
+                                                      wide[:, :table.shape[1]]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = fa.paged_attention_int4(q, cache, lens, table)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, other)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = fa.paged_attention_int4(q, cache, lens, table)
+    lens.copy_(torch.tensor([17, 45], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, fa.paged_attention_int4(q, cache, lens, table))
+
+
+def test_pool_past_32_bit_offsets():
+    """Blocks beyond 4 GiB of the pool."""
+    block, hk, d = 256, 8, 128
+    per = hk * block * 144
+    blocks = (5 << 30) // per
+    cache = fa.Int4KVCache(blocks, hk, block, d)
+    k, v = rows(300, hk, d, torch.bfloat16, 10)
+    table = torch.tensor([[blocks - 1, blocks - 7]], dtype=torch.int32, device="cuda")
+    t = torch.arange(300, device="cuda")
+    slots = table[0].long()[t // block] * block + t % block
+    fa.append_kv_int4(k, v, cache, slots)
+    assert same(fa.read_kv_int4(cache, slots)[0], values(k, 64).to(k.dtype))
+    q = torch.randn(1, 64, d, device="cuda").to(torch.bfloat16)
+    check(cache, table, q, [(k, v)], torch.tensor([300], dtype=torch.int32, device="cuda"))
+
+
+def test_refusals():
+    for bad in (dict(block_size=24), dict(head_size=96), dict(group_size=16),
+                dict(head_size=64, group_size=128), dict(head_size=256, group_size=32),
+                dict(dtype=torch.float32)):
+        args = dict(num_blocks=2, num_kv_heads=2, block_size=16, head_size=128, group_size=64)
+        args.update(bad)
+        with pytest.raises(fa.Unsupported):
+            fa.Int4KVCache(**args)
+    with pytest.raises(fa.InvalidArgument):
+        fa.Int4KVCache(2, 0, 16, 128)
+    with pytest.raises(fa.InvalidArgument):
+        fa.Int4KVCache(2, 2, 16, 128, device="cpu")
+    cache = fa.Int4KVCache(2, 2, 16, 128)
+    x = torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(3, device="cuda")
+    for k, v, s in ((x.half(), x, slots), (x, x[:, :1], slots), (x, x, slots.int()),
+                    (x[:2], x, slots), (x, x, slots.cpu())):
+        with pytest.raises(fa.InvalidArgument):
+            fa.append_kv_int4(k, v, cache, s)
+    with pytest.raises(fa.InvalidArgument):
+        fa.read_kv_int4(cache, slots.int())
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device="cuda")
+    lens = torch.ones(1, dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    for args in ((q[:, :3], lens, table), (q.half(), lens, table), (q[..., :64], lens, table),
+                 (q, lens.long(), table), (q, lens, table.long()), (q, lens[:0], table),
+                 (q, lens, table[0])):
+        with pytest.raises(fa.InvalidArgument):
+            fa.paged_attention_int4(args[0], cache, args[1], args[2])
+    with pytest.raises(fa.InvalidArgument):
+        fa.paged_attention_int4(q, cache, lens, table, attn_scale=0.0)
+    fa.append_kv_int4(x[:0], x[:0], cache, slots[:0])
+    assert fa.read_kv_int4(cache, slots[:0])[0].shape == (0, 2, 128)
+    assert fa.paged_attention_int4(q[:0], cache, lens[:0], table[:0]).shape == (0, 4, 128)
