@@ -25,6 +25,12 @@ def stream_of(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(device_index):
+    """Handle of the device's current stream, as an integer (``stream_of``
+    without building a Stream object: about 2 us less per call)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -51,6 +57,17 @@ def status_word(device):
         t = torch.zeros(1, dtype=torch.int32, device=device)
         _status[key] = t
     return t
+
+
+_status_ptr = {}
+
+
+def status_ptr(device_index):
+    """Address of the device's status word."""
+    p = _status_ptr.get(device_index)
+    if p is None:
+        p = _status_ptr[device_index] = status_word(torch.device("cuda", device_index)).data_ptr()
+    return p
 
 
 def read_status(device):

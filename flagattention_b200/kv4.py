@@ -8,12 +8,13 @@ counterpart in the reference, whose caches hold 16-bit rows (paged.py:22-23).
 """
 
 import ctypes
+import functools
 import math
 
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import ptr, require_cuda, status_word, stream_of
+from flagattention_b200._torch import raw_stream, require_cuda, status_ptr
 
 
 class Int4KVCache:
@@ -39,9 +40,12 @@ class Int4KVCache:
         if device.type != "cuda":
             raise _lib.InvalidArgument("flagattention_b200 operators take CUDA tensors only "
                                        "(there is no CPU path)")
+        code = _lib.FA_DTYPE_F16 if dtype == torch.float16 else _lib.FA_DTYPE_BF16
+        self._struct = _lib.Kv4Cache(None, self.num_blocks, self.num_kv_heads, self.block_size,
+                                     self.head_size, self.group_size, code)
         size = ctypes.c_int64(0)
-        _lib.check(_lib.lib().fa_kv4_cache_bytes(ctypes.byref(self._struct(None)),
-                                                 ctypes.byref(size)), "fa_kv4_cache_bytes")
+        _lib.check(_lib.lib().fa_kv4_cache_bytes(ctypes.byref(self._struct), ctypes.byref(size)),
+                   "fa_kv4_cache_bytes")
         tiles = self.block_size // 16
         row = self.head_size + 8 * (self.head_size // self.group_size)
         self.data = torch.zeros((self.num_blocks, self.num_kv_heads, tiles, 16 * row),
@@ -52,28 +56,42 @@ class Int4KVCache:
     def device(self):
         return self.data.device
 
-    def _struct(self, data):
-        code = _lib.FA_DTYPE_F16 if self.dtype == torch.float16 else _lib.FA_DTYPE_BF16
-        return _lib.Kv4Cache(data, self.num_blocks, self.num_kv_heads, self.block_size,
-                             self.head_size, self.group_size, code)
-
     def struct(self):
-        return self._struct(self.data.data_ptr())
+        """The pool as the library's ``fa_kv4_cache``."""
+        self._struct.data = self.data.data_ptr()
+        return self._struct
 
 
 def _rows16(x):
     """x, or a contiguous copy where the kernels cannot address its rows."""
-    if x.stride(-1) == 1 and all(s % 8 == 0 for s in x.stride()[:-1]) and x.data_ptr() % 16 == 0:
+    t, h, d = x.stride()
+    if d == 1 and t and h and not (t | h | (x.data_ptr() >> 1)) & 7:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
 def _check_slots(slot_mapping, cache):
+    if not slot_mapping.is_cuda:
+        require_cuda(slot_mapping)
     if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
         raise _lib.InvalidArgument("slot_mapping must be int64 [n]")
-    if slot_mapping.device != cache.device:
+    if slot_mapping.get_device() != cache.data.get_device():
         raise _lib.InvalidArgument("all tensors must be on the cache's device")
     return slot_mapping.contiguous()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device_index, batch, hq, hk, head_size, group_size, dtype):
+    """(part_o, part_lse, merge) bytes for these sizes on this device."""
+    a = _lib.Kv4AttentionArgs()
+    a.cache = _lib.Kv4Cache(None, 0, hk, 16, head_size, group_size, dtype)
+    a.batch, a.num_q_heads, a.scale = batch, hq, 1.0
+    po, pl, mg = (ctypes.c_size_t(0) for _ in range(3))
+    with torch.cuda.device(device_index):
+        _lib.check(_lib.lib().fa_kv4_attention_workspace_size(
+            ctypes.byref(a), ctypes.byref(po), ctypes.byref(pl), ctypes.byref(mg)),
+            "fa_kv4_attention_workspace_size")
+    return po.value, pl.value, mg.value
 
 
 def append_kv_int4(k, v, cache, slot_mapping):
@@ -82,21 +100,25 @@ def append_kv_int4(k, v, cache, slot_mapping):
     returns the cache.  A slot outside the pool (negative: padding) skips its
     row; slots must be distinct.  A group of dims that holds a NaN or an
     infinity reads back as NaN."""
-    require_cuda(k, v, slot_mapping)
-    want = (slot_mapping.shape[0] if slot_mapping.dim() else -1, cache.num_kv_heads,
-            cache.head_size)
-    if tuple(k.shape) != want or tuple(v.shape) != want:
+    if not (k.is_cuda and v.is_cuda):
+        require_cuda(k, v)
+    slot_mapping = _check_slots(slot_mapping, cache)
+    n = slot_mapping.shape[0]
+    want = (n, cache.num_kv_heads, cache.head_size)
+    if k.shape != want or v.shape != want:
         raise _lib.InvalidArgument(f"k and v must be [n, {want[1]}, {want[2]}]")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise _lib.InvalidArgument(f"rows must be in the cache's dtype ({cache.dtype})")
-    slot_mapping = _check_slots(slot_mapping, cache)
-    if k.device != cache.device or v.device != cache.device:
+    dev = slot_mapping.get_device()
+    if k.get_device() != dev or v.get_device() != dev:
         raise _lib.InvalidArgument("all tensors must be on the cache's device")
     k, v = _rows16(k), _rows16(v)
-    _lib.check(_lib.lib().fa_kv4_append(ctypes.byref(cache.struct()), ptr(k), k.stride(0),
-                                        k.stride(1), ptr(v), v.stride(0), v.stride(1),
-                                        ptr(slot_mapping), k.shape[0], stream_of(k)),
-               "fa_kv4_append")
+    (k_t, k_h, _), (v_t, v_h, _) = k.stride(), v.stride()
+    st = _lib.lib().fa_kv4_append(ctypes.byref(cache.struct()), k.data_ptr(), k_t, k_h,
+                                  v.data_ptr(), v_t, v_h, slot_mapping.data_ptr(), n,
+                                  raw_stream(dev))
+    if st:
+        _lib.check(st, "fa_kv4_append")
     return cache
 
 
@@ -104,15 +126,15 @@ def read_kv_int4(cache, slot_mapping):
     """(k, v) [n, num_kv_heads, head_size] of the pool slots in slot_mapping
     (int64 [n]), as the values their codes stand for, in cache.dtype; zeros for
     a slot outside the pool."""
-    require_cuda(slot_mapping)
     slot_mapping = _check_slots(slot_mapping, cache)
-    shape = (slot_mapping.shape[0], cache.num_kv_heads, cache.head_size)
-    k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-    v = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-    _lib.check(_lib.lib().fa_kv4_read(ctypes.byref(cache.struct()), ptr(k), k.stride(0),
-                                      k.stride(1), ptr(v), v.stride(0), v.stride(1),
-                                      ptr(slot_mapping), shape[0], stream_of(k)),
-               "fa_kv4_read")
+    n, heads, d = slot_mapping.shape[0], cache.num_kv_heads, cache.head_size
+    k = slot_mapping.new_empty((n, heads, d), dtype=cache.dtype)
+    v = torch.empty_like(k)
+    st = _lib.lib().fa_kv4_read(ctypes.byref(cache.struct()), k.data_ptr(), heads * d, d,
+                                v.data_ptr(), heads * d, d, slot_mapping.data_ptr(), n,
+                                raw_stream(slot_mapping.get_device()))
+    if st:
+        _lib.check(st, "fa_kv4_read")
     return k, v
 
 
@@ -126,7 +148,8 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
     also the log-sum-exp f32 [num_seqs, num_q_heads].  A sequence without
     cached tokens gets zeros and -inf.
     """
-    require_cuda(query, context_lens, block_tables)
+    if not (query.is_cuda and context_lens.is_cuda and block_tables.is_cuda):
+        require_cuda(query, context_lens, block_tables)
     if query.dim() != 3 or query.shape[2] != cache.head_size:
         raise _lib.InvalidArgument("query must be [num_seqs, num_q_heads, head_size of the cache]")
     if query.dtype != cache.dtype:
@@ -136,35 +159,31 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
         raise _lib.InvalidArgument("num_q_heads must be a multiple of the cache's kv heads")
     if context_lens.dtype != torch.int32 or block_tables.dtype != torch.int32:
         raise _lib.InvalidArgument("context_lens and block_tables must be int32")
-    if tuple(context_lens.shape) != (num_seqs,) or block_tables.dim() != 2 or \
+    if context_lens.shape != (num_seqs,) or block_tables.dim() != 2 or \
             block_tables.shape[0] != num_seqs:
         raise _lib.InvalidArgument("context_lens [num_seqs] and block_tables [num_seqs, width]")
-    if any(t.device != cache.device for t in (query, context_lens, block_tables)):
+    dev = query.get_device()
+    if cache.data.get_device() != dev or context_lens.get_device() != dev or \
+            block_tables.get_device() != dev:
         raise _lib.InvalidArgument("all tensors must be on the cache's device")
     query, context_lens = _rows16(query), context_lens.contiguous()
-    if block_tables.stride(-1) != 1:
+    if block_tables.stride(1) != 1:
         block_tables = block_tables.contiguous()
-    out = torch.empty((num_seqs, hq, d), dtype=query.dtype, device=query.device)
-    lse = torch.empty((num_seqs, hq), dtype=torch.float32, device=query.device) \
-        if return_lse else None
-    a = _lib.Kv4AttentionArgs()
-    a.q, a.q_stride_b, a.q_stride_h = query.data_ptr(), query.stride(0), query.stride(1)
-    a.cache = cache.struct()
-    a.block_table, a.bt_stride = block_tables.data_ptr(), block_tables.stride(0)
-    a.bt_width = block_tables.shape[1]
-    a.seq_lens = context_lens.data_ptr()
-    a.batch, a.num_q_heads = num_seqs, hq
-    a.scale = float(attn_scale if attn_scale is not None else 1.0 / math.sqrt(d))
-    a.o, a.o_stride_b, a.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    a.lse = lse.data_ptr() if return_lse else None
-    a.status = status_word(query.device).data_ptr()
-    po, pl, mg = (ctypes.c_size_t(0) for _ in range(3))
-    _lib.check(_lib.lib().fa_kv4_attention_workspace_size(
-        ctypes.byref(a), ctypes.byref(po), ctypes.byref(pl), ctypes.byref(mg)),
-        "fa_kv4_attention_workspace_size")
-    ws = torch.empty(po.value + pl.value + mg.value, dtype=torch.uint8, device=query.device)
-    a.part_o = ws.data_ptr()
-    a.part_lse = a.part_o + po.value
-    a.merge = a.part_lse + pl.value
-    _lib.check(_lib.lib().fa_kv4_attention(ctypes.byref(a), stream_of(query)), "fa_kv4_attention")
+    c = cache.struct()
+    out = query.new_empty((num_seqs, hq, d))
+    lse = query.new_empty((num_seqs, hq), dtype=torch.float32) if return_lse else None
+    po, pl, mg = _workspace_bytes(dev, num_seqs, hq, c.num_kv_heads, d, c.group_size, c.dtype)
+    ws = query.new_empty((po + pl + mg,), dtype=torch.uint8)
+    base = ws.data_ptr()
+    q_b, q_h, _ = query.stride()
+    # field order of fa_kv4_attention_args
+    a = _lib.Kv4AttentionArgs(query.data_ptr(), q_b, q_h, c, block_tables.data_ptr(),
+                              block_tables.stride(0), block_tables.shape[1],
+                              context_lens.data_ptr(), num_seqs, hq,
+                              1.0 / math.sqrt(d) if attn_scale is None else attn_scale,
+                              out.data_ptr(), hq * d, d, lse.data_ptr() if return_lse else None,
+                              base, base + po, base + po + pl, status_ptr(dev))
+    st = _lib.lib().fa_kv4_attention(ctypes.byref(a), raw_stream(dev))
+    if st:
+        _lib.check(st, "fa_kv4_attention")
     return (out, lse) if return_lse else out

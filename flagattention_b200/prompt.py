@@ -15,14 +15,14 @@ import math
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import dtype_code, require_cuda, status_word, stream_of
+from flagattention_b200._torch import dtype_code, raw_stream, require_cuda, status_ptr
 
 
 def _rows16(x):
     """x, or a contiguous copy where the kernel cannot address its rows
-    (inner stride, 16-byte alignment)."""
-    if x.stride(-1) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and \
-            x.stride(0) >= 0 and x.stride(1) >= 0 and x.data_ptr() % 16 == 0:
+    (inner stride, broadcast dims, 16-byte alignment)."""
+    t, h, d = x.stride()
+    if d == 1 and t and h and not (t | h | (x.data_ptr() >> 1)) & 7:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -43,40 +43,42 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
     """
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
-    require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and cu_seqlens_q.is_cuda and
+            cu_seqlens_k.is_cuda):
+        require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise _lib.InvalidArgument("q, k, v must be [tokens, heads, head size]")
-    (total_q, hq, d), (total_k, hk, _), d_v = q.shape, k.shape, v.shape[2]
-    if k.shape[2] != d or v.shape[:2] != k.shape[:2]:
+    (total_q, hq, d), (total_k, hk, d_k), (total_v, hv, d_v) = q.shape, k.shape, v.shape
+    if d_k != d or total_v != total_k or hv != hk:
         raise _lib.InvalidArgument("q/k/v shapes disagree")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise _lib.InvalidArgument("q, k and v dtypes differ")
     if hk == 0 or hq == 0 or hq % hk != 0:
         raise _lib.InvalidArgument("number of heads in q must be a multiple of that in k & v")
-    for cu in (cu_seqlens_q, cu_seqlens_k):
-        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape[0] < 1 or \
-                cu.shape != cu_seqlens_q.shape:
-            raise _lib.InvalidArgument("cu_seqlens must be int32 [batch + 1]")
-    devices = {t.device for t in (q, k, v, cu_seqlens_q, cu_seqlens_k)}
-    if len(devices) != 1:
+    if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_k.dtype != torch.int32 or \
+            cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] < 1 or \
+            cu_seqlens_k.shape != cu_seqlens_q.shape:
+        raise _lib.InvalidArgument("cu_seqlens must be int32 [batch + 1]")
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev or cu_seqlens_q.get_device() != dev or \
+            cu_seqlens_k.get_device() != dev:
         raise _lib.InvalidArgument("all tensors must be on one device")
+    code = dtype_code(q)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
-    out = torch.empty((total_q, hq, d_v), dtype=q.dtype, device=q.device)
-    lse = torch.empty((hq, total_q), dtype=torch.float32, device=q.device) if return_lse else None
-    a = _lib.PromptArgs()
-    a.q, a.q_stride_t, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.k_stride_t, a.k_stride_h = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.v_stride_t, a.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
-    a.cu_q, a.cu_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
-    a.batch, a.total_q, a.total_k = cu_seqlens_q.shape[0] - 1, total_q, total_k
-    a.num_q_heads, a.num_kv_heads, a.d_qk, a.d_v = hq, hk, d, d_v
-    a.causal = int(bool(causal))
-    a.dtype = dtype_code(q)
-    a.scale = float(sm_scale if sm_scale is not None else 1.0 / math.sqrt(d))
-    a.o, a.o_stride_t, a.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    a.lse = lse.data_ptr() if return_lse else None
-    a.status = status_word(q.device).data_ptr()
-    _lib.check(_lib.lib().fa_prompt_attention(ctypes.byref(a), stream_of(q)),
-               "fa_prompt_attention")
+    out = q.new_empty((total_q, hq, d_v))
+    lse = q.new_empty((hq, total_q), dtype=torch.float32) if return_lse else None
+    (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _) = q.stride(), k.stride(), v.stride()
+    # field order of fa_prompt_args
+    a = _lib.PromptArgs(q.data_ptr(), q_t, q_h, k.data_ptr(), k_t, k_h, v.data_ptr(), v_t, v_h,
+                        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+                        cu_seqlens_q.shape[0] - 1, total_q, total_k, hq, hk, d, d_v,
+                        1 if causal else 0, code,
+                        1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
+                        out.data_ptr(), hq * d_v, d_v, lse.data_ptr() if return_lse else None,
+                        status_ptr(dev))
+    st = _lib.lib().fa_prompt_attention(ctypes.byref(a), raw_stream(dev))
+    if st:
+        _lib.check(st, "fa_prompt_attention")
     return (out, lse) if return_lse else out
