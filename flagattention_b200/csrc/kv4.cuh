@@ -16,12 +16,13 @@
 //   keys (A operand, rows = tokens r and r + 8): lane q of row t owns the
 //     words j = 4 i + q (dims 8 j .. 8 j + 7, in order, nibble n = dim 8 j +
 //     n), adjacent in memory; rows of more than 128 dims are cut into planes
-//     of 128.
+//     of 128;
 //   values (A operand of V^T P, columns = tokens 2q, 2q + 1, 2q + 8, 2q + 9):
-//     lane (r, q) owns word (u, r) of each of its four tokens; the nibbles of
-//     word (u, r) are dims 64 u + 32 p + 4 r + i with p = (n >> 1) & 1, i =
-//     (n & 1) + 2 * (n >> 2), which keeps every m16 tile of dims inside one
-//     group of 32.  16-byte planes of [r][q][4 words].
+//     a 16-bit unit is four codes of one token, and a word is the same unit of
+//     two adjacent tokens, so a code and its neighbour token's code lie 16 bits
+//     apart.  Lane (r, q) owns words (pair, u, half): nibble n is dim 64 u + 32
+//     (n >> 1) + 4 r + 2 half + (n & 1), which keeps every m16 tile of dims
+//     inside one group of 32.  16-byte planes of [r][q][4 words].
 #pragma once
 
 #include "common.cuh"
@@ -45,13 +46,13 @@ __host__ __device__ constexpr int key_word(int t, int j) {
   const int plane = j / (kPlaneDims / 8), jj = j % (kPlaneDims / 8);
   return plane * (kTileTokens * kPlaneDims / 2) + t * (kPlaneDims / 2) + ((jj % 4) * kW + jj / 4) * 4;
 }
-// Byte offset of value word (u, r) of token t (inside the tile's value codes).
+// Byte offset of the 16-bit value unit (u, r, half) of token t (inside the
+// tile's value codes).
 template <int kD>
-__host__ __device__ constexpr int value_word(int t, int u, int r) {
+__host__ __device__ constexpr int value_unit(int t, int u, int r, int half) {
   constexpr int kU = kD / 64;
-  const int q = (t % 8) / 2, slot = (t % 2) + 2 * (t / 8);
-  const int idx = slot * kU + u;
-  return (idx / 4) * 512 + (r * 4 + q) * 16 + (idx % 4) * 4;
+  const int q = (t % 8) / 2, idx = ((t / 8) * kU + u) * 2 + half;
+  return (idx / 4) * 512 + (r * 4 + q) * 16 + (idx % 4) * 4 + (t % 2) * 2;
 }
 
 // Where a pool slot (block * block_size + offset) lives.

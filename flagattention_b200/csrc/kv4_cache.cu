@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
       word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
     }
   }
-  // value words gather four dims from each 32-dim half of their 64
+  // the units (u, r, 0 / 1) gather four dims from each 32-dim half of their 64
   const int r = j % 8;
   const uint32_t w0 = __shfl_sync(0xffffffffu, word, (j & ~7) + r / 2, kSeg);
   const uint32_t w1 = __shfl_sync(0xffffffffu, word, (j & ~7) + 4 + r / 2, kSeg);
@@ -99,11 +99,15 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
   const int64_t block = slot / pool.block_size;
   const int off = static_cast<int>(slot % pool.block_size), t = off % kTileTokens;
   uint8_t *tile = pool.tile(block, head, off / kTileTokens);
-  if (is_v)  // bytes (w0 lo, w1 lo, w0 hi, w1 hi) of the chosen 16-bit halves
-    *reinterpret_cast<uint32_t *>(tile + code_bytes(kD) + value_word<kD>(t, j / 8, r)) =
-        __byte_perm(w0, w1, (r & 1) ? 0x7362 : 0x5140);
-  else
+  if (is_v) {  // byte `half` of the chosen 16-bit halves of w0, then of w1
+    const uint32_t w = __byte_perm(w0, w1, (r & 1) ? 0x7362 : 0x5140);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      *reinterpret_cast<uint16_t *>(tile + code_bytes(kD) + value_unit<kD>(t, j / 8, r, half)) =
+          static_cast<uint16_t>(w >> (16 * half));
+  } else {
     *reinterpret_cast<uint32_t *>(tile + key_word<kD>(t, j)) = word;
+  }
   if (j % kLanes == 0) {
     T pair[2] = {bad ? Elem<T>::from_f(NAN) : Elem<T>::from_f(lo),
                  bad ? Elem<T>::from_f(0.f) : scale};
@@ -129,16 +133,22 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
     const int64_t block = slot / pool.block_size;
     const int off = static_cast<int>(slot % pool.block_size), t = off % kTileTokens;
     const uint8_t *tile = pool.tile(block, head, off / kTileTokens);
-    word = *reinterpret_cast<const uint32_t *>(
-        is_v ? tile + code_bytes(kD) + value_word<kD>(t, j / 8, r) : tile + key_word<kD>(t, j));
+    if (is_v) {
+      const uint8_t *codes = tile + code_bytes(kD);
+      word = *reinterpret_cast<const uint16_t *>(codes + value_unit<kD>(t, j / 8, r, 0)) |
+             static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(
+                 codes + value_unit<kD>(t, j / 8, r, 1))) << 16;
+    } else {
+      word = *reinterpret_cast<const uint32_t *>(tile + key_word<kD>(t, j));
+    }
     const uint32_t pair = *reinterpret_cast<const uint32_t *>(
         tile + 2 * code_bytes(kD) + t * (8 * kGroups) + (is_v * kGroups + j / kLanes) * 4);
     const T *e = reinterpret_cast<const T *>(&pair);
     lo = Elem<T>::to_f(e[0]);
     s = Elem<T>::to_f(e[1]);
   }
-  // value words: dims 8 j .. + 3 are 16 bits of word (u, 2 (j % 4)), the next
-  // four of word (u, 2 (j % 4) + 1), in the 32-dim half p = (j / 4) % 2
+  // values: dims 8 j .. + 3 are one byte of both units of r = 2 (j % 4), the
+  // next four of r + 1; the byte is the 32-dim half p = (j / 4) % 2
   const uint32_t w0 = __shfl_sync(0xffffffffu, word, (j & ~7) + 2 * (j % 4), kSeg);
   const uint32_t w1 = __shfl_sync(0xffffffffu, word, (j & ~7) + 2 * (j % 4) + 1, kSeg);
   if (!inside) return;

@@ -10,17 +10,26 @@
 // Byte-bound: a token and kv head is D + 8 D / G bytes (144 at D = 128, G =
 // 64; 512 in 16 bits).  At the measured copy rate an SM takes about 23 bytes a
 // cycle, one 16-token tile of 2304 bytes per 100 cycles, in which its four
-// schedulers issue 400 warp instructions: the instruction count per tile is
-// the second bound.  mma.sync m16n8k16 fits that: tokens (S = K Q^T) or dims
-// (O^T = V^T P) are the 16 rows, up to 8 heads the columns, codes come straight
-// from 16-byte shared-memory loads into A fragments (a shift and a three-input
-// logic operation make two 16-bit floats 16 + c from two codes), and P moves
-// between the two products in registers (movmatrix).  tcgen05 would need the
-// expanded operand written to shared memory first, 4x the bytes of the codes.
+// schedulers issue 400 warp instructions and its integer pipes 200: the
+// instruction count per tile is the second bound.  mma.sync m16n8k16 (f16)
+// fits that: tokens (S = K Q^T) or dims (O^T = V^T P) are the 16 rows, up to 8
+// heads the columns, codes come straight from 16-byte shared-memory loads into
+// A fragments, and P moves between the two products in registers (movmatrix).
+// tcgen05 would need the expanded operand written to shared memory first, 4x
+// the bytes of the codes.
 //
-// The "16 +" is taken out exactly where it is cheap: with q_i = sum_{d in i}
-// q_d,  sum (16 + c) q = sum c q + 16 q_i (folded into the lo term), and for
-// the values 16 * sum_t P'_t, accumulated in f32 next to the lo term.
+// A code becomes an operand with one AND and no conversion: four bits at the
+// bottom of a 16-bit half are the f16 subnormal c * 2^-24, the next four are
+// 16 c * 2^-24, both exact in the product; the word's upper codes need one
+// shift for four.  2^24 and the factor 16 of every other dim are powers of two
+// folded into Q and into the output.  Measured against two instructions a pair
+// for the normal numbers 16 + c (shift, AND-OR) and bf16 operands: 144 us ->
+// see the table at the end of the file's kernel.
+//
+// f16 operands hold Q and P' = p * s exactly enough because both are brought
+// near the top of its range by a power of two: Q by its row's largest
+// magnitude (bf16 and f16 queries then lose nothing above 2^-27 of it), P' by
+// the largest value scale a warp has met.
 //
 // Four warps of a CTA share a piece (a run of 64-token blocks of one entry),
 // one 16-token tile each per block; a warp has its own ring of tiles filled by
@@ -40,7 +49,11 @@ Pool pool_of(const fa_kv4_cache *c);
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlockTokens = kWarps * kTileTokens;  // schedule unit: one tile per warp
-constexpr float kRescaleThreshold = 8.0f;           // log2 units (factor 256)
+constexpr float kRescaleThreshold = 8.0f;           // log2 units (factor 256): p <= 2^8
+constexpr float kValueScaleTop = 64.f;              // normalised value scales: P' <= 2^14
+// Stands for "no key yet" as a running maximum: below every finite score, and
+// finite, so that differences with it need no special case.
+constexpr float kNoMax = -3.0e38f;
 
 struct Params {
   const void *q;
@@ -154,33 +167,24 @@ __device__ __noinline__ void compute_share(const Params &p, long long *scan, Con
   __syncthreads();
 }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  return __byte_perm(a, b, sel);
+// Operand pair k (0..3) of w: nibble k of both 16-bit halves as f16 numbers c *
+// 2^-24 (k even) or 16 c * 2^-24 (k odd); w8 = w >> 8.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int k) {
+  return (k < 2 ? w : w8) & ((k & 1) ? 0x00f000f0u : 0x000f000fu);
 }
-// Nibbles k (0..3) of both 16-bit halves of w as two floats 16 + c: the codes
-// land in the top mantissa bits under the exponent of 16.
-template <typename T>
-__device__ __forceinline__ uint32_t codes16(uint32_t w, int k) {
-  constexpr int kTop = std::is_same<T, __half>::value ? 6 : 3;  // mantissa bits below the code
-  constexpr uint32_t kMask = 0x000f000fu << kTop;
-  constexpr uint32_t kSixteen = std::is_same<T, __half>::value ? 0x4c004c00u : 0x41804180u;
-  const int sh = kTop - 4 * k;
-  return ((sh >= 0 ? w << sh : w >> -sh) & kMask) | kSixteen;
-}
-template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Exponent field of |x| unbiased (-127 for zero and subnormals, 128 for an
+// infinity), and 2^e for -126 <= e <= 127.
+__device__ __forceinline__ int exponent_of(float x) {
+  return static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 // 8x8 transpose across the warp: lane l held row l / 4, columns 2 (l % 4), +1.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -306,47 +310,71 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     };
     for (int i = 0; i < min(n, kStages); ++i) issue(i);
 
-    // Q as the B operand: pair k of word i holds dims 32 i + 8 q + {k, k + 4}
-    // of head r of each 8-head tile
+    // Q as the B operand, times a power of two that brings the row's largest
+    // magnitude to [2^13, 2^14): pair k of word i holds dims 32 i + 8 q + {k,
+    // k + 4} of head r of each 8-head tile, over 16 for odd k
     uint32_t qf[kNT][kW][4];
-    float qs[kNT][kGroups][2];  // sum of q over a group, heads 2 q and 2 q + 1
+    float qs[kNT][kGroups][2];  // 2^-24 * sum of q' over a group, heads 2 q, 2 q + 1
+    float unit[kNT][2];         // log2 score per unit of the products' sum, ditto
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
       const bool live = t * 8 + r < heads;
       const uint4 *src = reinterpret_cast<const uint4 *>(
           static_cast<const T *>(p.q) + b * p.q_sb +
           static_cast<int64_t>(kvh * p.group + h0 + (live ? t * 8 + r : 0)) * p.q_sh);
+      uint4 v[kW];
+      float mag = 0.f;
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        v[i] = live ? __ldg(src + 4 * i + q) : make_uint4(0u, 0u, 0u, 0u);
+        const T *el = reinterpret_cast<const T *>(&v[i]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) mag = fmaxf(mag, fabsf(Elem<T>::to_f(el[d])));
+      }
+      mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
+      mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
+      const int f = max(exponent_of(mag) - 13, -100);
+      const float norm = pow2(-f);
       float sum[kGroups];
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) sum[g] = 0.f;
 #pragma unroll
       for (int i = 0; i < kW; ++i) {
-        const uint4 v = live ? __ldg(src + 4 * i + q) : make_uint4(0u, 0u, 0u, 0u);
-        qf[t][i][0] = prmt(v.x, v.z, 0x5410);
-        qf[t][i][1] = prmt(v.x, v.z, 0x7632);
-        qf[t][i][2] = prmt(v.y, v.w, 0x5410);
-        qf[t][i][3] = prmt(v.y, v.w, 0x7632);
-        const T *el = reinterpret_cast<const T *>(&v);
+        const T *el = reinterpret_cast<const T *>(&v[i]);
+        float x[8];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) sum[32 * i / kG] += Elem<T>::to_f(el[d]);
+        for (int d = 0; d < 8; ++d) {
+          x[d] = Elem<T>::to_f(el[d]) * norm;
+          sum[32 * i / kG] += x[d];
+        }
+        qf[t][i][0] = Elem<__half>::pack2(x[0], x[4]);
+        qf[t][i][1] = Elem<__half>::pack2(x[1] * 0.0625f, x[5] * 0.0625f);
+        qf[t][i][2] = Elem<__half>::pack2(x[2], x[6]);
+        qf[t][i][3] = Elem<__half>::pack2(x[3] * 0.0625f, x[7] * 0.0625f);
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+        sum[g] *= 0x1p-24f;
         qs[t][g][0] = __shfl_sync(0xffffffffu, sum[g], 8 * q);
         qs[t][g][1] = __shfl_sync(0xffffffffu, sum[g], 8 * q + 4);
       }
+      const float un = p.scale_log2 * pow2(f + 12) * 4096.f;  // scale * 2^(f + 24)
+      unit[t][0] = __shfl_sync(0xffffffffu, un, 8 * q);
+      unit[t][1] = __shfl_sync(0xffffffffu, un, 8 * q + 4);
     }
 
     // running state; lanes of equal q agree on m; l and extra are partial sums
-    // over the lane's tokens
+    // over the lane's tokens; vnorm normalises the value scales (warp-uniform)
+    float vnorm = 1.f;
+    bool fresh = true;
     float m[kNT][2], l[kNT][2], extra[kNT][kGroups][2], o[kNT][kD / 16][4];
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        m[t][h] = -INFINITY;
+        m[t][h] = kNoMax;
         l[t][h] = 0.f;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) extra[t][g][h] = 0.f;
@@ -386,10 +414,6 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
         lds(tile + 2 * code_bytes(kD) + (r + 8) * 8 * kGroups, scb);
         float s[kNT][4];
 #pragma unroll
-        for (int t = 0; t < kNT; ++t)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[t][c] = 0.f;
-#pragma unroll
         for (int g = 0; g < kGroups; ++g) {
           float acc[kNT][4];
 #pragma unroll
@@ -397,45 +421,78 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[t][c] = 0.f;
 #pragma unroll
-          for (int i2 = g * kW / kGroups; i2 < (g + 1) * kW / kGroups; ++i2)
+          for (int i2 = g * kW / kGroups; i2 < (g + 1) * kW / kGroups; ++i2) {
+            const uint32_t ka8 = ka[i2] >> 8, kb8 = kb[i2] >> 8;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-              const uint32_t a0 = codes16<T>(ka[i2], 2 * ks), a1 = codes16<T>(kb[i2], 2 * ks),
-                             a2 = codes16<T>(ka[i2], 2 * ks + 1),
-                             a3 = codes16<T>(kb[i2], 2 * ks + 1);
+              const uint32_t a0 = code_pair(ka[i2], ka8, 2 * ks), a1 = code_pair(kb[i2], kb8, 2 * ks),
+                             a2 = code_pair(ka[i2], ka8, 2 * ks + 1),
+                             a3 = code_pair(kb[i2], kb8, 2 * ks + 1);
 #pragma unroll
               for (int t = 0; t < kNT; ++t)
-                mma16816<T>(acc[t], a0, a1, a2, a3, qf[t][i2][2 * ks], qf[t][i2][2 * ks + 1]);
+                mma16816(acc[t], a0, a1, a2, a3, qf[t][i2][2 * ks], qf[t][i2][2 * ks + 1]);
             }
+          }
           float loa, sa, lob, sb;
           pair_of<T>(sca[g], loa, sa);
           pair_of<T>(scb[g], lob, sb);
-          const float ca = fmaf(-16.f, sa, loa), cb = fmaf(-16.f, sb, lob);
 #pragma unroll
-          for (int t = 0; t < kNT; ++t) {
-            s[t][0] += fmaf(sa, acc[t][0], ca * qs[t][g][0]);
-            s[t][1] += fmaf(sa, acc[t][1], ca * qs[t][g][1]);
-            s[t][2] += fmaf(sb, acc[t][2], cb * qs[t][g][0]);
-            s[t][3] += fmaf(sb, acc[t][3], cb * qs[t][g][1]);
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float xa = fmaf(sa, acc[t][h], loa * qs[t][g][h]);
+              const float xb = fmaf(sb, acc[t][h + 2], lob * qs[t][g][h]);
+              s[t][h] = g == 0 ? xa : s[t][h] + xa;
+              s[t][h + 2] = g == 0 ? xb : s[t][h + 2] + xb;
+            }
+        }
+        float vla[kGroups], vsa[kGroups], vlb[kGroups], vsb[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          pair_of<T>(sca[kGroups + g], vla[g], vsa[g]);
+          pair_of<T>(scb[kGroups + g], vlb[g], vsb[g]);
+        }
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[t][c] *= unit[t][c & 1];
+        if (left < kTileTokens) {  // tokens past the end: any bits, so select
+          const bool la = r < left, lb = r + 8 < left;
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[t][h] = la ? s[t][h] : -INFINITY;
+              s[t][h + 2] = lb ? s[t][h + 2] : -INFINITY;
+            }
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            vla[g] = la ? vla[g] : 0.f;
+            vsa[g] = la ? vsa[g] : 0.f;
+            vlb[g] = lb ? vlb[g] : 0.f;
+            vsb[g] = lb ? vsb[g] : 0.f;
           }
         }
         // ------------------------------------------------- running softmax
-        const bool la = r < left, lb = r + 8 < left;  // tokens past the end: any bits
-        float top = -INFINITY;  // largest excess over the running maximum
+        float top = -INFINITY, big = 0.f;  // excess over the maxima; largest value scale
 #pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          s[t][0] = la ? s[t][0] * p.scale_log2 : -INFINITY;
-          s[t][1] = la ? s[t][1] * p.scale_log2 : -INFINITY;
-          s[t][2] = lb ? s[t][2] * p.scale_log2 : -INFINITY;
-          s[t][3] = lb ? s[t][3] * p.scale_log2 : -INFINITY;
+        for (int t = 0; t < kNT; ++t)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float mx = fmaxf(s[t][h], s[t][h + 2]);
-            top = fmaxf(top, m[t][h] == -INFINITY ? (mx == -INFINITY ? -INFINITY : INFINITY)
-                                                  : mx - m[t][h]);
+          for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(s[t][h], s[t][h + 2]) - m[t][h]);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) big = fmax3(big, vsa[g], vsb[g]);
+        if (__any_sync(0xffffffffu, top > kRescaleThreshold || big * vnorm > kValueScaleTop)) {
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1)
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+          float shrink = 1.f;  // of what the value products hold
+          if (fresh || big * vnorm > kValueScaleTop) {
+            fresh = false;
+            // scales up to `big` land below 32: room for the next to be larger
+            const float next = pow2(min(max(4 - exponent_of(big), -100), 100));
+            shrink = next / vnorm;
+            vnorm = next;
           }
-        }
-        if (__any_sync(0xffffffffu, top > kRescaleThreshold)) {
 #pragma unroll
           for (int t = 0; t < kNT; ++t)
 #pragma unroll
@@ -445,60 +502,48 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
               for (int off = 4; off < 32; off <<= 1)
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
               const float mn = fmaxf(m[t][h], mx);
-              const float alpha = m[t][h] == -INFINITY ? 0.f : fast_exp2(m[t][h] - mn);
+              const float alpha = fast_exp2(m[t][h] - mn);
               m[t][h] = mn;
               l[t][h] *= alpha;
 #pragma unroll
               for (int g = 0; g < kGroups; ++g) extra[t][g][h] *= alpha;
 #pragma unroll
               for (int i2 = 0; i2 < kD / 16; ++i2) {
-                o[t][i2][h] *= alpha;
-                o[t][i2][h + 2] *= alpha;
+                o[t][i2][h] *= alpha * shrink;
+                o[t][i2][h + 2] *= alpha * shrink;
               }
             }
         }
         // -------------------------------------------------------- P and P V
-        uint32_t pf[kNT][kGroups][kSplitP ? 4 : 2];  // B operands (hi, then lo parts)
+        uint32_t pf[kNT][kGroups][kSplitP ? 4 : 2];  // B operands (high, then low parts)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          vsa[g] *= vnorm;
+          vsb[g] *= vnorm;
+        }
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
-          const float ma = m[t][0] == -INFINITY ? 0.f : m[t][0];
-          const float mb = m[t][1] == -INFINITY ? 0.f : m[t][1];
-          const float p0 = fast_exp2(s[t][0] - ma), p1 = fast_exp2(s[t][1] - mb);
-          const float p2 = fast_exp2(s[t][2] - ma), p3 = fast_exp2(s[t][3] - mb);
+          const float p0 = fast_exp2(s[t][0] - m[t][0]), p1 = fast_exp2(s[t][1] - m[t][1]);
+          const float p2 = fast_exp2(s[t][2] - m[t][0]), p3 = fast_exp2(s[t][3] - m[t][1]);
           l[t][0] += p0 + p2;
           l[t][1] += p1 + p3;
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) {
-            float loa, sa, lob, sb;
-            pair_of<T>(sca[kGroups + g], loa, sa);
-            pair_of<T>(scb[kGroups + g], lob, sb);
-            loa = la ? loa : 0.f;  // select: scales past the end may be NaN
-            sa = la ? sa : 0.f;
-            lob = lb ? lob : 0.f;
-            sb = lb ? sb : 0.f;
-            const float x0 = p0 * sa, x1 = p1 * sa, x2 = p2 * sb, x3 = p3 * sb;
-            const uint32_t wa = Elem<__nv_bfloat16>::pack2(x0, x1);
-            const uint32_t wb = Elem<__nv_bfloat16>::pack2(x2, x3);
-            float y0 = __uint_as_float(wa << 16), y1 = __uint_as_float(wa & 0xffff0000u);
-            float y2 = __uint_as_float(wb << 16), y3 = __uint_as_float(wb & 0xffff0000u);
+            const float x0 = p0 * vsa[g], x1 = p1 * vsa[g], x2 = p2 * vsb[g], x3 = p3 * vsb[g];
+            const uint32_t wa = Elem<__half>::pack2(x0, x1), wb = Elem<__half>::pack2(x2, x3);
             pf[t][g][0] = transpose8(wa);
             pf[t][g][1] = transpose8(wb);
             if constexpr (kSplitP) {
-              const uint32_t va = Elem<__nv_bfloat16>::pack2(x0 - y0, x1 - y1);
-              const uint32_t vb = Elem<__nv_bfloat16>::pack2(x2 - y2, x3 - y3);
-              pf[t][g][2] = transpose8(va);
-              pf[t][g][3] = transpose8(vb);
-              y0 += __uint_as_float(va << 16);
-              y1 += __uint_as_float(va & 0xffff0000u);
-              y2 += __uint_as_float(vb << 16);
-              y3 += __uint_as_float(vb & 0xffff0000u);
+              const __half2 ha = *reinterpret_cast<const __half2 *>(&wa);
+              const __half2 hb = *reinterpret_cast<const __half2 *>(&wb);
+              pf[t][g][2] = transpose8(Elem<__half>::pack2(x0 - __low2float(ha), x1 - __high2float(ha)));
+              pf[t][g][3] = transpose8(Elem<__half>::pack2(x2 - __low2float(hb), x3 - __high2float(hb)));
             }
-            // the lo term, and the 16 that every code carries
-            extra[t][g][0] += fmaf(p0, loa, p2 * lob) - 16.f * (y0 + y2);
-            extra[t][g][1] += fmaf(p1, loa, p3 * lob) - 16.f * (y1 + y3);
+            extra[t][g][0] = fmaf(p0, vla[g], fmaf(p2, vlb[g], extra[t][g][0]));
+            extra[t][g][1] = fmaf(p1, vla[g], fmaf(p3, vlb[g], extra[t][g][1]));
           }
         }
-        uint32_t vw[4 * kU];  // [token slot][u]
+        uint32_t vw[4 * kU];  // [token pair][u][half]
 #pragma unroll
         for (int pl = 0; pl < kU; ++pl) {
           uint32_t w[4];
@@ -508,21 +553,19 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          const uint32_t lo01 = prmt(vw[u], vw[kU + u], 0x5410);
-          const uint32_t hi01 = prmt(vw[u], vw[kU + u], 0x7632);
-          const uint32_t lo23 = prmt(vw[2 * kU + u], vw[3 * kU + u], 0x5410);
-          const uint32_t hi23 = prmt(vw[2 * kU + u], vw[3 * kU + u], 0x7632);
+          const uint32_t w0 = vw[2 * u], w1 = vw[2 * u + 1], w2 = vw[2 * kU + 2 * u],
+                         w3 = vw[2 * kU + 2 * u + 1];
+          const uint32_t s0 = w0 >> 8, s1 = w1 >> 8, s2 = w2 >> 8, s3 = w3 >> 8;
 #pragma unroll
-          for (int e4 = 0; e4 < 4; ++e4) {
-            const int g = (64 * u + 32 * (e4 >> 1)) / kG;
-            using B = __nv_bfloat16;
-            const uint32_t a0 = codes16<B>(lo01, e4), a1 = codes16<B>(hi01, e4),
-                           a2 = codes16<B>(lo23, e4), a3 = codes16<B>(hi23, e4);
+          for (int k = 0; k < 4; ++k) {
+            const int g = (64 * u + 32 * (k >> 1)) / kG;
+            const uint32_t a0 = code_pair(w0, s0, k), a1 = code_pair(w1, s1, k),
+                           a2 = code_pair(w2, s2, k), a3 = code_pair(w3, s3, k);
 #pragma unroll
             for (int t = 0; t < kNT; ++t) {
-              mma16816<B>(o[t][4 * u + e4], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
+              mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
               if constexpr (kSplitP)
-                mma16816<B>(o[t][4 * u + e4], a0, a1, a2, a3, pf[t][g][2], pf[t][g][3]);
+                mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][2], pf[t][g][3]);
             }
           }
         }
@@ -555,22 +598,24 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
 #pragma unroll
           for (int pp = 0; pp < 2; ++pp) {
             const float ex = extra[t][(64 * u + 32 * pp) / kG][h];
+            const float even = 0x1p24f / vnorm, odd = 0x1p20f / vnorm;
             const float *oa = o[t][4 * u + 2 * pp], *ob = o[t][4 * u + 2 * pp + 1];
-            // nibbles 2 pp and 2 pp + 1 of rows m < 8, then of rows m >= 8
+            // codes 2 pp and 2 pp + 1 of rows m < 8, then of rows m >= 8
             *reinterpret_cast<float4 *>(row + 64 * u + 32 * pp + 4 * r) =
-                make_float4(oa[h] + ex, ob[h] + ex, oa[h + 2] + ex, ob[h + 2] + ex);
+                make_float4(fmaf(oa[h], even, ex), fmaf(ob[h], odd, ex), fmaf(oa[h + 2], even, ex),
+                            fmaf(ob[h + 2], odd, ex));
           }
       }
     __syncthreads();
     constexpr int kPer = kThreads / kHeads;       // threads of one head's row
     const int hh = threadIdx.x / kPer, part = threadIdx.x % kPer;
-    float M = -INFINITY;
+    float M = kNoMax;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ctl.m[w][hh]);
     float L = 0.f, f[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      f[w] = ctl.m[w][hh] == -INFINITY ? 0.f : fast_exp2(ctl.m[w][hh] - M);
+      f[w] = fast_exp2(ctl.m[w][hh] - M);
       L += ctl.l[w][hh] * f[w];
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;  // a NaN stays one
