@@ -97,7 +97,6 @@ struct Share {
 
 struct Control {
   uint64_t full[kWarps][8];
-  int valid[kWarps][8];  // the stage holds a tile of the pool
   long long warp_sum[kWarps];
   Share share;
   float m[kWarps][16], l[kWarps][16];
@@ -250,7 +249,10 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
   const Share &sh = ctl.share;
   volatile int *abort_flag = &ctl.abort_flag;
   const uint32_t ring = smem_u32(smem) + warp * kStages * kTileB;
-  uint32_t filled = 0, used = 0;  // tiles of this warp's ring so far
+  const uint32_t full0 = smem_u32(&ctl.full[warp][0]);
+  uint32_t fill_stage = 0, use_stage = 0, use_phase = 0;  // this warp's ring
+  uint32_t ahead = 0, valid_bits = 0;  // tiles issued and not yet used; bit i: the i-th newest
+                                       // issued one lies in the pool
   float *obuf = reinterpret_cast<float *>(smem);
 
   long long x = sh.x_lo;
@@ -282,31 +284,35 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     int n = j1 - j0;
     while (n > 0 && (j0 + n - 1) * kWarps + warp >= tiles_end) --n;
 
-    // tiles are issued kStages ahead; lane i keeps the page of tile page0 + i
+    // tiles are issued kStages ahead; every 32 tiles lane i looks up the pool
+    // tile of the warp's i-th next one (-1: block outside the pool)
     const int tiles_per_page = p.pool.block_size / kTileTokens;
-    int page0 = -32, my_page = -1;
+    int my_tile = -1;
     auto issue = [&](int i) {  // i-th tile of the piece
-      const int tile = (j0 + i) * kWarps + warp;
-      if (i >= page0 + 32) {
-        page0 = i;
+      if ((i & 31) == 0) {
         const int mine = (j0 + i + lane) * kWarps + warp;
-        my_page = mine < tiles_end
-                      ? __ldg(p.block_table + b * p.bt_stride + mine / tiles_per_page) : -1;
+        my_tile = -1;
+        if (mine < tiles_end) {
+          const int pg = mine / tiles_per_page;
+          const int page = __ldg(p.block_table + b * p.bt_stride + pg);
+          if (page >= 0 && page < p.num_blocks)
+            my_tile = (page * p.hkv + kvh) * tiles_per_page + (mine - pg * tiles_per_page);
+        }
       }
-      const int page = __shfl_sync(0xffffffffu, my_page, i - page0);
-      const uint32_t st = filled % kStages;
+      const int at = __shfl_sync(0xffffffffu, my_tile, i & 31);
+      valid_bits = (valid_bits << 1) | (at >= 0 ? 1u : 0u);
       if (lane == 0) {
-        const uint32_t bar = smem_u32(&ctl.full[warp][st]);
-        const bool ok = page >= 0 && page < p.num_blocks;  // others hold no token
-        ctl.valid[warp][st] = ok;
-        if (ok) {
+        const uint32_t bar = full0 + 8 * fill_stage;
+        if (at >= 0) {
           mbar_arrive_expect_tx(bar, kTileB);
-          bulk_load(ring + st * kTileB, p.pool.tile(page, kvh, tile % tiles_per_page), kTileB, bar);
+          bulk_load(ring + fill_stage * kTileB, p.pool.data + static_cast<int64_t>(at) * kTileB,
+                    kTileB, bar);
         } else {
           mbar_arrive(bar);
         }
       }
-      ++filled;
+      fill_stage = fill_stage + 1 == kStages ? 0 : fill_stage + 1;
+      ++ahead;
     };
     for (int i = 0; i < min(n, kStages); ++i) issue(i);
 
@@ -386,14 +392,17 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     }
 
     for (int i = 0; i < n; ++i) {
-      const uint32_t st = used % kStages;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.full[warp][st]), (used / kStages) & 1u,
-                                             abort_flag, p.status, kDevTimeoutProducer)))
+      const uint32_t bar = full0 + 8 * use_stage;
+      if (!__all_sync(0xffffffffu, mbar_probe(bar, use_phase)) &&
+          !__all_sync(0xffffffffu,
+                      mbar_wait(bar, use_phase, abort_flag, p.status, kDevTimeoutProducer)))
         break;  // the abort flag is set: copies in flight are waited for at the end
-      ++used;
-      const uint32_t tile = ring + st * kTileB;
+      const uint32_t tile = ring + use_stage * kTileB;
+      use_stage = use_stage + 1 == kStages ? 0 : use_stage + 1;
+      use_phase ^= use_stage == 0 ? 1u : 0u;
+      --ahead;
+      const bool valid = (valid_bits >> ahead) & 1u;
       const int left = len - ((j0 + i) * kWarps + warp) * kTileTokens;  // live tokens from row 0
-      const bool valid = *const_cast<volatile int *>(&ctl.valid[warp][st]) != 0;
       if (valid) {
         // ---------------------------------------------------------- scores
         uint32_t ka[kW], kb[kW];
@@ -440,10 +449,10 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
           for (int t = 0; t < kNT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float xa = fmaf(sa, acc[t][h], loa * qs[t][g][h]);
-              const float xb = fmaf(sb, acc[t][h + 2], lob * qs[t][g][h]);
-              s[t][h] = g == 0 ? xa : s[t][h] + xa;
-              s[t][h + 2] = g == 0 ? xb : s[t][h + 2] + xb;
+              s[t][h] = fmaf(sa, acc[t][h], g == 0 ? loa * qs[t][g][h]
+                                                   : fmaf(loa, qs[t][g][h], s[t][h]));
+              s[t][h + 2] = fmaf(sb, acc[t][h + 2], g == 0 ? lob * qs[t][g][h]
+                                                           : fmaf(lob, qs[t][g][h], s[t][h + 2]));
             }
         }
         float vla[kGroups], vsa[kGroups], vlb[kGroups], vsb[kGroups];
@@ -652,8 +661,11 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
   // the CTA's shared memory is given back
   if (*abort_flag) {
     volatile int never = 0;
-    for (; used < filled; ++used)
-      mbar_wait(smem_u32(&ctl.full[warp][used % kStages]), (used / kStages) & 1u, &never, nullptr, 0);
+    for (; ahead > 0; --ahead) {
+      mbar_wait(full0 + 8 * use_stage, use_phase, &never, nullptr, 0);
+      use_stage = use_stage + 1 == kStages ? 0 : use_stage + 1;
+      use_phase ^= use_stage == 0 ? 1u : 0u;
+    }
   }
 }
 
@@ -755,6 +767,10 @@ int validate_attention(const fa_kv4_attention_args *a) {
   if (a->batch < 0 || a->num_q_heads <= 0 || a->num_q_heads % a->cache.num_kv_heads)
     return record_error(FA_ERR_INVALID_ARGUMENT,
                         "kv4 attention: query heads must be a multiple of the cache's kv heads");
+  int64_t bytes = 0;
+  fa_kv4_cache_bytes(&a->cache, &bytes);
+  if (bytes / tile_bytes(a->cache.head_size, a->cache.head_size / a->cache.group_size) > INT32_MAX)
+    return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: pool of more than 2^31 tiles");
   if (a->bt_width < 0 || a->bt_stride < 0)
     return record_error(FA_ERR_INVALID_ARGUMENT, "kv4 attention: block table shape");
   if (!(a->scale > 0.f) || std::isinf(a->scale))
