@@ -99,7 +99,7 @@ class Kv4AttentionArgs(ctypes.Structure):
         ("block_table", _vp), ("bt_stride", _i64), ("bt_width", _i32), ("seq_lens", _vp),
         ("batch", _i32), ("num_q_heads", _i32), ("scale", _f32),
         ("o", _vp), ("o_stride_b", _i64), ("o_stride_h", _i64),
-        ("lse", _vp), ("part_o", _vp), ("part_lse", _vp), ("merge", _vp), ("status", _vp),
+        ("lse", _vp), ("part_o", _vp), ("part_lse", _vp), ("merge", _vp),
     ]
 
 

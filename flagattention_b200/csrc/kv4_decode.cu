@@ -32,8 +32,8 @@
 // the largest value scale a warp has met.
 //
 // Four warps of a CTA share a piece (a run of 64-token blocks of one entry),
-// one 16-token tile each per block; a warp has its own ring of tiles filled by
-// bulk copies.  The pieces are equal shares of all entries' blocks, cut from
+// one 16-token tile each per block, loaded straight into registers one tile
+// ahead while L2 fetches further ones.  The pieces are equal shares of all entries' blocks, cut from
 // the sequence lengths by every CTA; split entries are merged by a second
 // kernel launched as a programmatic dependent.
 #include "kv4.cuh"
@@ -73,7 +73,6 @@ struct Params {
   float *part_o;    // [slot][8 * kNT][kD]
   float *part_lse;  // [slot][8 * kNT]
   int4 *merge;      // per entry: {first slot or -1, first later slot, later slots, 0}
-  int *status;
 };
 
 template <int kD, int kGroups, int kNT>
@@ -82,13 +81,13 @@ struct Plan {
   static constexpr int kHeads = 8 * kNT;
   static constexpr int kORow = kD + 4;  // f32 row pitch of the merge buffer (bank spread)
   static constexpr int kMergeBytes = kWarps * kHeads * kORow * 4;
-  static constexpr int kMinBytes = kMergeBytes > 46080 ? kMergeBytes : 46080;
-  static constexpr int kStagesFit = kMinBytes / (kWarps * kTileB);
-  static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
-  static constexpr int kRing = kWarps * kStages * kTileB;
-  static constexpr int kBuf = kRing > kMergeBytes ? kRing : kMergeBytes;
-  static_assert(kStages >= 2, "ring");
 };
+// Shared memory holds the schedule's scan (batch + 1 int64), then the merge
+// buffer: sequences a call can take.
+constexpr int kMaxBatch = 6000;
+// Tiles a warp asks L2 to fetch ahead of the one it loads: 16 warps x 6 x 2304
+// bytes in flight cover the latency of HBM (44 KB per SM) several times over.
+constexpr int kAhead = 6;
 
 struct Share {
   long long a0, a1, x_lo, total;
@@ -96,11 +95,9 @@ struct Share {
 };
 
 struct Control {
-  uint64_t full[kWarps][8];
   long long warp_sum[kWarps];
   Share share;
   float m[kWarps][16], l[kWarps][16];
-  int abort_flag;
 };
 
 __device__ __forceinline__ int seq_len_of(const Params &p, int b) {
@@ -190,19 +187,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+// Cache words are read once: no L1 allocation.
 template <int kWords>
-__device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[kWords]) {
-  static_assert(kWords == 1 || kWords == 2 || kWords % 4 == 0, "vector width");
-  if constexpr (kWords == 1)
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
-  else if constexpr (kWords == 2)
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+__device__ __forceinline__ void load_words(const uint8_t *src, uint32_t *w) {
+  static_assert(kWords == 2 || kWords % 4 == 0, "vector width");
+  if constexpr (kWords == 2)
+    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];"
+                 : "=r"(w[0]), "=r"(w[1])
+                 : "l"(src));
   else
 #pragma unroll
     for (int i = 0; i < kWords / 4; ++i)
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+      asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
-                   : "r"(addr + 16 * i));
+                   : "l"(src + 16 * i));
 }
 // A (lo, scale) pair of the cache.
 template <typename T>
@@ -212,15 +210,6 @@ __device__ __forceinline__ void pair_of(uint32_t w, float &lo, float &scale) {
   scale = Elem<T>::to_f(e[1]);
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
 template <typename T, int kD, int kGroups, int kNT>
 __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     kv4_decode_kernel(const __grid_constant__ Params p) {
@@ -228,31 +217,16 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
   constexpr int kG = kD / kGroups;
   constexpr int kW = kD / 32;   // key words of a lane and token
   constexpr int kU = kD / 64;   // value words of a lane and token
-  constexpr int kStages = PL::kStages, kTileB = PL::kTileB, kHeads = PL::kHeads;
+  constexpr int kTileB = PL::kTileB, kHeads = PL::kHeads;
   constexpr bool kSplitP = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Control ctl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
 
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < kWarps; ++w)
-      for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&ctl.full[w][s]), 1);
-    ctl.abort_flag = 0;
-    fence_barrier_init();
-  }
-  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   compute_share(p, reinterpret_cast<long long *>(smem), &ctl);
-  fence_proxy_async_smem();  // the ring overlays the scan
-  __syncthreads();
   const Share &sh = ctl.share;
-  volatile int *abort_flag = &ctl.abort_flag;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kTileB;
-  const uint32_t full0 = smem_u32(&ctl.full[warp][0]);
-  uint32_t fill_stage = 0, use_stage = 0, use_phase = 0;  // this warp's ring
-  uint32_t ahead = 0, valid_bits = 0;  // tiles issued and not yet used; bit i: the i-th newest
-                                       // issued one lies in the pool
   float *obuf = reinterpret_cast<float *>(smem);
 
   long long x = sh.x_lo;
@@ -284,37 +258,55 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     int n = j1 - j0;
     while (n > 0 && (j0 + n - 1) * kWarps + warp >= tiles_end) --n;
 
-    // tiles are issued kStages ahead; every 32 tiles lane i looks up the pool
-    // tile of the warp's i-th next one (-1: block outside the pool)
+    // every 32 tiles lane i looks up the pool tile of the warp's i-th next one
+    // (-1: past the end, or a block outside the pool), one batch ahead
     const int tiles_per_page = p.pool.block_size / kTileTokens;
-    int my_tile = -1;
-    auto issue = [&](int i) {  // i-th tile of the piece
-      if ((i & 31) == 0) {
-        const int mine = (j0 + i + lane) * kWarps + warp;
-        my_tile = -1;
-        if (mine < tiles_end) {
-          const int pg = mine / tiles_per_page;
-          const int page = __ldg(p.block_table + b * p.bt_stride + pg);
-          if (page >= 0 && page < p.num_blocks)
-            my_tile = (page * p.hkv + kvh) * tiles_per_page + (mine - pg * tiles_per_page);
-        }
-      }
-      const int at = __shfl_sync(0xffffffffu, my_tile, i & 31);
-      valid_bits = (valid_bits << 1) | (at >= 0 ? 1u : 0u);
-      if (lane == 0) {
-        const uint32_t bar = full0 + 8 * fill_stage;
-        if (at >= 0) {
-          mbar_arrive_expect_tx(bar, kTileB);
-          bulk_load(ring + fill_stage * kTileB, p.pool.data + static_cast<int64_t>(at) * kTileB,
-                    kTileB, bar);
-        } else {
-          mbar_arrive(bar);
-        }
-      }
-      fill_stage = fill_stage + 1 == kStages ? 0 : fill_stage + 1;
-      ++ahead;
+    auto look_up = [&](int i0) {
+      const int mine = (j0 + i0 + lane) * kWarps + warp;
+      if (mine >= tiles_end || i0 + lane >= n) return -1;
+      const int pg = mine / tiles_per_page;
+      const int page = __ldg(p.block_table + b * p.bt_stride + pg);
+      if (page < 0 || page >= p.num_blocks) return -1;
+      return (page * p.hkv + kvh) * tiles_per_page + (mine - pg * tiles_per_page);
     };
-    for (int i = 0; i < min(n, kStages); ++i) issue(i);
+    int tiles_a = look_up(0), tiles_b = n > 32 ? look_up(32) : -1;  // tiles base .. + 31, + 32 .. + 63
+    auto tile_at = [&](int i) {  // i: relative to the current batch of 32, 0 .. 63
+      return __shfl_sync(0xffffffffu, i < 32 ? tiles_a : tiles_b, i & 31);
+    };
+    auto prefetch = [&](int at) {
+      if (at >= 0 && lane == 0)
+        bulk_prefetch_l2(p.pool.data + static_cast<int64_t>(at) * kTileB, kTileB);
+    };
+    constexpr int kLaneWords = kW < 4 ? kW : 4;
+    constexpr int kRowBytes = 16 * kLaneWords;
+    const int key_off = r * kRowBytes + q * 4 * kLaneWords;  // row r + 8: + 8 * kRowBytes
+    uint32_t ka[kW] = {}, kb[kW] = {}, sca[2 * kGroups] = {}, scb[2 * kGroups] = {}, vw[4 * kU] = {};
+    auto load_keys = [&](const uint8_t *tile) {
+#pragma unroll
+      for (int pl = 0; pl < kW / kLaneWords; ++pl) {
+        const uint8_t *plane = tile + pl * (kTileTokens * kRowBytes) + key_off;
+        load_words<kLaneWords>(plane, ka + pl * kLaneWords);
+        load_words<kLaneWords>(plane + 8 * kRowBytes, kb + pl * kLaneWords);
+      }
+    };
+    auto load_scales = [&](const uint8_t *tile) {  // all pairs of tokens r, r + 8
+      load_words<2 * kGroups>(tile + 2 * code_bytes(kD) + r * 8 * kGroups, sca);
+      load_words<2 * kGroups>(tile + 2 * code_bytes(kD) + (r + 8) * 8 * kGroups, scb);
+    };
+    auto load_values = [&](const uint8_t *tile) {  // [token pair][u][half]
+#pragma unroll
+      for (int pl = 0; pl < kU; ++pl)
+        load_words<4>(tile + code_bytes(kD) + pl * 512 + lane * 16, vw + 4 * pl);
+    };
+    int at = tile_at(0);
+    if (at >= 0) {
+      const uint8_t *tile = p.pool.data + static_cast<int64_t>(at) * kTileB;
+      load_keys(tile);
+      load_scales(tile);
+      load_values(tile);
+    }
+#pragma unroll 1
+    for (int i = 1; i < kAhead; ++i) prefetch(tile_at(i));
 
     // Q as the B operand, times a power of two that brings the row's largest
     // magnitude to [2^13, 2^14): pair k of word i holds dims 32 i + 8 q + {k,
@@ -391,201 +383,174 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
         for (int c = 0; c < 4; ++c) o[t][i][c] = 0.f;
     }
 
+    // The tile's words are in registers; each set of them is loaded again, for
+    // the warp's next tile, as soon as its products are issued.
+    int base = 0;  // of tiles_a
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      const uint32_t bar = full0 + 8 * use_stage;
-      if (!__all_sync(0xffffffffu, mbar_probe(bar, use_phase)) &&
-          !__all_sync(0xffffffffu,
-                      mbar_wait(bar, use_phase, abort_flag, p.status, kDevTimeoutProducer)))
-        break;  // the abort flag is set: copies in flight are waited for at the end
-      const uint32_t tile = ring + use_stage * kTileB;
-      use_stage = use_stage + 1 == kStages ? 0 : use_stage + 1;
-      use_phase ^= use_stage == 0 ? 1u : 0u;
-      --ahead;
-      const bool valid = (valid_bits >> ahead) & 1u;
-      const int left = len - ((j0 + i) * kWarps + warp) * kTileTokens;  // live tokens from row 0
-      if (valid) {
-        // ---------------------------------------------------------- scores
-        uint32_t ka[kW], kb[kW];
-        constexpr int kLaneWords = kW < 4 ? kW : 4;
-        constexpr int kRowBytes = 16 * kLaneWords;
+      const int left = at >= 0 ? len - ((j0 + i) * kWarps + warp) * kTileTokens : 0;
+      if (i - base == 32) {
+        base += 32;
+        tiles_a = tiles_b;
+        tiles_b = base + 32 < n ? look_up(base + 32) : -1;
+      }
+      at = tile_at(i + 1 - base);
+      prefetch(tile_at(i + kAhead - base));
+      const uint8_t *next = p.pool.data + static_cast<int64_t>(at) * kTileB;
+      // ------------------------------------------------------------ scores
+      float s[kNT][4];
 #pragma unroll
-        for (int pl = 0; pl < kW / kLaneWords; ++pl) {
-          uint32_t w[kLaneWords];
-          lds(tile + pl * (kTileTokens * kRowBytes) + r * kRowBytes + q * 4 * kLaneWords, w);
+      for (int g = 0; g < kGroups; ++g) {
+        float acc[kNT][4];
 #pragma unroll
-          for (int c = 0; c < kLaneWords; ++c) ka[pl * kLaneWords + c] = w[c];
-          lds(tile + pl * (kTileTokens * kRowBytes) + (r + 8) * kRowBytes + q * 4 * kLaneWords, w);
+        for (int t = 0; t < kNT; ++t)
 #pragma unroll
-          for (int c = 0; c < kLaneWords; ++c) kb[pl * kLaneWords + c] = w[c];
+          for (int c = 0; c < 4; ++c) acc[t][c] = 0.f;
+#pragma unroll
+        for (int i2 = g * kW / kGroups; i2 < (g + 1) * kW / kGroups; ++i2) {
+          const uint32_t ka8 = ka[i2] >> 8, kb8 = kb[i2] >> 8;
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const uint32_t a0 = code_pair(ka[i2], ka8, 2 * ks), a1 = code_pair(kb[i2], kb8, 2 * ks),
+                           a2 = code_pair(ka[i2], ka8, 2 * ks + 1),
+                           a3 = code_pair(kb[i2], kb8, 2 * ks + 1);
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+              mma16816(acc[t], a0, a1, a2, a3, qf[t][i2][2 * ks], qf[t][i2][2 * ks + 1]);
+          }
         }
-        uint32_t sca[2 * kGroups], scb[2 * kGroups];  // scale pairs of tokens r, r + 8
-        lds(tile + 2 * code_bytes(kD) + r * 8 * kGroups, sca);
-        lds(tile + 2 * code_bytes(kD) + (r + 8) * 8 * kGroups, scb);
-        float s[kNT][4];
+        float loa, sa, lob, sb;
+        pair_of<T>(sca[g], loa, sa);
+        pair_of<T>(scb[g], lob, sb);
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          float acc[kNT][4];
+        for (int t = 0; t < kNT; ++t)
 #pragma unroll
-          for (int t = 0; t < kNT; ++t)
+          for (int h = 0; h < 2; ++h) {
+            s[t][h] = fmaf(sa, acc[t][h], g == 0 ? loa * qs[t][g][h]
+                                                 : fmaf(loa, qs[t][g][h], s[t][h]));
+            s[t][h + 2] = fmaf(sb, acc[t][h + 2], g == 0 ? lob * qs[t][g][h]
+                                                         : fmaf(lob, qs[t][g][h], s[t][h + 2]));
+          }
+      }
+      if (at >= 0) load_keys(next);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[t][c] = 0.f;
+      for (int t = 0; t < kNT; ++t)
 #pragma unroll
-          for (int i2 = g * kW / kGroups; i2 < (g + 1) * kW / kGroups; ++i2) {
-            const uint32_t ka8 = ka[i2] >> 8, kb8 = kb[i2] >> 8;
+        for (int c = 0; c < 4; ++c) s[t][c] *= unit[t][c & 1];
+      if (left < kTileTokens) {  // tokens past the end: any bits, so select
+        const bool la = r < left, lb = r + 8 < left;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const uint32_t a0 = code_pair(ka[i2], ka8, 2 * ks), a1 = code_pair(kb[i2], kb8, 2 * ks),
-                             a2 = code_pair(ka[i2], ka8, 2 * ks + 1),
-                             a3 = code_pair(kb[i2], kb8, 2 * ks + 1);
+        for (int t = 0; t < kNT; ++t)
 #pragma unroll
-              for (int t = 0; t < kNT; ++t)
-                mma16816(acc[t], a0, a1, a2, a3, qf[t][i2][2 * ks], qf[t][i2][2 * ks + 1]);
+          for (int h = 0; h < 2; ++h) {
+            s[t][h] = la ? s[t][h] : -INFINITY;
+            s[t][h + 2] = lb ? s[t][h + 2] : -INFINITY;
+          }
+#pragma unroll
+        for (int g = kGroups; g < 2 * kGroups; ++g) {
+          sca[g] = la ? sca[g] : 0u;
+          scb[g] = lb ? scb[g] : 0u;
+        }
+      }
+      // --------------------------------------------------- running softmax
+      float top = -INFINITY, big = 0.f;  // excess over the maxima; largest value scale
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(s[t][h], s[t][h + 2]) - m[t][h]);
+#pragma unroll
+      for (int g = kGroups; g < 2 * kGroups; ++g) {
+        float lo, sa, sb;
+        pair_of<T>(sca[g], lo, sa);
+        pair_of<T>(scb[g], lo, sb);
+        big = fmax3(big, sa, sb);
+      }
+      if (__any_sync(0xffffffffu, top > kRescaleThreshold || big * vnorm > kValueScaleTop)) {
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1)
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+        float shrink = 1.f;  // of what the value products hold
+        if (fresh || big * vnorm > kValueScaleTop) {
+          fresh = false;
+          // scales up to `big` land below 32: room for the next to be larger
+          const float larger = pow2(min(max(4 - exponent_of(big), -100), 100));
+          shrink = larger / vnorm;
+          vnorm = larger;
+        }
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(s[t][h], s[t][h + 2]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1)
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            const float mn = fmaxf(m[t][h], mx);
+            const float alpha = fast_exp2(m[t][h] - mn);
+            m[t][h] = mn;
+            l[t][h] *= alpha;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) extra[t][g][h] *= alpha;
+#pragma unroll
+            for (int i2 = 0; i2 < kD / 16; ++i2) {
+              o[t][i2][h] *= alpha * shrink;
+              o[t][i2][h + 2] *= alpha * shrink;
             }
           }
+      }
+      // ---------------------------------------------------------- P and P V
+      uint32_t pf[kNT][kGroups][kSplitP ? 4 : 2];  // B operands (high, then low parts)
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+        const float p0 = fast_exp2(s[t][0] - m[t][0]), p1 = fast_exp2(s[t][1] - m[t][1]);
+        const float p2 = fast_exp2(s[t][2] - m[t][0]), p3 = fast_exp2(s[t][3] - m[t][1]);
+        l[t][0] += p0 + p2;
+        l[t][1] += p1 + p3;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
           float loa, sa, lob, sb;
-          pair_of<T>(sca[g], loa, sa);
-          pair_of<T>(scb[g], lob, sb);
-#pragma unroll
-          for (int t = 0; t < kNT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              s[t][h] = fmaf(sa, acc[t][h], g == 0 ? loa * qs[t][g][h]
-                                                   : fmaf(loa, qs[t][g][h], s[t][h]));
-              s[t][h + 2] = fmaf(sb, acc[t][h + 2], g == 0 ? lob * qs[t][g][h]
-                                                           : fmaf(lob, qs[t][g][h], s[t][h + 2]));
-            }
-        }
-        float vla[kGroups], vsa[kGroups], vlb[kGroups], vsb[kGroups];
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          pair_of<T>(sca[kGroups + g], vla[g], vsa[g]);
-          pair_of<T>(scb[kGroups + g], vlb[g], vsb[g]);
-        }
-#pragma unroll
-        for (int t = 0; t < kNT; ++t)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[t][c] *= unit[t][c & 1];
-        if (left < kTileTokens) {  // tokens past the end: any bits, so select
-          const bool la = r < left, lb = r + 8 < left;
-#pragma unroll
-          for (int t = 0; t < kNT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              s[t][h] = la ? s[t][h] : -INFINITY;
-              s[t][h + 2] = lb ? s[t][h + 2] : -INFINITY;
-            }
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            vla[g] = la ? vla[g] : 0.f;
-            vsa[g] = la ? vsa[g] : 0.f;
-            vlb[g] = lb ? vlb[g] : 0.f;
-            vsb[g] = lb ? vsb[g] : 0.f;
+          pair_of<T>(sca[kGroups + g], loa, sa);
+          pair_of<T>(scb[kGroups + g], lob, sb);
+          sa *= vnorm;
+          sb *= vnorm;
+          const float x0 = p0 * sa, x1 = p1 * sa, x2 = p2 * sb, x3 = p3 * sb;
+          const uint32_t wa = Elem<__half>::pack2(x0, x1), wb = Elem<__half>::pack2(x2, x3);
+          pf[t][g][0] = transpose8(wa);
+          pf[t][g][1] = transpose8(wb);
+          if constexpr (kSplitP) {
+            const __half2 ha = *reinterpret_cast<const __half2 *>(&wa);
+            const __half2 hb = *reinterpret_cast<const __half2 *>(&wb);
+            pf[t][g][2] = transpose8(Elem<__half>::pack2(x0 - __low2float(ha), x1 - __high2float(ha)));
+            pf[t][g][3] = transpose8(Elem<__half>::pack2(x2 - __low2float(hb), x3 - __high2float(hb)));
           }
+          extra[t][g][0] = fmaf(p0, loa, fmaf(p2, lob, extra[t][g][0]));
+          extra[t][g][1] = fmaf(p1, loa, fmaf(p3, lob, extra[t][g][1]));
         }
-        // ------------------------------------------------- running softmax
-        float top = -INFINITY, big = 0.f;  // excess over the maxima; largest value scale
+      }
+      if (at >= 0) load_scales(next);
 #pragma unroll
-        for (int t = 0; t < kNT; ++t)
+      for (int u = 0; u < kU; ++u) {
+        const uint32_t w0 = vw[2 * u], w1 = vw[2 * u + 1], w2 = vw[2 * kU + 2 * u],
+                       w3 = vw[2 * kU + 2 * u + 1];
+        const uint32_t s0 = w0 >> 8, s1 = w1 >> 8, s2 = w2 >> 8, s3 = w3 >> 8;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(s[t][h], s[t][h + 2]) - m[t][h]);
+        for (int k = 0; k < 4; ++k) {
+          const int g = (64 * u + 32 * (k >> 1)) / kG;
+          const uint32_t a0 = code_pair(w0, s0, k), a1 = code_pair(w1, s1, k),
+                         a2 = code_pair(w2, s2, k), a3 = code_pair(w3, s3, k);
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) big = fmax3(big, vsa[g], vsb[g]);
-        if (__any_sync(0xffffffffu, top > kRescaleThreshold || big * vnorm > kValueScaleTop)) {
-#pragma unroll
-          for (int off = 1; off < 32; off <<= 1)
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-          float shrink = 1.f;  // of what the value products hold
-          if (fresh || big * vnorm > kValueScaleTop) {
-            fresh = false;
-            // scales up to `big` land below 32: room for the next to be larger
-            const float next = pow2(min(max(4 - exponent_of(big), -100), 100));
-            shrink = next / vnorm;
-            vnorm = next;
-          }
-#pragma unroll
-          for (int t = 0; t < kNT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float mx = fmaxf(s[t][h], s[t][h + 2]);
-#pragma unroll
-              for (int off = 4; off < 32; off <<= 1)
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-              const float mn = fmaxf(m[t][h], mx);
-              const float alpha = fast_exp2(m[t][h] - mn);
-              m[t][h] = mn;
-              l[t][h] *= alpha;
-#pragma unroll
-              for (int g = 0; g < kGroups; ++g) extra[t][g][h] *= alpha;
-#pragma unroll
-              for (int i2 = 0; i2 < kD / 16; ++i2) {
-                o[t][i2][h] *= alpha * shrink;
-                o[t][i2][h + 2] *= alpha * shrink;
-              }
-            }
-        }
-        // -------------------------------------------------------- P and P V
-        uint32_t pf[kNT][kGroups][kSplitP ? 4 : 2];  // B operands (high, then low parts)
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          vsa[g] *= vnorm;
-          vsb[g] *= vnorm;
-        }
-#pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          const float p0 = fast_exp2(s[t][0] - m[t][0]), p1 = fast_exp2(s[t][1] - m[t][1]);
-          const float p2 = fast_exp2(s[t][2] - m[t][0]), p3 = fast_exp2(s[t][3] - m[t][1]);
-          l[t][0] += p0 + p2;
-          l[t][1] += p1 + p3;
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            const float x0 = p0 * vsa[g], x1 = p1 * vsa[g], x2 = p2 * vsb[g], x3 = p3 * vsb[g];
-            const uint32_t wa = Elem<__half>::pack2(x0, x1), wb = Elem<__half>::pack2(x2, x3);
-            pf[t][g][0] = transpose8(wa);
-            pf[t][g][1] = transpose8(wb);
-            if constexpr (kSplitP) {
-              const __half2 ha = *reinterpret_cast<const __half2 *>(&wa);
-              const __half2 hb = *reinterpret_cast<const __half2 *>(&wb);
-              pf[t][g][2] = transpose8(Elem<__half>::pack2(x0 - __low2float(ha), x1 - __high2float(ha)));
-              pf[t][g][3] = transpose8(Elem<__half>::pack2(x2 - __low2float(hb), x3 - __high2float(hb)));
-            }
-            extra[t][g][0] = fmaf(p0, vla[g], fmaf(p2, vlb[g], extra[t][g][0]));
-            extra[t][g][1] = fmaf(p1, vla[g], fmaf(p3, vlb[g], extra[t][g][1]));
-          }
-        }
-        uint32_t vw[4 * kU];  // [token pair][u][half]
-#pragma unroll
-        for (int pl = 0; pl < kU; ++pl) {
-          uint32_t w[4];
-          lds(tile + code_bytes(kD) + pl * 512 + lane * 16, w);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) vw[4 * pl + c] = w[c];
-        }
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const uint32_t w0 = vw[2 * u], w1 = vw[2 * u + 1], w2 = vw[2 * kU + 2 * u],
-                         w3 = vw[2 * kU + 2 * u + 1];
-          const uint32_t s0 = w0 >> 8, s1 = w1 >> 8, s2 = w2 >> 8, s3 = w3 >> 8;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int g = (64 * u + 32 * (k >> 1)) / kG;
-            const uint32_t a0 = code_pair(w0, s0, k), a1 = code_pair(w1, s1, k),
-                           a2 = code_pair(w2, s2, k), a3 = code_pair(w3, s3, k);
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) {
-              mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
-              if constexpr (kSplitP)
-                mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][2], pf[t][g][3]);
-            }
+          for (int t = 0; t < kNT; ++t) {
+            mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
+            if constexpr (kSplitP)
+              mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][2], pf[t][g][3]);
           }
         }
       }
-      __syncwarp();  // every lane has read the stage
-      if (i + kStages < n) issue(i + kStages);
+      if (at >= 0) load_values(next);
     }
 
     // ------------------------------------------------ the warps' states meet
-    __syncthreads();  // every ring is drained: its space becomes the buffer
-    if (*abort_flag) break;  // set before the barrier: all warps leave together
+    __syncthreads();  // the previous piece's merge (or the scan) is done with
 #pragma unroll
     for (int t = 0; t < kNT; ++t)
 #pragma unroll
@@ -654,18 +619,6 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
           p.lse[static_cast<int64_t>(b) * p.hq + h] = lse;
       }
     }
-    __syncthreads();          // the buffer becomes rings again
-    fence_proxy_async_smem();
-  }
-  // after a time-out copies may still be in flight: they must land before
-  // the CTA's shared memory is given back
-  if (*abort_flag) {
-    volatile int never = 0;
-    for (; ahead > 0; --ahead) {
-      mbar_wait(full0 + 8 * use_stage, use_phase, &never, nullptr, 0);
-      use_stage = use_stage + 1 == kStages ? 0 : use_stage + 1;
-      use_phase ^= use_stage == 0 ? 1u : 0u;
-    }
   }
 }
 
@@ -715,21 +668,20 @@ int launch_t(const Params &p, int sms, cudaStream_t stream, int *grid_out, bool 
   constexpr int per_sm = kD * kNT <= 128 ? 4 : 2;
   *grid_out = sms * per_sm;
   if (query) return FA_OK;
-  if (static_cast<int64_t>(p.batch + 1) * 8 > PL::kBuf)
-    return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many sequences per call");
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PL::kBuf);
-  if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
+  if (p.batch > kMaxBatch)
+    return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: at most 6000 sequences per call");
+  const int scan = (p.batch + 1) * 8;  // at most 48 KB: no opt-in needed
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(*grid_out);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = PL::kBuf;
+  cfg.dynamicSmemBytes = scan > PL::kMergeBytes ? scan : PL::kMergeBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
   const int64_t blocks =
       static_cast<int64_t>(p.batch) * p.hkv * p.head_tiles * PL::kHeads;
@@ -810,7 +762,6 @@ int run(const fa_kv4_attention_args *a, cudaStream_t stream, bool query, int *gr
   p.part_o = a->part_o;
   p.part_lse = a->part_lse;
   p.merge = reinterpret_cast<int4 *>(a->merge);
-  p.status = a->status;
   *rows = 8 * nt;
   const int64_t n = static_cast<int64_t>(a->batch) * p.hkv * p.head_tiles;
   if (n > INT32_MAX / 16) return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many rows");

@@ -14,7 +14,7 @@ import math
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import raw_stream, require_cuda, status_ptr
+from flagattention_b200._torch import raw_stream, require_cuda
 
 
 class Int4KVCache:
@@ -182,7 +182,7 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
                               context_lens.data_ptr(), num_seqs, hq,
                               1.0 / math.sqrt(d) if attn_scale is None else attn_scale,
                               out.data_ptr(), hq * d, d, lse.data_ptr() if return_lse else None,
-                              base, base + po, base + po + pl, status_ptr(dev))
+                              base, base + po, base + po + pl)
     st = _lib.lib().fa_kv4_attention(ctypes.byref(a), raw_stream(dev))
     if st:
         _lib.check(st, "fa_kv4_attention")

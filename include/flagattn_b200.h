@@ -246,7 +246,6 @@ typedef struct fa_kv4_attention_args {
   float *part_o;
   float *part_lse;
   int32_t *merge;
-  int *status;
 } fa_kv4_attention_args;
 int fa_kv4_attention_workspace_size(const fa_kv4_attention_args *args, size_t *part_o_bytes,
                                     size_t *part_lse_bytes, size_t *merge_bytes);
