@@ -150,7 +150,9 @@ __device__ __noinline__ void compute_share(const Params &p, long long *scan, Con
           if (per_seq * scan[mid] <= u) lo = mid; else hi = mid - 1;
         }
         const long long c = scan[lo + 1] - scan[lo];
-        const long long h = (u - per_seq * scan[lo]) / c;
+        const long long in = u - per_seq * scan[lo];  // 32-bit division where it fits
+        const long long h = in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(c)
+                                             : in / c;
         e = static_cast<int>(lo * per_seq + h);
         x = per_seq * scan[lo] + h * c;
       };
@@ -167,6 +169,14 @@ __device__ __noinline__ void compute_share(const Params &p, long long *scan, Con
 // 2^-24 (k even) or 16 c * 2^-24 (k odd); w8 = w >> 8.
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int k) {
   return (k < 2 ? w : w8) & ((k & 1) ? 0x00f000f0u : 0x000f000fu);
+}
+// The values' operands: byte k / 2 of both halves whole, c + 16 c' times 2^-24
+// (k even), or its upper code alone, 16 c' * 2^-24 (k odd).  The sums for the
+// lower code are their difference, taken once per piece: one instruction per
+// operand.  (The keys cannot: their two codes meet different query numbers.)
+__device__ __forceinline__ uint32_t code_bytes16(uint32_t w, int k) {
+  const uint32_t both = k < 2 ? w & 0x00ff00ffu : __byte_perm(w, 0u, 0x4341);
+  return (k & 1) ? (k < 2 ? w : both) & 0x00f000f0u : both;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -241,16 +251,16 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     x += 1 + nb;
     if (nb > 0 ? j1l <= j0l : x_e < sh.a0) continue;  // the entry's unit alone: no piece here
     const int j0 = static_cast<int>(j0l), j1 = static_cast<int>(j1l);
-    auto part_of = [&](long long u) {
-      return static_cast<int>(min(static_cast<long long>(sh.parts - 1),
-                                  ((u + 1) * sh.parts + sh.total - 1) / sh.total - 1));
-    };
-    const int p_lo = nb > 0 ? part_of(x_e + 1) : static_cast<int>(blockIdx.x);
-    const int p_hi = nb > 0 ? part_of(x_e + nb) : static_cast<int>(blockIdx.x);
-    const bool final_out = p_lo == p_hi;
-    if (j0 == 0 && threadIdx.x == 0)
-      p.merge[e] = make_int4(final_out ? -1 : sh.parts + p_lo, p_lo + 1, p_hi - p_lo, 0);
-    const int slot = j0 == 0 ? sh.parts + static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
+    const int self = static_cast<int>(blockIdx.x);
+    const bool final_out = j1 - j0 == nb;
+    if (j0 == 0 && threadIdx.x == 0) {
+      int last = self;  // CTA with the entry's last block
+      if (!final_out)
+        last = static_cast<int>(min(static_cast<long long>(sh.parts - 1),
+                                    ((x_e + nb + 1) * sh.parts + sh.total - 1) / sh.total - 1));
+      p.merge[e] = make_int4(final_out ? -1 : sh.parts + self, self + 1, last - self, 0);
+    }
+    const int slot = j0 == 0 ? sh.parts + self : self;
     const int h0 = ht * kHeads;                      // first head inside the group
     const int heads = min(kHeads, p.group - h0);
     // this warp's tiles: block j holds its tile j * 4 + warp
@@ -532,12 +542,11 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
       for (int u = 0; u < kU; ++u) {
         const uint32_t w0 = vw[2 * u], w1 = vw[2 * u + 1], w2 = vw[2 * kU + 2 * u],
                        w3 = vw[2 * kU + 2 * u + 1];
-        const uint32_t s0 = w0 >> 8, s1 = w1 >> 8, s2 = w2 >> 8, s3 = w3 >> 8;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int g = (64 * u + 32 * (k >> 1)) / kG;
-          const uint32_t a0 = code_pair(w0, s0, k), a1 = code_pair(w1, s1, k),
-                         a2 = code_pair(w2, s2, k), a3 = code_pair(w3, s3, k);
+          const uint32_t a0 = code_bytes16(w0, k), a1 = code_bytes16(w1, k),
+                         a2 = code_bytes16(w2, k), a3 = code_bytes16(w3, k);
 #pragma unroll
           for (int t = 0; t < kNT; ++t) {
             mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
@@ -572,12 +581,12 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
 #pragma unroll
           for (int pp = 0; pp < 2; ++pp) {
             const float ex = extra[t][(64 * u + 32 * pp) / kG][h];
-            const float even = 0x1p24f / vnorm, odd = 0x1p20f / vnorm;
+            const float unit_o = 0x1p24f / vnorm, odd = 0x1p20f / vnorm;
             const float *oa = o[t][4 * u + 2 * pp], *ob = o[t][4 * u + 2 * pp + 1];
             // codes 2 pp and 2 pp + 1 of rows m < 8, then of rows m >= 8
             *reinterpret_cast<float4 *>(row + 64 * u + 32 * pp + 4 * r) =
-                make_float4(fmaf(oa[h], even, ex), fmaf(ob[h], odd, ex), fmaf(oa[h + 2], even, ex),
-                            fmaf(ob[h + 2], odd, ex));
+                make_float4(fmaf(oa[h] - ob[h], unit_o, ex), fmaf(ob[h], odd, ex),
+                            fmaf(oa[h + 2] - ob[h + 2], unit_o, ex), fmaf(ob[h + 2], odd, ex));
           }
       }
     __syncthreads();
@@ -623,34 +632,39 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
 }
 
 // Merge of split entries: entry e = (sequence, kv head, run of head tiles),
-// one warp per row; partials f32 [slot][rows][kD].
-template <typename T>
+// partials f32 [slot][rows][kD].  Narrow: one warp per row.  Wide: the four
+// warps of a block take every fourth partial of one row, for entries cut
+// into many pieces.
+template <typename T, bool kWide>
 __global__ void __launch_bounds__(128)
     kv4_combine_kernel(const float *__restrict__ part_o, const float *__restrict__ part_lse,
                        const int4 *__restrict__ merge, int rows, int group, int head_tiles,
                        int hkv, int hq, int d, T *__restrict__ out, int64_t o_sb, int64_t o_sh,
                        float *__restrict__ lse) {
-  __shared__ MergeState states[4][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  // one block per row, its four warps take every fourth partial
-  const int e = blockIdx.x / rows, row = blockIdx.x % rows;
-  const int4 mg = merge[e];
-  if (mg.x < 0) return;
+  __shared__ MergeState states[kWide ? 4 : 1][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = kWide ? rows : rows / 4;  // blocks of an entry
+  const int e = blockIdx.x / per;
+  const int row = kWide ? blockIdx.x % per : (blockIdx.x % per) * 4 + warp;
   const int ht = e % head_tiles, kvh = (e / head_tiles) % hkv, b = e / (head_tiles * hkv);
   const int in_group = ht * rows + row;
-  if (in_group >= group) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 mg = merge[e];
+  if (mg.x < 0 || in_group >= group) return;  // of all threads when wide
   const int64_t os = static_cast<int64_t>(rows) * d, off = static_cast<int64_t>(row) * d;
   MergeState st;
   st.init();
-  if (warp == 0)
+  if (!kWide || warp == 0)
     fold_parts<false, 1>(st, part_o, part_lse, mg.x, 0, 1, 1, os, rows, off, row, d, lane);
-  fold_parts<false, 2>(st, part_o, part_lse, mg.y, warp, 4, mg.z, os, rows, off, row, d, lane);
-  states[warp][lane] = st;
-  __syncthreads();
-  if (warp != 0) return;
+  fold_parts<false, 2>(st, part_o, part_lse, mg.y, kWide ? warp : 0, kWide ? 4 : 1, mg.z, os, rows,
+                       off, row, d, lane);
+  if constexpr (kWide) {
+    states[warp][lane] = st;
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) fold_state(st, states[w][lane]);
+    for (int w = 1; w < 4; ++w) fold_state(st, states[w][lane]);
+  }
   const int h = kvh * group + in_group;
   const float l = finish_row<T>(st, d, out + b * o_sb + h * o_sh, lane);
   if (lse && lane == 0) lse[static_cast<int64_t>(b) * hq + h] = l;
@@ -683,13 +697,16 @@ int launch_t(const Params &p, int sms, cudaStream_t stream, int *grid_out, bool 
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
-  const int64_t blocks =
-      static_cast<int64_t>(p.batch) * p.hkv * p.head_tiles * PL::kHeads;
+  // about grid / entries pieces per entry
+  const int64_t entries = static_cast<int64_t>(p.batch) * p.hkv * p.head_tiles;
+  const bool wide = entries * 8 <= *grid_out;
+  const int64_t blocks = entries * (wide ? PL::kHeads : PL::kHeads / 4);
   if (blocks > INT32_MAX) return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many rows");
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T>, static_cast<const float *>(p.part_o),
+  e = cudaLaunchKernelEx(&cfg, wide ? kv4_combine_kernel<T, true> : kv4_combine_kernel<T, false>,
+                         static_cast<const float *>(p.part_o),
                          static_cast<const float *>(p.part_lse),
                          static_cast<const int4 *>(p.merge), PL::kHeads, p.group, p.head_tiles,
                          p.hkv, p.hq, kD, static_cast<T *>(p.o), p.o_sb, p.o_sh, p.lse);
