@@ -34,6 +34,9 @@ namespace prompt {
 
 constexpr int kThreads = 320;
 constexpr int kMmaWarp = 8, kProducerWarp = 9;
+// Of every 8 pairs of columns this many take their exponentials on the FMA
+// pipes instead of the special-function unit.
+constexpr int kFmaPairs = 2;
 constexpr int kTile = 128;                 // rows of a Q tile, keys of a K / V tile
 constexpr uint32_t kTmemCols = 512;
 // O is rescaled only when the maximum grows by more than this (log2 units):
@@ -159,6 +162,33 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
 }
 
+// 2^x for two x >= -126 without the special-function unit: x = n + f with n
+// the nearest integer (adding 1.5 * 2^23 leaves n in the low mantissa bits),
+// 2^f by a polynomial of degree 4 (minimax in relative error on [-1/2, 1/2],
+// Remez exchange: 2.6e-6, below the rounding of P to 16 bits), n added to
+// the exponent field.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float &y0, float &y1) {
+  constexpr float kMagic = 12582912.f;
+  const uint64_t r = fadd2(x, f32x2(kMagic, kMagic));
+  const uint64_t f = fadd2(x, fadd2(f32x2(kMagic, kMagic), r ^ 0x8000000080000000ull));
+  uint64_t p = ffma2(f32x2(0.009570102207362652f, 0.009570102207362652f), f,
+                     f32x2(0.05591785907745361f, 0.05591785907745361f));
+  p = ffma2(p, f, f32x2(0.240247443318367f, 0.240247443318367f));
+  p = ffma2(p, f, f32x2(0.6931217908859253f, 0.6931217908859253f));
+  p = ffma2(p, f, f32x2(0.9999992847442627f, 0.9999992847442627f));
+  float r0, r1, p0, p1;
+  f32x2_split(r, r0, r1);
+  f32x2_split(p, p0, p1);
+  y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
+  y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
+}
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <typename T, int kDqk, int kDv>
 __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *bars,
                                          uint8_t *smem, uint32_t tmem, int x, int warp,
@@ -186,22 +216,30 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
       break;
     tc_fence_after();
     float s[kTile];
-#pragma unroll
-    for (int c = 0; c < kTile / 32; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
-    tmem_wait_ld();
+    // four running maxima; the second half of the row arrives meanwhile
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     const int hi = end - j * kTile;
-    float mx = -INFINITY;
-    if (__all_sync(0xffffffffu, hi >= kTile)) {
+    const bool masked = !__all_sync(0xffffffffu, hi >= kTile);
+    tmem_ld32(t_s, s);
+    tmem_ld32(t_s + 32, s + 32);
+    tmem_wait_ld();
+    tmem_ld32(t_s + 64, s + 64);
+    tmem_ld32(t_s + 96, s + 96);
+    if (masked) {
+      tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < kTile; c += 2) mx = fmax3(mx, s[c], s[c + 1]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < kTile; ++c) {
-        s[c] = c < hi ? s[c] : -INFINITY;  // select: whatever a masked key holds
-        mx = fmaxf(mx, s[c]);
-      }
+      for (int c = 0; c < kTile; ++c) s[c] = c < hi ? s[c] : -INFINITY;  // whatever a masked key holds
     }
-    const float m_tile = mx * p.scale_log2;
+#pragma unroll
+    for (int c = 0; c < kTile / 2; c += 2) mx[(c / 2) & 3] = max3_nan(mx[(c / 2) & 3], s[c], s[c + 1]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = kTile / 2; c < kTile; c += 2)
+      mx[(c / 2) & 3] = max3_nan(mx[(c / 2) & 3], s[c], s[c + 1]);
+    const float m_row = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+    // a NaN score, or an infinite one, makes the row NaN
+    if (!(m_row < INFINITY)) l = NAN;
+    const float m_tile = m_row * p.scale_log2;
     bool resc = false;
     float alpha = 1.f;
     if (j == 0) {
@@ -212,23 +250,6 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
       l *= alpha;
       m_use = m_tile;
     }
-    const float msafe = m_use == -INFINITY ? 0.f : m_use;
-    const uint64_t nm2 = f32x2(-msafe, -msafe);
-    uint32_t w[kTile / 2];
-    uint64_t acc2 = f32x2(0.f, 0.f);
-#pragma unroll
-    for (int c = 0; c < kTile / 2; ++c) {
-      float x0, x1;
-      f32x2_split(ffma2(f32x2(s[2 * c], s[2 * c + 1]), c2, nm2), x0, x1);
-      const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-      acc2 = fadd2(acc2, f32x2(p0, p1));
-      w[c] = Elem<T>::pack2(p0, p1);
-    }
-    float a0, a1;
-    f32x2_split(acc2, a0, a1);
-    l += a0 + a1;
-    tmem_st32(t_s, w);
-    tmem_st32(t_s + 32, w + 32);
     if (__any_sync(0xffffffffu, resc)) {
       const float a = resc ? alpha : 1.f;
 #pragma unroll 1
@@ -242,6 +263,41 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
         tmem_st32(t_o + 32 * c, u);
       }
     }
+    const float msafe = m_use == -INFINITY ? 0.f : m_use;
+    const uint64_t nm2 = f32x2(-msafe, -msafe);
+    uint64_t acc2 = f32x2(0.f, 0.f), acc2b = f32x2(0.f, 0.f);
+    // P over S in place, 32 columns at a time
+    auto chunk = [&](auto fma_pairs, int c0) {
+      uint32_t w[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        uint64_t x2 = ffma2(f32x2(s[c0 + 2 * c], s[c0 + 2 * c + 1]), c2, nm2);
+        float x0, x1, p0, p1;
+        f32x2_split(x2, x0, x1);
+        if ((c & 7) < decltype(fma_pairs)::value) {
+          exp2_pair(f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f)), p0, p1);
+        } else {
+          p0 = fast_exp2(x0);
+          p1 = fast_exp2(x1);
+        }
+        if (c & 1)
+          acc2b = fadd2(acc2b, f32x2(p0, p1));
+        else
+          acc2 = fadd2(acc2, f32x2(p0, p1));
+        w[c] = Elem<T>::pack2(p0, p1);
+      }
+      tmem_st16p(t_s + c0 / 2, w);
+    };
+    if (masked) {  // a masked weight has to be exactly 0
+#pragma unroll
+      for (int c = 0; c < 4; ++c) chunk(std::integral_constant<int, 0>(), 32 * c);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) chunk(std::integral_constant<int, kFmaPairs>(), 32 * c);
+    }
+    float a0, a1;
+    f32x2_split(fadd2(acc2, acc2b), a0, a1);
+    l += a0 + a1;
     // Value rows past the sequence's end belong to the next sequence and may
     // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them.
     // The first Q tile that uses this V tile does so (its P V goes first).
