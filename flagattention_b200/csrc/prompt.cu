@@ -17,9 +17,9 @@
 // cycle (1024 cycles at head size 128) and the exponentials 128 * 128 at 16 a
 // cycle (1024 cycles), so neither may wait for the other.
 //
-//   warps 0-3 / 4-7: rows of Q tile 0 / 1 (one thread per row, S read from
+//   warps 0-7 / 8-15: rows of Q tile 0 / 1 (two threads per row, S read from
 //     TMEM, P written over it as the A operand of P V)
-//   warp 8: MMA issuer    warp 9: TMA producer
+//   warp 16: MMA issuer    warp 17: TMA producer
 //
 // TMEM: S0 S1 (128 columns each, P in place), O0 O1.  The issuer's stream is
 // in order, so the barrier that announces S of step j also says that P V of
@@ -32,11 +32,13 @@
 namespace fa {
 namespace prompt {
 
-constexpr int kThreads = 320;
-constexpr int kMmaWarp = 8, kProducerWarp = 9;
-// Of every 8 pairs of columns this many take their exponentials on the FMA
+// Two warps beyond the roles fill up the last warpgroup, which gives its
+// registers to the row warps: 16 * 112 + 4 * 32 = 20 * 96, the launch's.
+constexpr int kThreads = 640, kRowRegs = 112, kOtherRegs = 32;
+constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17;
+// Of every 16 pairs of columns this many take their exponentials on the FMA
 // pipes instead of the special-function unit.
-constexpr int kFmaPairs = 2;
+constexpr int kFmaPairs = 4;
 constexpr int kTile = 128;                 // rows of a Q tile, keys of a K / V tile
 constexpr uint32_t kTmemCols = 512;
 // O is rescaled only when the maximum grows by more than this (log2 units):
@@ -52,11 +54,12 @@ struct Plan {
   static constexpr int kVBytes = kVChunks * kChunkBytes;
   static constexpr int kKStages = kDqk == 192 ? 2 : (kDqk == 128 ? 3 : 4);
   static constexpr int kVStages = kDqk == 192 ? 1 : (kDqk == 128 ? 2 : 4);
-  static constexpr int kOffQ = 1024;
+  static constexpr int kOffX = 1024;
+  static constexpr int kOffQ = 3072;
   static constexpr int kOffK = kOffQ + 2 * kQBytes;
   static constexpr int kOffV = kOffK + kKStages * kKBytes;
   static constexpr int kSmemUsed = kOffV + kVStages * kVBytes;
-  static constexpr int kSmemBytes = kSmemUsed + 1024;  // base alignment slack
+  static constexpr int kSmemBytes = kSmemUsed;
   static constexpr uint32_t kColS = 0, kColO = 2 * kTile;
   static_assert(kColO + 2 * kDv <= kTmemCols, "TMEM plan");
   static_assert(kSmemBytes <= 232448, "shared memory plan exceeds 227 KB");
@@ -65,13 +68,19 @@ struct Plan {
 struct Bars {
   uint64_t q_full;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], o_full[2];
+  uint64_t p_full[2][2];  // [Q tile][first / last 32 columns of both halves]
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
   int warp_sum[kThreads / 32];
   int item_seq, item_tile;  // -1: no work
 };
+// Row maxima, at the end row sums, that the two threads of a row exchange.
+struct Exchange {
+  float v[2][2][kTile];  // [Q tile][half][row]
+};
+static_assert(sizeof(Exchange) == 2048, "exchange block");
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
 struct Params {
@@ -155,32 +164,71 @@ __device__ __forceinline__ Item get_item(const Params &p, int kvh, int b, int pa
   return it;
 }
 
+// mbar_wait without its out-of-line loop: setmaxnreg does not go with calls.
+__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int *abort_flag,
+                                            int *status, int code) {
+  if (mbar_test(bar, parity)) return true;
+  const long long t0 = clock64();
+#pragma unroll 1
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_test(bar, parity)) return true;
+    if ((i & 63u) == 0) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kWaitLimitCycles) {
+        *abort_flag = 1;
+        if (status) atomicExch(status, code);
+        return false;
+      }
+    }
+  }
+}
 // Warp-wide bounded wait: all lanes return the same verdict.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                           int *status, int code) {
-  if (mbar_probe(bar, parity)) return true;
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
+  return __all_sync(0xffffffffu, wait_inline(bar, parity, abort_flag, status, code)) != 0;
+}
+template <int kRegs>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-// 2^x for two x >= -126 without the special-function unit: x = n + f with n
-// the nearest integer (adding 1.5 * 2^23 leaves n in the low mantissa bits),
-// 2^f by a polynomial of degree 4 (minimax in relative error on [-1/2, 1/2],
-// Remez exchange: 2.6e-6, below the rounding of P to 16 bits), n added to
-// the exponent field.
-__device__ __forceinline__ void exp2_pair(uint64_t x, float &y0, float &y1) {
+// 2^x for kN pairs of x >= -126 without the special-function unit: x = n + f
+// with n the nearest integer (adding 1.5 * 2^23 leaves n in the low mantissa
+// bits), 2^f by a polynomial of degree 4 (minimax in relative error on [-1/2,
+// 1/2], Remez exchange: 2.6e-6, below the rounding of P to 16 bits), n added
+// to the exponent field.  Written step by step over all pairs: the chains are
+// independent and hide one another's latency.
+template <int kN>
+__device__ __forceinline__ void exp2_pairs(uint64_t (&x)[kN]) {
   constexpr float kMagic = 12582912.f;
-  const uint64_t r = fadd2(x, f32x2(kMagic, kMagic));
-  const uint64_t f = fadd2(x, fadd2(f32x2(kMagic, kMagic), r ^ 0x8000000080000000ull));
-  uint64_t p = ffma2(f32x2(0.009570102207362652f, 0.009570102207362652f), f,
-                     f32x2(0.05591785907745361f, 0.05591785907745361f));
-  p = ffma2(p, f, f32x2(0.240247443318367f, 0.240247443318367f));
-  p = ffma2(p, f, f32x2(0.6931217908859253f, 0.6931217908859253f));
-  p = ffma2(p, f, f32x2(0.9999992847442627f, 0.9999992847442627f));
-  float r0, r1, p0, p1;
-  f32x2_split(r, r0, r1);
-  f32x2_split(p, p0, p1);
-  y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
-  y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
+  const float k[5] = {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f,
+                      0.05591785907745361f, 0.009570102207362652f};
+  const uint64_t magic = f32x2(kMagic, kMagic);
+  uint64_t r[kN], y[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) r[i] = fadd2(x[i], magic);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) y[i] = fadd2(r[i], f32x2(-kMagic, -kMagic));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) x[i] = ffma2(y[i], f32x2(-1.f, -1.f), x[i]);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) y[i] = ffma2(x[i], f32x2(k[4], k[4]), f32x2(k[3], k[3]));
+#pragma unroll
+  for (int d = 2; d >= 0; --d)
+#pragma unroll
+    for (int i = 0; i < kN; ++i) y[i] = ffma2(y[i], x[i], f32x2(k[d], k[d]));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    float r0, r1, y0, y1;
+    f32x2_split(r[i], r0, r1);
+    f32x2_split(y[i], y0, y1);
+    x[i] = f32x2(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(r0) << 23)),
+                 __uint_as_float(__float_as_uint(y1) + (__float_as_uint(r1) << 23)));
+  }
 }
 // Maximum that keeps a NaN.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -189,19 +237,28 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
+// Rows of Q tile x: two threads per row, each with half of the key tile's
+// columns (`half`) and of O's.  A wait that gives up does not end the loop
+// (every wait returns at once from then on): the two warps of a row keep
+// meeting at their named barrier.
 template <typename T, int kDqk, int kDv>
 __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *bars,
-                                         uint8_t *smem, uint32_t tmem, int x, int warp,
-                                         int lane) {
+                                         uint8_t *smem, uint32_t tmem, int warp, int lane) {
   using PL = Plan<kDqk, kDv>;
+  constexpr int kCols = kTile / 2, kOCols = kDv / 2;
   volatile int *abort_flag = &bars->abort_flag;
-  const int row = (warp & 3) * 32 + lane;
+  const int x = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+  const int row = quad * 32 + lane;
   const int tok = it.i0 + x * p.tq + row / p.group;  // token in its sequence
   const int head = it.kvh * p.group + row % p.group;
   const bool live = row < p.tq * p.group && tok < it.lq;
-  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  const uint32_t t_s = tmem + lane_off + PL::kColS + x * kTile;
-  const uint32_t t_o = tmem + lane_off + PL::kColO + x * kDv;
+  const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
+  // this half's S columns; its P (32 words) goes over the first of them
+  const uint32_t t_s = tmem + lane_off + PL::kColS + x * kTile + half * kCols;
+  const uint32_t t_o = tmem + lane_off + PL::kColO + x * kDv + half * kOCols;
+  float *mine = reinterpret_cast<Exchange *>(smem + PL::kOffX)->v[x][half] + row;
+  volatile float *other = reinterpret_cast<Exchange *>(smem + PL::kOffX)->v[x][half ^ 1] + row;
+  const int meet = 1 + x * 4 + quad;  // named barrier of the row's two warps
   // keys this row sees: [0, end); rows without a token count as unmasked
   // (their P and O rows are never read)
   const int end = !live ? INT32_MAX
@@ -209,34 +266,34 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
   const int n = it.n[x];
   float m_use = -INFINITY, l = 0.f;
   const uint64_t c2 = f32x2(p.scale_log2, p.scale_log2);
-  bool ok = true;
   for (int j = 0; j < n; ++j) {
-    if (!(ok = warp_wait(smem_u32(&bars->s_full[x]), j & 1u, abort_flag, p.status,
-                         kDevTimeoutSoftmax)))
-      break;
+    warp_wait(smem_u32(&bars->s_full[x]), j & 1u, abort_flag, p.status, kDevTimeoutSoftmax);
     tc_fence_after();
-    float s[kTile];
-    // four running maxima; the second half of the row arrives meanwhile
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    const int hi = end - j * kTile;
-    const bool masked = !__all_sync(0xffffffffu, hi >= kTile);
+    float s[32], s2[32];
     tmem_ld32(t_s, s);
-    tmem_ld32(t_s + 32, s + 32);
+    tmem_ld32(t_s + 32, s2);
+    const int hi = end - j * kTile - half * kCols;
+    const bool masked = !__all_sync(0xffffffffu, hi >= kCols);
     tmem_wait_ld();
-    tmem_ld32(t_s + 64, s + 64);
-    tmem_ld32(t_s + 96, s + 96);
     if (masked) {
-      tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < kTile; ++c) s[c] = c < hi ? s[c] : -INFINITY;  // whatever a masked key holds
+      for (int c = 0; c < 32; ++c) {
+        s[c] = c < hi ? s[c] : -INFINITY;  // select: whatever a masked key holds
+        s2[c] = c + 32 < hi ? s2[c] : -INFINITY;
+      }
     }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < kTile / 2; c += 2) mx[(c / 2) & 3] = max3_nan(mx[(c / 2) & 3], s[c], s[c + 1]);
-    tmem_wait_ld();
-#pragma unroll
-    for (int c = kTile / 2; c < kTile; c += 2)
-      mx[(c / 2) & 3] = max3_nan(mx[(c / 2) & 3], s[c], s[c + 1]);
-    const float m_row = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+    for (int c = 0; c < 32; c += 4) {
+      mx[0] = max3_nan(mx[0], s[c], s[c + 1]);
+      mx[1] = max3_nan(mx[1], s[c + 2], s[c + 3]);
+      mx[2] = max3_nan(mx[2], s2[c], s2[c + 1]);
+      mx[3] = max3_nan(mx[3], s2[c + 2], s2[c + 3]);
+    }
+    float m_row = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+    *mine = m_row;
+    named_bar_sync(meet, 64);
+    m_row = max3_nan(m_row, *other, *other);
     // a NaN score, or an infinite one, makes the row NaN
     if (!(m_row < INFINITY)) l = NAN;
     const float m_tile = m_row * p.scale_log2;
@@ -253,59 +310,23 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
     if (__any_sync(0xffffffffu, resc)) {
       const float a = resc ? alpha : 1.f;
 #pragma unroll 1
-      for (int c = 0; c < kDv / 32; ++c) {
-        float v[32];
-        uint32_t u[32];
-        tmem_ld32(t_o + 32 * c, v);
+      for (int c = 0; c < kOCols / 16; ++c) {
+        float v[16];
+        uint32_t u[16];
+        tmem_ld16(t_o + 16 * c, v);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * a);
-        tmem_st32(t_o + 32 * c, u);
+        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i] * a);
+        tmem_st16(t_o + 16 * c, u);
       }
     }
-    const float msafe = m_use == -INFINITY ? 0.f : m_use;
-    const uint64_t nm2 = f32x2(-msafe, -msafe);
-    uint64_t acc2 = f32x2(0.f, 0.f), acc2b = f32x2(0.f, 0.f);
-    // P over S in place, 32 columns at a time
-    auto chunk = [&](auto fma_pairs, int c0) {
-      uint32_t w[16];
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        uint64_t x2 = ffma2(f32x2(s[c0 + 2 * c], s[c0 + 2 * c + 1]), c2, nm2);
-        float x0, x1, p0, p1;
-        f32x2_split(x2, x0, x1);
-        if ((c & 7) < decltype(fma_pairs)::value) {
-          exp2_pair(f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f)), p0, p1);
-        } else {
-          p0 = fast_exp2(x0);
-          p1 = fast_exp2(x1);
-        }
-        if (c & 1)
-          acc2b = fadd2(acc2b, f32x2(p0, p1));
-        else
-          acc2 = fadd2(acc2, f32x2(p0, p1));
-        w[c] = Elem<T>::pack2(p0, p1);
-      }
-      tmem_st16p(t_s + c0 / 2, w);
-    };
-    if (masked) {  // a masked weight has to be exactly 0
-#pragma unroll
-      for (int c = 0; c < 4; ++c) chunk(std::integral_constant<int, 0>(), 32 * c);
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) chunk(std::integral_constant<int, kFmaPairs>(), 32 * c);
-    }
-    float a0, a1;
-    f32x2_split(fadd2(acc2, acc2b), a0, a1);
-    l += a0 + a1;
     // Value rows past the sequence's end belong to the next sequence and may
     // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them.
     // The first Q tile that uses this V tile does so (its P V goes first).
-    if ((warp & 3) == 0 && it.lk < (j + 1) * kTile && (x == 0 || j >= it.n[0])) {
+    if (quad == 0 && half == 0 && it.lk < (j + 1) * kTile && (x == 0 || j >= it.n[0])) {
       const int st = j % PL::kVStages;
-      if (!(ok = warp_wait(smem_u32(&bars->v_full[st]), (j / PL::kVStages) & 1u, abort_flag,
-                           p.status, kDevTimeoutSoftmax)))
-        break;
+      warp_wait(smem_u32(&bars->v_full[st]), (j / PL::kVStages) & 1u, abort_flag, p.status,
+                kDevTimeoutSoftmax);
       const uint32_t tile = smem_u32(smem + PL::kOffV) + st * PL::kVBytes;
       const int r0 = it.lk - j * kTile;
       const int units = (kTile - r0) * 8;  // 16-byte units of a chunk's rows
@@ -316,42 +337,103 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
                      : "memory");
       fence_proxy_async_smem();
     }
-    tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&bars->p_full[x]));
+    const float msafe = m_use == -INFINITY ? 0.f : m_use;
+    const uint64_t nm2 = f32x2(-msafe, -msafe);
+    uint64_t acc2 = f32x2(0.f, 0.f), acc2b = f32x2(0.f, 0.f);
+    // P over S in place, 32 columns at a time
+    auto chunk = [&](auto fma_pairs, const float (&v)[32], uint32_t to) {
+      constexpr int kF = decltype(fma_pairs)::value;  // the first pairs go to the FMA pipes
+      uint64_t y[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) y[c] = ffma2(f32x2(v[2 * c], v[2 * c + 1]), c2, nm2);
+#pragma unroll
+      for (int c = kF; c < 16; ++c) {
+        float x0, x1;
+        f32x2_split(y[c], x0, x1);
+        y[c] = f32x2(fast_exp2(x0), fast_exp2(x1));
+      }
+      if constexpr (kF > 0) {
+        uint64_t z[kF];
+#pragma unroll
+        for (int c = 0; c < kF; ++c) {
+          float x0, x1;
+          f32x2_split(y[c], x0, x1);
+          z[c] = f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+        }
+        exp2_pairs<kF>(z);
+#pragma unroll
+        for (int c = 0; c < kF; ++c) y[c] = z[c];
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float p0, p1;
+        f32x2_split(y[c], p0, p1);
+        w[c] = Elem<T>::pack2(p0, p1);
+        if (c & 1)
+          acc2b = fadd2(acc2b, y[c]);
+        else
+          acc2 = fadd2(acc2, y[c]);
+      }
+      tmem_st16p(to, w);
+    };
+    // P of a chunk (and the rescaled O, the cleared V) is there: the value
+    // product of the first columns starts while the last are computed
+    auto hand_over = [&](int part) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars->p_full[x][part]));
+    };
+    if (masked) {  // a masked weight has to be exactly 0
+      chunk(std::integral_constant<int, 0>(), s, t_s);
+      hand_over(0);
+      chunk(std::integral_constant<int, 0>(), s2, t_s + 16);
+    } else {
+      chunk(std::integral_constant<int, kFmaPairs>(), s, t_s);
+      hand_over(0);
+      chunk(std::integral_constant<int, kFmaPairs>(), s2, t_s + 16);
+    }
+    hand_over(1);
+    float a0, a1;
+    f32x2_split(fadd2(acc2, acc2b), a0, a1);
+    l += a0 + a1;
   }
-  if (ok && n > 0)
-    ok = warp_wait(smem_u32(&bars->o_full[x]), 0, abort_flag, p.status, kDevTimeoutSoftmax);
-  if (!ok) return;
-  tc_fence_after();
+  if (n > 0) {
+    *mine = l;
+    named_bar_sync(meet, 64);
+    l += *other;
+    if (!warp_wait(smem_u32(&bars->o_full[x]), 0, abort_flag, p.status, kDevTimeoutSoftmax)) return;
+    tc_fence_after();
+  }
   const float f = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
-  T *orow = static_cast<T *>(p.o) + static_cast<int64_t>(it.q0 + tok) * p.o_st + head * p.o_sh;
+  T *orow = static_cast<T *>(p.o) + static_cast<int64_t>(it.q0 + tok) * p.o_st + head * p.o_sh +
+            half * kOCols;
 #pragma unroll 1
-  for (int c = 0; c < kDv / 32; ++c) {
-    float v[32];
+  for (int c = 0; c < kOCols / 16; ++c) {
+    float v[16];
     if (n > 0) {
-      tmem_ld32(t_o + 32 * c, v);
+      tmem_ld16(t_o + 16 * c, v);
       tmem_wait_ld();
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
     }
     if (live) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (32 * c + 8 * i < p.d_v) {
+      for (int i = 0; i < 2; ++i) {
+        if (half * kOCols + 16 * c + 8 * i < p.d_v) {
           uint4 u;
           u.x = Elem<T>::pack2(v[8 * i] * f, v[8 * i + 1] * f);
           u.y = Elem<T>::pack2(v[8 * i + 2] * f, v[8 * i + 3] * f);
           u.z = Elem<T>::pack2(v[8 * i + 4] * f, v[8 * i + 5] * f);
           u.w = Elem<T>::pack2(v[8 * i + 6] * f, v[8 * i + 7] * f);
-          *reinterpret_cast<uint4 *>(orow + 32 * c + 8 * i) = u;
+          *reinterpret_cast<uint4 *>(orow + 16 * c + 8 * i) = u;
         }
       }
     }
   }
-  if (live && p.lse)
+  if (half == 0 && live && p.lse)
     p.lse[static_cast<int64_t>(head) * p.total_q + it.q0 + tok] =
         l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.6931471805599453f;
 }
@@ -363,9 +445,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const __grid_constant__ CUtensorMap v_map,
                             const __grid_constant__ Params p) {
   using PL = Plan<kDqk, kDv>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                              ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, kDevBadSmemAlign);
+    return;
+  }
   Bars *bars = reinterpret_cast<Bars *>(smem);
   volatile int *abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -388,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bars->s_full[i]), 1);
-      mbar_init(smem_u32(&bars->p_full[i]), 4);
+      mbar_init(smem_u32(&bars->p_full[i][0]), 8);
+      mbar_init(smem_u32(&bars->p_full[i][1]), 8);
       mbar_init(smem_u32(&bars->o_full[i]), 1);
     }
     mbar_init(smem_u32(&bars->drain), 1);
@@ -406,9 +491,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t qbase = smem_u32(smem + PL::kOffQ), kbase = smem_u32(smem + PL::kOffK),
                  vbase = smem_u32(smem + PL::kOffV);
 
-  if (warp < 8) {
-    row_role<T, kDqk, kDv>(p, it, bars, smem, tmem, warp >> 2, warp, lane);
+  if (warp < kRowWarps) {
+    take_registers<kRowRegs>();
+    row_role<T, kDqk, kDv>(p, it, bars, smem, tmem, warp, lane);
+  } else if (warp > kProducerWarp) {
+    give_registers<kOtherRegs>();
   } else if (warp == kProducerWarp) {
+    give_registers<kOtherRegs>();
     int gk = 0, gv = 0, gq = 0;
     if (lane == 0 && n_max > 0) {
       tma_prefetch_desc(&q_map);
@@ -424,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       it.kvh * p.group, it.q0 + it.i0 + x * p.tq);
       for (int j = 0; j < n_max; ++j) {
         const int ks = j % PL::kKStages, vs = j % PL::kVStages;
-        if (!mbar_wait(smem_u32(&bars->k_empty[ks]), ((j / PL::kKStages) & 1u) ^ 1u, abort_flag,
+        if (!wait_inline(smem_u32(&bars->k_empty[ks]), ((j / PL::kKStages) & 1u) ^ 1u, abort_flag,
                        p.status, kDevTimeoutProducer))
           break;
         const uint32_t kf = smem_u32(&bars->k_full[ks]);
@@ -433,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_3d(kbase + ks * PL::kKBytes + ch * PL::kChunkBytes, &k_map, kf, ch * 64,
                       it.k0 + j * kTile, it.kvh);
         ++gk;
-        if (!mbar_wait(smem_u32(&bars->v_empty[vs]), ((j / PL::kVStages) & 1u) ^ 1u, abort_flag,
+        if (!wait_inline(smem_u32(&bars->v_empty[vs]), ((j / PL::kVStages) & 1u) ^ 1u, abort_flag,
                        p.status, kDevTimeoutProducer))
           break;
         const uint32_t vf = smem_u32(&bars->v_full[vs]);
@@ -446,18 +535,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*abort_flag) {
         // copies in flight must land before the CTA may exit
         volatile int never = 0;
-        if (gq) mbar_wait(qf, 0, &never, nullptr, 0);
+        if (gq) wait_inline(qf, 0, &never, nullptr, 0);
         for (int t = max(0, gk - PL::kKStages); t < gk; ++t)
-          mbar_wait(smem_u32(&bars->k_full[t % PL::kKStages]), (t / PL::kKStages) & 1u, &never,
+          wait_inline(smem_u32(&bars->k_full[t % PL::kKStages]), (t / PL::kKStages) & 1u, &never,
                     nullptr, 0);
         for (int t = max(0, gv - PL::kVStages); t < gv; ++t)
-          mbar_wait(smem_u32(&bars->v_full[t % PL::kVStages]), (t / PL::kVStages) & 1u, &never,
+          wait_inline(smem_u32(&bars->v_full[t % PL::kVStages]), (t / PL::kVStages) & 1u, &never,
                     nullptr, 0);
       }
     }
     __syncwarp();
   } else {
     // ---------------------------------------------------------- MMA issuer
+    give_registers<kOtherRegs>();
     constexpr uint32_t kIdescQK = umma_idesc_f16(128, kTile, fmt, 0);
     constexpr uint32_t kIdescPV = umma_idesc_f16(128, kDv, fmt, 1);
     const uint64_t q_desc = smem_desc_swz(qbase, 16, 1024, 2);
@@ -481,14 +571,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       tc_commit_warp(smem_u32(&bars->s_full[x]));
     };
-    auto issue_pv = [&](int x, int j) {
+    // value product of key tile j, K steps of the first (part 0) or last 32
+    // columns of each half
+    auto issue_pv = [&](int x, int j, int part) {
       const uint64_t vd = v_desc + static_cast<uint64_t>(((j % PL::kVStages) * PL::kVBytes) >> 4);
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk)
-        umma_ts_warp(tmem + PL::kColO + x * kDv, tmem + PL::kColS + x * kTile + kk * 8,
+      for (int i = 0; i < 4; ++i) {
+        const int kk = (i / 2) * 4 + part * 2 + i % 2;  // 16 keys each
+        umma_ts_warp(tmem + PL::kColO + x * kDv,
+                     tmem + PL::kColS + x * kTile + (kk / 4) * (kTile / 2) + (kk % 4) * 8,
                      vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
-                     (j | kk) ? 1u : 0u);
-      if (j == it.n[x] - 1) tc_commit_warp(smem_u32(&bars->o_full[x]));
+                     (j | part | i) ? 1u : 0u);
+      }
+      if (part == 1 && j == it.n[x] - 1) tc_commit_warp(smem_u32(&bars->o_full[x]));
     };
     if (n_max > 0) ok = wait(&bars->q_full, 0);
     // step j: scores of key tile j, after the value product of tile j - 1
@@ -503,9 +598,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (j > 0 && j - 1 < it.n[x]) {
-          if (!(ok = wait(&bars->p_full[x], (j - 1) & 1u))) break;
+          if (!(ok = wait(&bars->p_full[x][0], (j - 1) & 1u))) break;
           tc_fence_after();
-          issue_pv(x, j - 1);
+          issue_pv(x, j - 1, 0);
+          if (!(ok = wait(&bars->p_full[x][1], (j - 1) & 1u))) break;
+          tc_fence_after();
+          issue_pv(x, j - 1, 1);
         }
         if (j < it.n[x]) {
           tc_fence_after();
@@ -519,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // every issued MMA must finish before TMEM is released
     tc_commit_warp(smem_u32(&bars->drain));
     volatile int never = 0;
-    mbar_wait(smem_u32(&bars->drain), 0, &never, p.status, kDevTimeoutDrain);
+    wait_inline(smem_u32(&bars->drain), 0, &never, p.status, kDevTimeoutDrain);
     __syncwarp();
   }
 
