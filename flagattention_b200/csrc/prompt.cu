@@ -36,9 +36,9 @@ namespace prompt {
 // registers to the row warps: 16 * 112 + 4 * 32 = 20 * 96, the launch's.
 constexpr int kThreads = 640, kRowRegs = 112, kOtherRegs = 32;
 constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17;
-// Of every 16 pairs of columns this many take their exponentials on the FMA
+// Of every 8 pairs of columns this many take their exponentials on the FMA
 // pipes instead of the special-function unit.
-constexpr int kFmaPairs = 4;
+constexpr int kFmaPairs = 2;
 constexpr int kTile = 128;                 // rows of a Q tile, keys of a K / V tile
 constexpr uint32_t kTmemCols = 512;
 // O is rescaled only when the maximum grows by more than this (log2 units):
@@ -230,6 +230,19 @@ __device__ __forceinline__ void exp2_pairs(uint64_t (&x)[kN]) {
                  __uint_as_float(__float_as_uint(y1) + (__float_as_uint(r1) << 23)));
   }
 }
+// Named barrier that returns whether any of its threads' predicates holds.
+__device__ __forceinline__ bool barrier_any(int id, int threads, bool pred) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return any != 0;
+}
 // Maximum that keeps a NaN.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
@@ -291,21 +304,27 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
       mx[3] = max3_nan(mx[3], s2[c + 2], s2[c + 3]);
     }
     float m_row = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-    *mine = m_row;
-    named_bar_sync(meet, 64);
-    m_row = max3_nan(m_row, *other, *other);
     // a NaN score, or an infinite one, makes the row NaN
     if (!(m_row < INFINITY)) l = NAN;
-    const float m_tile = m_row * p.scale_log2;
+    // The two halves of a row share one maximum.  It is exchanged through
+    // shared memory only when some row of the two warps needs a new one; the
+    // barrier itself tells.
     bool resc = false;
     float alpha = 1.f;
-    if (j == 0) {
-      m_use = m_tile;
-    } else if (m_tile > m_use + kRescaleThreshold) {
-      resc = m_use != -INFINITY;  // O is all zeros while no key was visible
-      alpha = resc ? fast_exp2(m_use - m_tile) : 0.f;
-      l *= alpha;
-      m_use = m_tile;
+    if (barrier_any(meet, 64, j == 0 || m_row * p.scale_log2 > m_use + kRescaleThreshold)) {
+      *mine = m_row;
+      named_bar_sync(meet, 64);
+      m_row = max3_nan(m_row, *other, *other);
+      named_bar_sync(meet, 64);  // read before the next exchange writes
+      const float m_tile = m_row * p.scale_log2;
+      if (j == 0) {
+        m_use = m_tile;
+      } else if (m_tile > m_use + kRescaleThreshold) {
+        resc = m_use != -INFINITY;  // O is all zeros while no key was visible
+        alpha = resc ? fast_exp2(m_use - m_tile) : 0.f;
+        l *= alpha;
+        m_use = m_tile;
+      }
     }
     if (__any_sync(0xffffffffu, resc)) {
       const float a = resc ? alpha : 1.f;
@@ -341,13 +360,15 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
     const uint64_t nm2 = f32x2(-msafe, -msafe);
     uint64_t acc2 = f32x2(0.f, 0.f), acc2b = f32x2(0.f, 0.f);
     // P over S in place, 32 columns at a time
-    auto chunk = [&](auto fma_pairs, const float (&v)[32], uint32_t to) {
+    // kPairs pairs of columns of v from the first on, to words of w
+    auto exps = [&](auto fma_pairs, const float *v, uint32_t *w) {
       constexpr int kF = decltype(fma_pairs)::value;  // the first pairs go to the FMA pipes
-      uint64_t y[16];
+      constexpr int kPairs = 8;
+      uint64_t y[kPairs];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) y[c] = ffma2(f32x2(v[2 * c], v[2 * c + 1]), c2, nm2);
+      for (int c = 0; c < kPairs; ++c) y[c] = ffma2(f32x2(v[2 * c], v[2 * c + 1]), c2, nm2);
 #pragma unroll
-      for (int c = kF; c < 16; ++c) {
+      for (int c = kF; c < kPairs; ++c) {
         float x0, x1;
         f32x2_split(y[c], x0, x1);
         y[c] = f32x2(fast_exp2(x0), fast_exp2(x1));
@@ -364,9 +385,8 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
 #pragma unroll
         for (int c = 0; c < kF; ++c) y[c] = z[c];
       }
-      uint32_t w[16];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
+      for (int c = 0; c < kPairs; ++c) {
         float p0, p1;
         f32x2_split(y[c], p0, p1);
         w[c] = Elem<T>::pack2(p0, p1);
@@ -375,9 +395,8 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
         else
           acc2 = fadd2(acc2, y[c]);
       }
-      tmem_st16p(to, w);
     };
-    // P of a chunk (and the rescaled O, the cleared V) is there: the value
+    // P of 32 columns (and the rescaled O, the cleared V) is there: the value
     // product of the first columns starts while the last are computed
     auto hand_over = [&](int part) {
       tmem_wait_st();
@@ -385,16 +404,21 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars->p_full[x][part]));
     };
-    if (masked) {  // a masked weight has to be exactly 0
-      chunk(std::integral_constant<int, 0>(), s, t_s);
+    auto all = [&](auto fma_pairs) {
+      uint32_t w[16], w2[16];
+      exps(fma_pairs, s, w);
+      exps(fma_pairs, s + 16, w + 8);
+      tmem_st16p(t_s, w);
+      exps(fma_pairs, s2, w2);  // hides the store's latency
       hand_over(0);
-      chunk(std::integral_constant<int, 0>(), s2, t_s + 16);
-    } else {
-      chunk(std::integral_constant<int, kFmaPairs>(), s, t_s);
-      hand_over(0);
-      chunk(std::integral_constant<int, kFmaPairs>(), s2, t_s + 16);
-    }
-    hand_over(1);
+      exps(fma_pairs, s2 + 16, w2 + 8);
+      tmem_st16p(t_s + 16, w2);
+      hand_over(1);
+    };
+    if (masked)  // a masked weight has to be exactly 0
+      all(std::integral_constant<int, 0>());
+    else
+      all(std::integral_constant<int, kFmaPairs>());
     float a0, a1;
     f32x2_split(fadd2(acc2, acc2b), a0, a1);
     l += a0 + a1;
