@@ -82,7 +82,7 @@ class PromptArgs(ctypes.Structure):
         ("num_q_heads", _i32), ("num_kv_heads", _i32), ("d_qk", _i32), ("d_v", _i32),
         ("causal", _i32), ("dtype", _i32), ("scale", _f32),
         ("o", _vp), ("o_stride_t", _i64), ("o_stride_h", _i64),
-        ("lse", _vp), ("status", _vp),
+        ("lse", _vp), ("workspace", _vp), ("status", _vp),
     ]
 
 
@@ -120,6 +120,8 @@ SIGNATURES = [
                                         ctypes.POINTER(ctypes.c_size_t)]),
     ("fa_paged_attention", _i32, [ctypes.POINTER(DecodeArgs), _vp]),
     ("fa_split_kv_attention", _i32, [ctypes.POINTER(DecodeArgs), _vp]),
+    ("fa_prompt_workspace_size", _i32, [ctypes.POINTER(PromptArgs),
+                                        ctypes.POINTER(ctypes.c_size_t)]),
     ("fa_prompt_attention", _i32, [ctypes.POINTER(PromptArgs), _vp]),
     ("fa_kv4_cache_bytes", _i32, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(_i64)]),
     ("fa_kv4_append", _i32, [ctypes.POINTER(Kv4Cache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,

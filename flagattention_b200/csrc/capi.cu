@@ -36,8 +36,9 @@ bool gqa_pairs_heads(const fa_decode_args *);
 cudaError_t launch_mla_sv(const CUtensorMap &, const CUtensorMap &, const CUtensorMap &,
                           const CUtensorMap &, const fa_mla_args *, int, cudaStream_t);
 int prompt_tile_tokens(const fa_prompt_args *);
+int prompt_splits(const fa_prompt_args *, int);
 cudaError_t launch_prompt(const CUtensorMap &, const CUtensorMap &, const CUtensorMap &,
-                          const fa_prompt_args *, cudaStream_t);
+                          const fa_prompt_args *, int, float *, float *, cudaStream_t);
 }  // namespace fa
 
 namespace {
@@ -570,6 +571,22 @@ int fa_split_kv_attention(const fa_decode_args *a, void *stream) {
   return run_decode(a, stream);
 }
 
+int fa_prompt_workspace_size(const fa_prompt_args *a, size_t *bytes) {
+  if (!a || !bytes) return fail(FA_ERR_INVALID_ARGUMENT, "null");
+  if (a->batch < 0 || a->total_q < 0 || a->total_k < 0 || a->num_kv_heads <= 0 ||
+      a->num_q_heads <= 0 || a->num_q_heads % a->num_kv_heads ||
+      a->num_q_heads / a->num_kv_heads > 128 || a->d_v <= 0 || a->d_v > 128)
+    return fail(FA_ERR_INVALID_ARGUMENT, "prompt: bad arguments");
+  *bytes = 0;
+  int sms = 0;
+  const int st = current_sm_count(&sms);
+  if (st != FA_OK) return st;
+  const size_t splits = static_cast<size_t>(fa::prompt_splits(a, sms));
+  if (splits > 1)
+    *bytes = splits * a->num_q_heads * a->total_q * (a->d_v + size_t{1}) * sizeof(float);
+  return FA_OK;
+}
+
 int fa_prompt_attention(const fa_prompt_args *a, void *stream) {
   int st = validate_prompt(a);
   if (st != FA_OK) return st;
@@ -589,7 +606,18 @@ int fa_prompt_attention(const fa_prompt_args *a, void *stream) {
   } else {
     km = vm = qm;  // no key exists, so no key tile is ever loaded
   }
-  const cudaError_t e = fa::launch_prompt(qm, km, vm, a, static_cast<cudaStream_t>(stream));
+  int sms = 0;
+  st = current_sm_count(&sms);
+  if (st != FA_OK) return st;
+  const int splits = fa::prompt_splits(a, sms);
+  float *part_o = static_cast<float *>(a->workspace), *part_lse = nullptr;
+  if (splits > 1) {
+    if (!part_o || !aligned16(part_o))
+      return fail(FA_ERR_INVALID_ARGUMENT, "prompt: needs a 16-byte aligned workspace");
+    part_lse = part_o + static_cast<int64_t>(splits) * a->num_q_heads * a->total_q * a->d_v;
+  }
+  const cudaError_t e = fa::launch_prompt(qm, km, vm, a, splits, part_o, part_lse,
+                                          static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? FA_OK : cuda_fail(e, "prompt attention launch");
 }
 

@@ -19,23 +19,26 @@
 //
 //   warps 0-7 / 8-15: rows of Q tile 0 / 1 (two threads per row, S read from
 //     TMEM, P written over it as the A operand of P V)
-//   warp 16: MMA issuer    warp 17: TMA producer
+//   warp 16: MMA issuer    warp 17: TMA producer    warp 18: scheduler
 //
 // TMEM: S0 S1 (128 columns each, P in place), O0 O1.  The issuer's stream is
 // in order, so the barrier that announces S of step j also says that P V of
 // step j - 1 is complete: the rows rescale O without a further wait.
 //
 // Every mbarrier wait is bounded (common.cuh).
+#include <algorithm>
+
 #include "common.cuh"
 #include "flagattn_b200.h"
+#include "merge.cuh"
 
 namespace fa {
 namespace prompt {
 
-// Two warps beyond the roles fill up the last warpgroup, which gives its
+// One warp beyond the roles fills up the last warpgroup, which gives its
 // registers to the row warps: 16 * 112 + 4 * 32 = 20 * 96, the launch's.
 constexpr int kThreads = 640, kRowRegs = 112, kOtherRegs = 32;
-constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17;
+constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17, kSchedulerWarp = 18;
 // Of every 8 pairs of columns this many take their exponentials on the FMA
 // pipes instead of the special-function unit.
 constexpr int kFmaPairs = 2;
@@ -65,16 +68,27 @@ struct Plan {
   static_assert(kSmemBytes <= 232448, "shared memory plan exceeds 227 KB");
 };
 
+// One unit of work, as the scheduler warp hands it to the others.  Key tiles
+// [j0, j1); Q tile x takes those below end[x].
+struct Work {
+  int kvh;                 // -1: no more work
+  int q0, lq, k0, lk, i0;  // i0: first token of Q tile 0 in its sequence
+  int j0, j1, end[2];
+  int split;
+};
+
 struct Bars {
-  uint64_t q_full;
+  uint64_t q_full, q_empty;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t s_full[2], o_full[2];
   uint64_t p_full[2][2];  // [Q tile][first / last 32 columns of both halves]
+  uint64_t work_full[2], work_empty[2];
+  uint64_t cancel_full;
   uint64_t drain;
+  uint4 cancelled;  // response of the launch control unit
+  Work work[2];
   uint32_t tmem_base;
   int abort_flag;
-  int warp_sum[kThreads / 32];
-  int item_seq, item_tile;  // -1: no work
 };
 // Row maxima, at the end row sums, that the two threads of a row exchange.
 struct Exchange {
@@ -86,11 +100,15 @@ static_assert(sizeof(Bars) <= 1024, "barrier block");
 struct Params {
   const int32_t *cu_q, *cu_k;
   int32_t batch, total_q, total_k, hq, hkv, group, tq;  // tq: tokens of a Q tile
+  int32_t items;     // upper bound of the (sequence, Q tile pair) items
+  int32_t splits;    // units an item's keys are cut into
+  int32_t section;   // kv heads whose units go together
   int32_t d_v, causal;
   float scale_log2;
   void *o;
   int64_t o_st, o_sh;
   float *lse;  // nullable, [hq][total_q]
+  float *part_o, *part_lse;  // splits > 1: [split][hq][total_q] ([d_v])
   int *status;
 };
 
@@ -100,68 +118,6 @@ __device__ __forceinline__ void seq_range(const int32_t *cu, int b, int total, i
                                           int &len) {
   start = min(max(__ldg(cu + b), 0), total);
   len = min(max(__ldg(cu + b + 1), start), total) - start;
-}
-
-// Sequence and Q-tile pair of item x: sequences in order, each from its last
-// pair (under a causal mask the one with most keys) to its first.  All
-// threads take part.
-__device__ __forceinline__ void find_item(const Params &p, int x, Bars *bars) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-  const int span = 2 * p.tq;
-  int local = 0;
-  for (int b = b0; b < b1; ++b) {
-    int s, n;
-    seq_range(p.cu_q, b, p.total_q, s, n);
-    local += (n + span - 1) / span;
-  }
-  int incl = local;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) bars->warp_sum[warp] = incl;
-  __syncthreads();
-  int run = incl - local;
-  for (int w = 0; w < warp; ++w) run += bars->warp_sum[w];
-  if (x >= run && x < run + local) {
-    for (int b = b0; b < b1; ++b) {
-      int s, n;
-      seq_range(p.cu_q, b, p.total_q, s, n);
-      const int tiles = (n + span - 1) / span;
-      if (x < run + tiles) {
-        bars->item_seq = b;
-        bars->item_tile = tiles - 1 - (x - run);
-        break;
-      }
-      run += tiles;
-    }
-  }
-  __syncthreads();
-}
-
-struct Item {
-  int kvh, q0, lq, k0, lk, i0;  // i0: first token of Q tile 0 in its sequence
-  int n[2];                     // key tiles of each Q tile
-};
-
-__device__ __forceinline__ Item get_item(const Params &p, int kvh, int b, int pair) {
-  Item it;
-  it.kvh = kvh;
-  seq_range(p.cu_q, b, p.total_q, it.q0, it.lq);
-  seq_range(p.cu_k, b, p.total_k, it.k0, it.lk);
-  it.i0 = pair * 2 * p.tq;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int first = it.i0 + x * p.tq;
-    const int last = min(first + p.tq, it.lq) - 1;  // last live token
-    int keys = p.causal ? min(it.lk, last + it.lk - it.lq + 1) : it.lk;
-    if (last < first) keys = 0;
-    it.n[x] = keys > 0 ? (keys + kTile - 1) / kTile : 0;
-  }
-  return it;
 }
 
 // mbar_wait without its out-of-line loop: setmaxnreg does not go with calls.
@@ -255,8 +211,9 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // (every wait returns at once from then on): the two warps of a row keep
 // meeting at their named barrier.
 template <typename T, int kDqk, int kDv>
-__device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *bars,
-                                         uint8_t *smem, uint32_t tmem, int warp, int lane) {
+__device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *bars,
+                                         uint8_t *smem, uint32_t tmem, int warp, int lane,
+                                         uint32_t &steps, uint32_t &outs, uint32_t tiles) {
   using PL = Plan<kDqk, kDv>;
   constexpr int kCols = kTile / 2, kOCols = kDv / 2;
   volatile int *abort_flag = &bars->abort_flag;
@@ -276,11 +233,11 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
   // (their P and O rows are never read)
   const int end = !live ? INT32_MAX
                         : (p.causal ? min(it.lk, tok + it.lk - it.lq + 1) : it.lk);
-  const int n = it.n[x];
+  const int n = it.end[x];
   float m_use = -INFINITY, l = 0.f;
   const uint64_t c2 = f32x2(p.scale_log2, p.scale_log2);
-  for (int j = 0; j < n; ++j) {
-    warp_wait(smem_u32(&bars->s_full[x]), j & 1u, abort_flag, p.status, kDevTimeoutSoftmax);
+  for (int j = it.j0; j < n; ++j, ++steps) {
+    warp_wait(smem_u32(&bars->s_full[x]), steps & 1u, abort_flag, p.status, kDevTimeoutSoftmax);
     tc_fence_after();
     float s[32], s2[32];
     tmem_ld32(t_s, s);
@@ -311,13 +268,13 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
     // barrier itself tells.
     bool resc = false;
     float alpha = 1.f;
-    if (barrier_any(meet, 64, j == 0 || m_row * p.scale_log2 > m_use + kRescaleThreshold)) {
+    if (barrier_any(meet, 64, j == it.j0 || m_row * p.scale_log2 > m_use + kRescaleThreshold)) {
       *mine = m_row;
       named_bar_sync(meet, 64);
       m_row = max3_nan(m_row, *other, *other);
       named_bar_sync(meet, 64);  // read before the next exchange writes
       const float m_tile = m_row * p.scale_log2;
-      if (j == 0) {
+      if (j == it.j0) {
         m_use = m_tile;
       } else if (m_tile > m_use + kRescaleThreshold) {
         resc = m_use != -INFINITY;  // O is all zeros while no key was visible
@@ -342,9 +299,10 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
     // Value rows past the sequence's end belong to the next sequence and may
     // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them.
     // The first Q tile that uses this V tile does so (its P V goes first).
-    if (quad == 0 && half == 0 && it.lk < (j + 1) * kTile && (x == 0 || j >= it.n[0])) {
-      const int st = j % PL::kVStages;
-      warp_wait(smem_u32(&bars->v_full[st]), (j / PL::kVStages) & 1u, abort_flag, p.status,
+    if (quad == 0 && half == 0 && it.lk < (j + 1) * kTile && (x == 0 || j >= it.end[0])) {
+      const uint32_t v_tile = tiles + (j - it.j0);
+      const int st = v_tile % PL::kVStages;
+      warp_wait(smem_u32(&bars->v_full[st]), (v_tile / PL::kVStages) & 1u, abort_flag, p.status,
                 kDevTimeoutSoftmax);
       const uint32_t tile = smem_u32(smem + PL::kOffV) + st * PL::kVBytes;
       const int r0 = it.lk - j * kTile;
@@ -423,43 +381,255 @@ __device__ __forceinline__ void row_role(const Params &p, const Item &it, Bars *
     f32x2_split(fadd2(acc2, acc2b), a0, a1);
     l += a0 + a1;
   }
-  if (n > 0) {
+  const bool any = n > it.j0;
+  if (any) {
     *mine = l;
     named_bar_sync(meet, 64);
     l += *other;
-    if (!warp_wait(smem_u32(&bars->o_full[x]), 0, abort_flag, p.status, kDevTimeoutSoftmax)) return;
+    warp_wait(smem_u32(&bars->o_full[x]), outs & 1u, abort_flag, p.status, kDevTimeoutSoftmax);
+    ++outs;
     tc_fence_after();
   }
   const float f = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
-  T *orow = static_cast<T *>(p.o) + static_cast<int64_t>(it.q0 + tok) * p.o_st + head * p.o_sh +
-            half * kOCols;
+  const float lse = l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.6931471805599453f;
+  const int col0 = half * kOCols;
+  // rows of the output, or (f32) of this split's partial result
+  const int64_t prow = (static_cast<int64_t>(it.split) * p.hq + head) * p.total_q + it.q0 + tok;
+  T *orow = static_cast<T *>(p.o) + static_cast<int64_t>(it.q0 + tok) * p.o_st + head * p.o_sh + col0;
+  float *po = p.part_o + prow * p.d_v + col0;
 #pragma unroll 1
   for (int c = 0; c < kOCols / 16; ++c) {
     float v[16];
-    if (n > 0) {
+    if (any) {
       tmem_ld16(t_o + 16 * c, v);
       tmem_wait_ld();
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.f;
     }
-    if (live) {
+    if (!live) continue;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (half * kOCols + 16 * c + 8 * i < p.d_v) {
-          uint4 u;
-          u.x = Elem<T>::pack2(v[8 * i] * f, v[8 * i + 1] * f);
-          u.y = Elem<T>::pack2(v[8 * i + 2] * f, v[8 * i + 3] * f);
-          u.z = Elem<T>::pack2(v[8 * i + 4] * f, v[8 * i + 5] * f);
-          u.w = Elem<T>::pack2(v[8 * i + 6] * f, v[8 * i + 7] * f);
-          *reinterpret_cast<uint4 *>(orow + 16 * c + 8 * i) = u;
-        }
+    for (int i = 0; i < 16; ++i) v[i] *= f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (col0 + 16 * c + 8 * i >= p.d_v) continue;
+      if (p.splits == 1) {
+        uint4 u;
+        u.x = Elem<T>::pack2(v[8 * i], v[8 * i + 1]);
+        u.y = Elem<T>::pack2(v[8 * i + 2], v[8 * i + 3]);
+        u.z = Elem<T>::pack2(v[8 * i + 4], v[8 * i + 5]);
+        u.w = Elem<T>::pack2(v[8 * i + 6], v[8 * i + 7]);
+        *reinterpret_cast<uint4 *>(orow + 16 * c + 8 * i) = u;
+      } else {
+        float4 *dst = reinterpret_cast<float4 *>(po + 16 * c + 8 * i);
+        dst[0] = make_float4(v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3]);
+        dst[1] = make_float4(v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]);
       }
     }
   }
-  if (half == 0 && live && p.lse)
-    p.lse[static_cast<int64_t>(head) * p.total_q + it.q0 + tok] =
-        l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.6931471805599453f;
+  if (half == 0 && live) {
+    if (p.splits > 1)
+      p.part_lse[prow] = lse;
+    else if (p.lse)
+      p.lse[static_cast<int64_t>(head) * p.total_q + it.q0 + tok] = lse;
+  }
+  // the O reads above precede the next unit's first product into it (issued
+  // after this warp's next hand-over)
+  tc_fence_before();
+}
+
+// --------------------------------------------------------------- scheduling
+// The grid holds one CTA per unit; those that run take the units of CTAs not
+// yet launched (cluster launch control), so every unit starts as soon as an
+// SM is free for it and a CTA's set-up is paid once per SM.
+__device__ __forceinline__ void cancel_next(uint32_t response, uint32_t bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], "
+      "[%1];" ::"r"(response),
+      "r"(bar)
+      : "memory");
+}
+// The unit taken over (its block index), or -1 when none was left.
+__device__ __forceinline__ int cancelled_block(uint32_t response) {
+  uint32_t ok, x = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, h;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(response)
+      : "memory");
+  return ok ? static_cast<int>(x) : -1;
+}
+
+// Finds the sequence and Q-tile pair of an item.  One warp; remembers where it
+// was, since the items a CTA takes come in increasing order.
+//
+// Up to 32 sequences: all items by falling number of key tiles, so that the
+// units that run last are short.  A lane keeps one sequence; the pairs with at
+// least c key tiles are its last ones, counted in closed form, and c falls as
+// the item number grows.  More sequences: sequence by sequence, each from its
+// last pair (under a causal mask the one with most keys) to its first.
+struct Finder {
+  const Params &p;
+  const int lane, span;
+  int lq = 0, lk = 0, pairs = 0;  // of the lane's sequence
+  int c = -1;                     // key tiles of the current items
+  int base = 0, first = 0;        // items before them / before sequence `first`
+
+  __device__ __forceinline__ Finder(const Params &p_, int lane_) : p(p_), lane(lane_), span(2 * p_.tq) {
+    if (p.batch > 32) return;
+    if (lane < p.batch) {
+      int s;
+      seq_range(p.cu_q, lane, p.total_q, s, lq);
+      seq_range(p.cu_k, lane, p.total_k, s, lk);
+      pairs = (lq + span - 1) / span;
+    }
+    restart();
+  }
+  __device__ __forceinline__ void restart() {
+    base = 0;
+    c = __reduce_max_sync(0xffffffffu, pairs > 0 ? (lk + kTile - 1) / kTile : 0);
+  }
+  // pairs of the lane's sequence with at least n key tiles: pair i sees
+  // min((i + 1) * span, lq) + lk - lq keys when causal, lk otherwise
+  __device__ __forceinline__ int at_least(int n) const {
+    if (n <= 0) return pairs;
+    const int64_t need = static_cast<int64_t>(n - 1) * kTile + 1;
+    if (!p.causal) return lk >= need ? pairs : 0;
+    const int64_t t = need - lk + lq;  // tokens the pair must reach
+    if (t > lq) return 0;
+    const int skip = t > span ? static_cast<int>((t + span - 1) / span) - 1 : 0;
+    return pairs - min(skip, pairs - 1);
+  }
+  __device__ __forceinline__ int inclusive_scan(int v) const {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  }
+  __device__ __forceinline__ bool by_cost(int x, int &b, int &pair) {
+    if (x < base) restart();
+    for (; c >= 0; --c) {
+      const int more = at_least(c + 1), mine = (pairs > 0 ? at_least(c) : 0) - (pairs > 0 ? more : 0);
+      const int incl = inclusive_scan(mine);
+      const int all = __shfl_sync(0xffffffffu, incl, 31);
+      if (x < base + all) {
+        const int at = __ffs(__ballot_sync(0xffffffffu, x < base + incl)) - 1;
+        b = at;
+        pair = __shfl_sync(0xffffffffu, pairs - more - 1 + (incl - mine), at) - (x - base);
+        return true;
+      }
+      base += all;
+    }
+    return false;  // the bound of the items is not tight
+  }
+  __device__ __forceinline__ bool in_order(int x, int &b, int &pair) {
+    if (x < base) base = first = 0;
+    for (; first < p.batch; first += 32) {
+      int s, n = 0;
+      if (first + lane < p.batch) seq_range(p.cu_q, first + lane, p.total_q, s, n);
+      const int incl = inclusive_scan((n + span - 1) / span);
+      const int all = __shfl_sync(0xffffffffu, incl, 31);
+      if (x < base + all) {
+        const int at = __ffs(__ballot_sync(0xffffffffu, x < base + incl)) - 1;
+        b = first + at;
+        pair = base + __shfl_sync(0xffffffffu, incl, at) - 1 - x;
+        return true;
+      }
+      base += all;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool find(int x, int &b, int &pair) {
+    return p.batch <= 32 ? by_cost(x, b, pair) : in_order(x, b, pair);
+  }
+};
+
+__device__ __forceinline__ void scheduler_role(const Params &p, Bars *bars, int lane) {
+  volatile int *abort_flag = &bars->abort_flag;
+  const uint32_t response = smem_u32(&bars->cancelled);
+  Finder finder(p, lane);
+  uint32_t count = 0;  // units handed out
+  int idx = blockIdx.x;
+  for (uint32_t asked = 0; idx >= 0; ++asked) {
+    if (lane == 0) cancel_next(response, smem_u32(&bars->cancel_full));
+    // units of a section of kv heads: item by item, its splits, its heads
+    const int per_section = p.items * p.splits * p.section;
+    const int sec = idx / per_section, in = idx - sec * per_section;
+    const int width = min(p.section, p.hkv - sec * p.section);
+    const int x = in / (width * p.splits), rest = in - x * width * p.splits;
+    int b, pair;
+    if (finder.find(x, b, pair)) {
+      Work w;
+      w.kvh = sec * p.section + rest % width;
+      w.split = rest / width;
+      seq_range(p.cu_q, b, p.total_q, w.q0, w.lq);
+      seq_range(p.cu_k, b, p.total_k, w.k0, w.lk);
+      w.i0 = pair * 2 * p.tq;
+      int n[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int first = w.i0 + t * p.tq;
+        const int last = min(first + p.tq, w.lq) - 1;  // last live token
+        int keys = p.causal ? min(w.lk, last + w.lk - w.lq + 1) : w.lk;
+        if (last < first) keys = 0;
+        n[t] = keys > 0 ? (keys + kTile - 1) / kTile : 0;
+      }
+      const int n_max = max(n[0], n[1]);
+      w.j0 = static_cast<int>(static_cast<int64_t>(w.split) * n_max / p.splits);
+      w.j1 = static_cast<int>(static_cast<int64_t>(w.split + 1) * n_max / p.splits);
+      w.end[0] = min(w.j1, n[0]);
+      w.end[1] = min(w.j1, n[1]);
+      const uint32_t slot = count & 1u;
+      if (!warp_wait(smem_u32(&bars->work_empty[slot]), ((count >> 1) & 1u) ^ 1u, abort_flag,
+                     p.status, kDevTimeoutProducer))
+        return;  // nothing more is handed out: the others' waits run out
+      if (lane == 0) {
+        bars->work[slot] = w;
+        mbar_arrive(smem_u32(&bars->work_full[slot]));
+      }
+      __syncwarp();
+      ++count;
+    }
+    if (!warp_wait(smem_u32(&bars->cancel_full), asked & 1u, abort_flag, p.status,
+                   kDevTimeoutProducer))
+      return;
+    idx = cancelled_block(response);
+    fence_proxy_async_smem();  // read before the next response is written
+    __syncwarp();
+  }
+  const uint32_t slot = count & 1u;
+  if (!warp_wait(smem_u32(&bars->work_empty[slot]), ((count >> 1) & 1u) ^ 1u, abort_flag,
+                 p.status, kDevTimeoutProducer))
+    return;
+  if (lane == 0) {
+    bars->work[slot].kvh = -1;
+    mbar_arrive(smem_u32(&bars->work_full[slot]));
+  }
+}
+
+// The k-th unit of this CTA; false when there is none left.  The wait ends
+// by its own time limit only: the two warps of a row both get the unit or
+// both give up.
+__device__ __forceinline__ bool next_work(Bars *bars, uint32_t k, int lane, int *status, Work &w) {
+  volatile int no_abort = 0;
+  const uint32_t slot = k & 1u;
+  if (!warp_wait(smem_u32(&bars->work_full[slot]), (k >> 1) & 1u, &no_abort, status,
+                 kDevTimeoutProducer)) {
+    *const_cast<volatile int *>(&bars->abort_flag) = 1;
+    return false;
+  }
+  w = bars->work[slot];
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_u32(&bars->work_empty[slot]));
+  return w.kvh >= 0;
 }
 
 template <typename T, int kDqk, int kDv>
@@ -479,15 +649,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
 
-  if (threadIdx.x == 0) bars->item_seq = -1;
-  __syncthreads();
-  find_item(p, blockIdx.x / p.hkv, bars);
-  if (bars->item_seq < 0) return;  // the grid is an upper bound of the items
-  const Item it = get_item(p, blockIdx.x % p.hkv, bars->item_seq, bars->item_tile);
-  const int n_max = max(it.n[0], it.n[1]);
-
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&bars->q_full), 1);
+    mbar_init(smem_u32(&bars->q_empty), 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&bars->k_full[i]), 1);
       mbar_init(smem_u32(&bars->k_empty[i]), 1);
@@ -499,7 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->p_full[i][0]), 8);
       mbar_init(smem_u32(&bars->p_full[i][1]), 8);
       mbar_init(smem_u32(&bars->o_full[i]), 1);
+      mbar_init(smem_u32(&bars->work_full[i]), 1);
+      mbar_init(smem_u32(&bars->work_empty[i]), kRowWarps + 2);  // rows, MMA, producer
     }
+    mbar_init(smem_u32(&bars->cancel_full), 1);
     mbar_init(smem_u32(&bars->drain), 1);
     bars->abort_flag = 0;
     fence_barrier_init();
@@ -517,56 +684,78 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kRowWarps) {
     take_registers<kRowRegs>();
-    row_role<T, kDqk, kDv>(p, it, bars, smem, tmem, warp, lane);
+    uint32_t steps = 0, outs = 0, tiles = 0;
+    Work it;
+    for (uint32_t k = 0; next_work(bars, k, lane, p.status, it); ++k) {
+      row_role<T, kDqk, kDv>(p, it, bars, smem, tmem, warp, lane, steps, outs, tiles);
+      tiles += it.j1 - it.j0;
+    }
   } else if (warp > kProducerWarp) {
     give_registers<kOtherRegs>();
+    if (warp == kSchedulerWarp) scheduler_role(p, bars, lane);
   } else if (warp == kProducerWarp) {
     give_registers<kOtherRegs>();
-    int gk = 0, gv = 0, gq = 0;
-    if (lane == 0 && n_max > 0) {
+    uint32_t g = 0, gv = 0, gq = 0;  // K tiles, V tiles, Q pairs issued
+    if (lane == 0) {
       tma_prefetch_desc(&q_map);
       tma_prefetch_desc(&k_map);
       tma_prefetch_desc(&v_map);
+    }
+    Work it;
+    bool ok = true;
+    for (uint32_t k = 0; ok && next_work(bars, k, lane, p.status, it); ++k) {
+      if (it.j1 <= it.j0) continue;
+      if (!(ok = warp_wait(smem_u32(&bars->q_empty), (gq & 1u) ^ 1u, abort_flag, p.status,
+                           kDevTimeoutProducer)))
+        break;
       const uint32_t qf = smem_u32(&bars->q_full);
-      const int qtiles = it.n[1] > 0 ? 2 : 1;
-      mbar_arrive_expect_tx(qf, qtiles * PL::kQkChunks * p.tq * p.group * 128);
-      gq = 1;
-      for (int x = 0; x < qtiles; ++x)
-        for (int ch = 0; ch < PL::kQkChunks; ++ch)
-          tma_load_3d(qbase + x * PL::kQBytes + ch * PL::kChunkBytes, &q_map, qf, ch * 64,
-                      it.kvh * p.group, it.q0 + it.i0 + x * p.tq);
-      for (int j = 0; j < n_max; ++j) {
-        const int ks = j % PL::kKStages, vs = j % PL::kVStages;
-        if (!wait_inline(smem_u32(&bars->k_empty[ks]), ((j / PL::kKStages) & 1u) ^ 1u, abort_flag,
-                       p.status, kDevTimeoutProducer))
+      const int qtiles = it.end[1] > it.j0 ? 2 : 1;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(qf, qtiles * PL::kQkChunks * p.tq * p.group * 128);
+        for (int x = 0; x < qtiles; ++x)
+          for (int ch = 0; ch < PL::kQkChunks; ++ch)
+            tma_load_3d(qbase + x * PL::kQBytes + ch * PL::kChunkBytes, &q_map, qf, ch * 64,
+                        it.kvh * p.group, it.q0 + it.i0 + x * p.tq);
+      }
+      ++gq;
+      for (int j = it.j0; j < it.j1; ++j) {
+        const uint32_t ks = g % PL::kKStages, vs = gv % PL::kVStages;
+        if (!(ok = warp_wait(smem_u32(&bars->k_empty[ks]), ((g / PL::kKStages) & 1u) ^ 1u,
+                             abort_flag, p.status, kDevTimeoutProducer)))
           break;
-        const uint32_t kf = smem_u32(&bars->k_full[ks]);
-        mbar_arrive_expect_tx(kf, PL::kKBytes);
-        for (int ch = 0; ch < PL::kQkChunks; ++ch)
-          tma_load_3d(kbase + ks * PL::kKBytes + ch * PL::kChunkBytes, &k_map, kf, ch * 64,
-                      it.k0 + j * kTile, it.kvh);
-        ++gk;
-        if (!wait_inline(smem_u32(&bars->v_empty[vs]), ((j / PL::kVStages) & 1u) ^ 1u, abort_flag,
-                       p.status, kDevTimeoutProducer))
+        if (lane == 0) {
+          const uint32_t kf = smem_u32(&bars->k_full[ks]);
+          mbar_arrive_expect_tx(kf, PL::kKBytes);
+#pragma unroll
+          for (int ch = 0; ch < PL::kQkChunks; ++ch)
+            tma_load_3d(kbase + ks * PL::kKBytes + ch * PL::kChunkBytes, &k_map, kf, ch * 64,
+                        it.k0 + j * kTile, it.kvh);
+        }
+        ++g;
+        if (!(ok = warp_wait(smem_u32(&bars->v_empty[vs]), ((gv / PL::kVStages) & 1u) ^ 1u,
+                             abort_flag, p.status, kDevTimeoutProducer)))
           break;
-        const uint32_t vf = smem_u32(&bars->v_full[vs]);
-        mbar_arrive_expect_tx(vf, PL::kVBytes);
-        for (int ch = 0; ch < PL::kVChunks; ++ch)
-          tma_load_3d(vbase + vs * PL::kVBytes + ch * PL::kChunkBytes, &v_map, vf, ch * 64,
-                      it.k0 + j * kTile, it.kvh);
+        if (lane == 0) {
+          const uint32_t vf = smem_u32(&bars->v_full[vs]);
+          mbar_arrive_expect_tx(vf, PL::kVBytes);
+#pragma unroll
+          for (int ch = 0; ch < PL::kVChunks; ++ch)
+            tma_load_3d(vbase + vs * PL::kVBytes + ch * PL::kChunkBytes, &v_map, vf, ch * 64,
+                        it.k0 + j * kTile, it.kvh);
+        }
         ++gv;
       }
-      if (*abort_flag) {
-        // copies in flight must land before the CTA may exit
-        volatile int never = 0;
-        if (gq) wait_inline(qf, 0, &never, nullptr, 0);
-        for (int t = max(0, gk - PL::kKStages); t < gk; ++t)
-          wait_inline(smem_u32(&bars->k_full[t % PL::kKStages]), (t / PL::kKStages) & 1u, &never,
+    }
+    if (*abort_flag) {
+      // copies in flight must land before the CTA may exit
+      volatile int never = 0;
+      if (gq) wait_inline(smem_u32(&bars->q_full), (gq - 1) & 1u, &never, nullptr, 0);
+      for (uint32_t t = g > PL::kKStages ? g - PL::kKStages : 0; t < g; ++t)
+        wait_inline(smem_u32(&bars->k_full[t % PL::kKStages]), (t / PL::kKStages) & 1u, &never,
                     nullptr, 0);
-        for (int t = max(0, gv - PL::kVStages); t < gv; ++t)
-          wait_inline(smem_u32(&bars->v_full[t % PL::kVStages]), (t / PL::kVStages) & 1u, &never,
+      for (uint32_t t = gv > PL::kVStages ? gv - PL::kVStages : 0; t < gv; ++t)
+        wait_inline(smem_u32(&bars->v_full[t % PL::kVStages]), (t / PL::kVStages) & 1u, &never,
                     nullptr, 0);
-      }
     }
     __syncwarp();
   } else {
@@ -577,14 +766,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t q_desc = smem_desc_swz(qbase, 16, 1024, 2);
     const uint64_t k_desc = smem_desc_swz(kbase, 16, 1024, 2);
     const uint64_t v_desc = smem_desc_swz(vbase, PL::kChunkBytes, 1024, 2);
-    bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       return warp_wait(smem_u32(bar), parity, abort_flag, p.status, kDevTimeoutMma);
     };
-    // S of Q tile x and key tile j
-    auto issue_qk = [&](int x, int j) {
+    // S of Q tile x and the key tile in stage st
+    auto issue_qk = [&](int x, uint32_t st) {
       const uint64_t qd = q_desc + static_cast<uint64_t>((x * PL::kQBytes) >> 4);
-      const uint64_t kd = k_desc + static_cast<uint64_t>(((j % PL::kKStages) * PL::kKBytes) >> 4);
+      const uint64_t kd = k_desc + static_cast<uint64_t>((st * PL::kKBytes) >> 4);
 #pragma unroll
       for (int ch = 0; ch < PL::kQkChunks; ++ch)
 #pragma unroll
@@ -595,48 +783,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       tc_commit_warp(smem_u32(&bars->s_full[x]));
     };
-    // value product of key tile j, K steps of the first (part 0) or last 32
-    // columns of each half
-    auto issue_pv = [&](int x, int j, int part) {
-      const uint64_t vd = v_desc + static_cast<uint64_t>(((j % PL::kVStages) * PL::kVBytes) >> 4);
+    // value product with the tile in stage st, K steps of the first (part 0)
+    // or last 32 columns of each half
+    auto issue_pv = [&](int x, uint32_t st, int part, bool first) {
+      const uint64_t vd = v_desc + static_cast<uint64_t>((st * PL::kVBytes) >> 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int kk = (i / 2) * 4 + part * 2 + i % 2;  // 16 keys each
         umma_ts_warp(tmem + PL::kColO + x * kDv,
                      tmem + PL::kColS + x * kTile + (kk / 4) * (kTile / 2) + (kk % 4) * 8,
                      vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
-                     (j | part | i) ? 1u : 0u);
+                     (first && part == 0 && i == 0) ? 0u : 1u);
       }
-      if (part == 1 && j == it.n[x] - 1) tc_commit_warp(smem_u32(&bars->o_full[x]));
     };
-    if (n_max > 0) ok = wait(&bars->q_full, 0);
-    // step j: scores of key tile j, after the value product of tile j - 1
-    for (int j = 0; j <= n_max && ok; ++j) {
-      if (j < n_max) {
-        if (!(ok = wait(&bars->k_full[j % PL::kKStages], (j / PL::kKStages) & 1u))) break;
-      }
-      if (j > 0) {
-        if (!(ok = wait(&bars->v_full[(j - 1) % PL::kVStages], ((j - 1) / PL::kVStages) & 1u)))
-          break;
-      }
+    uint32_t g = 0, gq = 0, steps[2] = {0, 0};  // K / V tiles and Q pairs used, P taken
+    Work it;
+    bool ok = true;
+    for (uint32_t k = 0; ok && next_work(bars, k, lane, p.status, it); ++k) {
+      const int n = it.j1 - it.j0;
+      if (n <= 0) continue;
+      if (!(ok = wait(&bars->q_full, gq & 1u))) break;
+      ++gq;
+      // step i: scores of key tile i, after the value product of tile i - 1
+      for (int i = 0; i <= n && ok; ++i) {
+        const uint32_t ks = (g + i) % PL::kKStages, vs = (g + i - 1) % PL::kVStages;
+        if (i < n && !(ok = wait(&bars->k_full[ks], ((g + i) / PL::kKStages) & 1u))) break;
+        if (i > 0 && !(ok = wait(&bars->v_full[vs], ((g + i - 1) / PL::kVStages) & 1u))) break;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (j > 0 && j - 1 < it.n[x]) {
-          if (!(ok = wait(&bars->p_full[x][0], (j - 1) & 1u))) break;
-          tc_fence_after();
-          issue_pv(x, j - 1, 0);
-          if (!(ok = wait(&bars->p_full[x][1], (j - 1) & 1u))) break;
-          tc_fence_after();
-          issue_pv(x, j - 1, 1);
+        for (int x = 0; x < 2; ++x) {
+          const int left = it.end[x] - it.j0;  // tiles of this Q tile
+          if (i > 0 && i <= left) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              ok = ok && wait(&bars->p_full[x][part], steps[x] & 1u);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(x, vs, part, i == 1);
+            }
+            if (!ok) break;
+            ++steps[x];
+            if (i == left) tc_commit_warp(smem_u32(&bars->o_full[x]));
+          }
+          if (i < left) {
+            tc_fence_after();
+            issue_qk(x, ks);
+          }
         }
-        if (j < it.n[x]) {
-          tc_fence_after();
-          issue_qk(x, j);
-        }
+        if (!ok) break;
+        if (i > 0) tc_commit_warp(smem_u32(&bars->v_empty[vs]));
+        if (i < n) tc_commit_warp(smem_u32(&bars->k_empty[ks]));
+        if (i == n - 1) tc_commit_warp(smem_u32(&bars->q_empty));
       }
-      if (!ok) break;
-      if (j > 0) tc_commit_warp(smem_u32(&bars->v_empty[(j - 1) % PL::kVStages]));
-      if (j < n_max) tc_commit_warp(smem_u32(&bars->k_empty[j % PL::kKStages]));
+      g += n;
     }
     // every issued MMA must finish before TMEM is released
     tc_commit_warp(smem_u32(&bars->drain));
@@ -653,6 +851,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Merge of a row's partial results (splits > 1), one warp per row.
+template <typename T>
+__global__ void __launch_bounds__(128) prompt_merge_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int64_t rows = static_cast<int64_t>(p.hq) * p.total_q;
+  if (row >= rows) return;
+  const int head = static_cast<int>(row / p.total_q), tok = static_cast<int>(row % p.total_q);
+  if (tok >= __ldg(p.cu_q + p.batch)) return;  // of no sequence: not written
+  const int lane = threadIdx.x & 31;
+  MergeState st;
+  st.init();
+  fold_parts<false, 2>(st, p.part_o, p.part_lse, 0, 0, 1, p.splits, rows * p.d_v, rows, row * p.d_v,
+                       row, p.d_v, lane);
+  const float l = finish_row<T>(
+      st, p.d_v, static_cast<T *>(p.o) + static_cast<int64_t>(tok) * p.o_st + head * p.o_sh, lane);
+  if (p.lse && lane == 0) p.lse[row] = l;
+}
+
 template <typename T, int kDqk, int kDv>
 cudaError_t launch_t(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm,
                      const Params &p, unsigned grid, cudaStream_t stream) {
@@ -661,7 +878,18 @@ cudaError_t launch_t(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kern<<<grid, kThreads, smem, stream>>>(qm, km, vm, p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess || p.splits == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.hq) * p.total_q + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prompt_merge_kernel<T>, p);
 }
 
 template <typename T>
@@ -679,8 +907,41 @@ int prompt_tile_tokens(const fa_prompt_args *a) {
   return prompt::kTile / (a->num_q_heads / a->num_kv_heads);
 }
 
+// Upper bound of the (sequence, Q tile pair) items: the sum over sequences of
+// ceil(tokens / span) with span = the tokens of a pair.
+int64_t prompt_items(const fa_prompt_args *a) {
+  return a->total_q / (2 * prompt_tile_tokens(a)) + a->batch;
+}
+
+// Units an item's keys are cut into when there are fewer items than SMs (few
+// new tokens over many keys).  In steps of one key tile (about 1.7 us): a unit
+// of n tiles costs n + 4, units run in rounds of one per SM, and the partial
+// rows are written and read once.  The count with the lowest estimate.
+int prompt_splits(const fa_prompt_args *a, int sms) {
+  const int64_t span = 2 * prompt_tile_tokens(a);
+  const int64_t items = std::max<int64_t>((a->total_q + span - 1) / span, a->batch);
+  const int64_t units = items * a->num_kv_heads;
+  if (units >= sms || a->batch == 0) return 1;
+  const int64_t seen = a->causal ? a->total_k - std::min(a->total_q, a->total_k) / 2 : a->total_k;
+  const int64_t tiles = seen / a->batch / prompt::kTile;
+  const double row_bytes = 8.0 * a->num_q_heads * a->total_q * a->d_v;  // written and read, f32
+  int best = 1;
+  double best_cost = static_cast<double>(tiles + 4);
+  for (int s = 2; s <= 32 && tiles / s >= 4; ++s) {
+    const double rounds = static_cast<double>((units * s + sms - 1) / sms);
+    const double cost =
+        rounds * (static_cast<double>(tiles) / s + 4) + 2 + s * row_bytes / (1.7 * 5.0e6);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
 cudaError_t launch_prompt(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm,
-                          const fa_prompt_args *a, cudaStream_t stream) {
+                          const fa_prompt_args *a, int splits, float *part_o, float *part_lse,
+                          cudaStream_t stream) {
   prompt::Params p;
   p.cu_q = a->cu_q;
   p.cu_k = a->cu_k;
@@ -699,9 +960,15 @@ cudaError_t launch_prompt(const CUtensorMap &qm, const CUtensorMap &km, const CU
   p.o_sh = a->o_stride_h;
   p.lse = a->lse;
   p.status = a->status;
-  // sum over sequences of ceil(tokens / span) is at most this
-  const int64_t items = a->total_q / (2 * p.tq) + a->batch;
-  const int64_t grid = items * a->num_kv_heads;
+  p.items = static_cast<int32_t>(prompt_items(a));
+  p.splits = splits;
+  p.part_o = part_o;
+  p.part_lse = part_lse;
+  // kv heads at a time whose keys and values stay in L2 (half of 126 MB)
+  const int64_t head_bytes = static_cast<int64_t>(a->total_k) * (a->d_qk + a->d_v) * 2 + 1;
+  p.section = static_cast<int32_t>(
+      std::min<int64_t>(std::max<int64_t>((int64_t{63} << 20) / head_bytes, 1), a->num_kv_heads));
+  const int64_t grid = static_cast<int64_t>(p.items) * splits * a->num_kv_heads;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
   return a->dtype == FA_DTYPE_F16
              ? prompt::launch_d<__half>(qm, km, vm, p, a->d_qk, static_cast<unsigned>(grid), stream)

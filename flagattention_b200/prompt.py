@@ -10,6 +10,7 @@ only, as every operator of this package.
 """
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -25,6 +26,18 @@ def _rows16(x):
     if d == 1 and t and h and not (t | h | (x.data_ptr() >> 1)) & 7:
         return x
     return x.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device_index, batch, total_q, total_k, hq, hk, d_v, causal):
+    """Scratch of a call of these sizes on this device."""
+    a = _lib.PromptArgs(batch=batch, total_q=total_q, total_k=total_k, num_q_heads=hq,
+                        num_kv_heads=hk, d_v=d_v, causal=causal)
+    size = ctypes.c_size_t(0)
+    with torch.cuda.device(device_index):
+        _lib.check(_lib.lib().fa_prompt_workspace_size(ctypes.byref(a), ctypes.byref(size)),
+                   "fa_prompt_workspace_size")
+    return size.value
 
 
 def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_scale=None,
@@ -65,19 +78,23 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
             cu_seqlens_k.get_device() != dev:
         raise _lib.InvalidArgument("all tensors must be on one device")
     code = dtype_code(q)
+    batch = cu_seqlens_q.shape[0] - 1
+    causal = 1 if causal else 0
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     out = q.new_empty((total_q, hq, d_v))
     lse = q.new_empty((hq, total_q), dtype=torch.float32) if return_lse else None
+    size = _workspace_bytes(dev, batch, total_q, total_k, hq, hk, d_v, causal) \
+        if hq // hk <= 128 and 0 < d_v <= 128 else 0
+    ws = q.new_empty((size,), dtype=torch.uint8) if size else None
     (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _) = q.stride(), k.stride(), v.stride()
     # field order of fa_prompt_args
     a = _lib.PromptArgs(q.data_ptr(), q_t, q_h, k.data_ptr(), k_t, k_h, v.data_ptr(), v_t, v_h,
                         cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-                        cu_seqlens_q.shape[0] - 1, total_q, total_k, hq, hk, d, d_v,
-                        1 if causal else 0, code,
+                        batch, total_q, total_k, hq, hk, d, d_v, causal, code,
                         1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
                         out.data_ptr(), hq * d_v, d_v, lse.data_ptr() if return_lse else None,
-                        status_ptr(dev))
+                        ws.data_ptr() if size else None, status_ptr(dev))
     st = _lib.lib().fa_prompt_attention(ctypes.byref(a), raw_stream(dev))
     if st:
         _lib.check(st, "fa_prompt_attention")

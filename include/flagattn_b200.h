@@ -192,8 +192,13 @@ typedef struct fa_prompt_args {
   void *o;
   int64_t o_stride_t, o_stride_h;
   float *lse;
-  int *status; /* nullable device status word (kernel time-outs) */
+  void *workspace; /* fa_prompt_workspace_size bytes, 16-byte aligned        */
+  int *status;     /* nullable device status word (kernel time-outs)         */
 } fa_prompt_args;
+/* Scratch of a call: 0 unless few new tokens meet many keys, whose key ranges
+ * are then cut over the SMs and merged by a second launch (f32 partials).
+ * Depends on the sizes only, not on pointers. */
+int fa_prompt_workspace_size(const fa_prompt_args *args, size_t *bytes);
 int fa_prompt_attention(const fa_prompt_args *args, void *stream);
 
 /* ---- 4-bit key / value cache ----------------------------------------------
