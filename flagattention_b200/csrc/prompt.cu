@@ -78,7 +78,7 @@ struct Work {
 };
 
 struct Bars {
-  uint64_t q_full, q_empty;
+  uint64_t q_full[2], q_empty[2];  // per Q tile
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t s_full[2], o_full[2];
   uint64_t p_full[2][2];  // [Q tile][first / last 32 columns of both halves]
@@ -297,9 +297,9 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
       }
     }
     // Value rows past the sequence's end belong to the next sequence and may
-    // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them.
-    // The first Q tile that uses this V tile does so (its P V goes first).
-    if (quad == 0 && half == 0 && it.lk < (j + 1) * kTile && (x == 0 || j >= it.end[0])) {
+    // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them
+    // (both Q tiles do, before their own products; either may come first).
+    if (quad == 0 && half == 0 && it.lk < (j + 1) * kTile) {
       const uint32_t v_tile = tiles + (j - it.j0);
       const int st = v_tile % PL::kVStages;
       warp_wait(smem_u32(&bars->v_full[st]), (v_tile / PL::kVStages) & 1u, abort_flag, p.status,
@@ -650,21 +650,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
 
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&bars->q_full), 1);
-    mbar_init(smem_u32(&bars->q_empty), 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&bars->k_full[i]), 1);
-      mbar_init(smem_u32(&bars->k_empty[i]), 1);
+      mbar_init(smem_u32(&bars->k_empty[i]), 2);  // once per Q tile
       mbar_init(smem_u32(&bars->v_full[i]), 1);
-      mbar_init(smem_u32(&bars->v_empty[i]), 1);
+      mbar_init(smem_u32(&bars->v_empty[i]), 2);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->q_full[i]), 1);
+      mbar_init(smem_u32(&bars->q_empty[i]), 1);
       mbar_init(smem_u32(&bars->s_full[i]), 1);
       mbar_init(smem_u32(&bars->p_full[i][0]), 8);
       mbar_init(smem_u32(&bars->p_full[i][1]), 8);
       mbar_init(smem_u32(&bars->o_full[i]), 1);
       mbar_init(smem_u32(&bars->work_full[i]), 1);
-      mbar_init(smem_u32(&bars->work_empty[i]), kRowWarps + 2);  // rows, MMA, producer
+      mbar_init(smem_u32(&bars->work_empty[i]), kRowWarps + 3);  // rows, producer, MMA twice
     }
     mbar_init(smem_u32(&bars->cancel_full), 1);
     mbar_init(smem_u32(&bars->drain), 1);
@@ -695,30 +695,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kSchedulerWarp) scheduler_role(p, bars, lane);
   } else if (warp == kProducerWarp) {
     give_registers<kOtherRegs>();
-    uint32_t g = 0, gv = 0, gq = 0;  // K tiles, V tiles, Q pairs issued
+    uint32_t g = 0, gv = 0, gq[2] = {0, 0};  // K tiles, V tiles, Q tiles issued
     if (lane == 0) {
       tma_prefetch_desc(&q_map);
       tma_prefetch_desc(&k_map);
       tma_prefetch_desc(&v_map);
     }
-    Work it;
+    Work it{};
     bool ok = true;
+    auto load_q = [&](int x) {
+      if (it.end[x] <= it.j0) return;
+      if (!(ok = warp_wait(smem_u32(&bars->q_empty[x]), (gq[x] & 1u) ^ 1u, abort_flag, p.status,
+                           kDevTimeoutProducer)))
+        return;
+      if (lane == 0) {
+        const uint32_t qf = smem_u32(&bars->q_full[x]);
+        mbar_arrive_expect_tx(qf, PL::kQkChunks * p.tq * p.group * 128);
+#pragma unroll
+        for (int ch = 0; ch < PL::kQkChunks; ++ch)
+          tma_load_3d(qbase + x * PL::kQBytes + ch * PL::kChunkBytes, &q_map, qf, ch * 64,
+                      it.kvh * p.group, it.q0 + it.i0 + x * p.tq);
+      }
+      ++gq[x];
+    };
     for (uint32_t k = 0; ok && next_work(bars, k, lane, p.status, it); ++k) {
       if (it.j1 <= it.j0) continue;
-      if (!(ok = warp_wait(smem_u32(&bars->q_empty), (gq & 1u) ^ 1u, abort_flag, p.status,
-                           kDevTimeoutProducer)))
-        break;
-      const uint32_t qf = smem_u32(&bars->q_full);
-      const int qtiles = it.end[1] > it.j0 ? 2 : 1;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(qf, qtiles * PL::kQkChunks * p.tq * p.group * 128);
-        for (int x = 0; x < qtiles; ++x)
-          for (int ch = 0; ch < PL::kQkChunks; ++ch)
-            tma_load_3d(qbase + x * PL::kQBytes + ch * PL::kChunkBytes, &q_map, qf, ch * 64,
-                        it.kvh * p.group, it.q0 + it.i0 + x * p.tq);
-      }
-      ++gq;
-      for (int j = it.j0; j < it.j1; ++j) {
+      load_q(0);
+      for (int j = it.j0; ok && j < it.j1; ++j) {
         const uint32_t ks = g % PL::kKStages, vs = gv % PL::kVStages;
         if (!(ok = warp_wait(smem_u32(&bars->k_empty[ks]), ((g / PL::kKStages) & 1u) ^ 1u,
                              abort_flag, p.status, kDevTimeoutProducer)))
@@ -732,6 +735,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.k0 + j * kTile, it.kvh);
         }
         ++g;
+        if (j == it.j0) {  // Q tile 1 of the last unit may be in use a little longer
+          load_q(1);
+          if (!ok) break;
+        }
         if (!(ok = warp_wait(smem_u32(&bars->v_empty[vs]), ((gv / PL::kVStages) & 1u) ^ 1u,
                              abort_flag, p.status, kDevTimeoutProducer)))
           break;
@@ -749,7 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (*abort_flag) {
       // copies in flight must land before the CTA may exit
       volatile int never = 0;
-      if (gq) wait_inline(smem_u32(&bars->q_full), (gq - 1) & 1u, &never, nullptr, 0);
+      for (int x = 0; x < 2; ++x)
+        if (gq[x]) wait_inline(smem_u32(&bars->q_full[x]), (gq[x] - 1) & 1u, &never, nullptr, 0);
       for (uint32_t t = g > PL::kKStages ? g - PL::kKStages : 0; t < g; ++t)
         wait_inline(smem_u32(&bars->k_full[t % PL::kKStages]), (t / PL::kKStages) & 1u, &never,
                     nullptr, 0);
@@ -766,8 +774,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t q_desc = smem_desc_swz(qbase, 16, 1024, 2);
     const uint64_t k_desc = smem_desc_swz(kbase, 16, 1024, 2);
     const uint64_t v_desc = smem_desc_swz(vbase, PL::kChunkBytes, 1024, 2);
-    auto wait = [&](uint64_t *bar, uint32_t parity) {
-      return warp_wait(smem_u32(bar), parity, abort_flag, p.status, kDevTimeoutMma);
+    auto ready = [&](const uint64_t *bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_probe(smem_u32(bar), parity)) != 0;
     };
     // S of Q tile x and the key tile in stage st
     auto issue_qk = [&](int x, uint32_t st) {
@@ -796,46 +804,116 @@ __global__ void __launch_bounds__(kThreads, 1)
                      (first && part == 0 && i == 0) ? 0u : 1u);
       }
     };
-    uint32_t g = 0, gq = 0, steps[2] = {0, 0};  // K / V tiles and Q pairs used, P taken
-    Work it;
-    bool ok = true;
-    for (uint32_t k = 0; ok && next_work(bars, k, lane, p.status, it); ++k) {
-      const int n = it.j1 - it.j0;
-      if (n <= 0) continue;
-      if (!(ok = wait(&bars->q_full, gq & 1u))) break;
-      ++gq;
-      // step i: scores of key tile i, after the value product of tile i - 1
-      for (int i = 0; i <= n && ok; ++i) {
-        const uint32_t ks = (g + i) % PL::kKStages, vs = (g + i - 1) % PL::kVStages;
-        if (i < n && !(ok = wait(&bars->k_full[ks], ((g + i) / PL::kKStages) & 1u))) break;
-        if (i > 0 && !(ok = wait(&bars->v_full[vs], ((g + i - 1) / PL::kVStages) & 1u))) break;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int left = it.end[x] - it.j0;  // tiles of this Q tile
-          if (i > 0 && i <= left) {
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              ok = ok && wait(&bars->p_full[x][part], steps[x] & 1u);
-              if (!ok) break;
-              tc_fence_after();
-              issue_pv(x, vs, part, i == 1);
-            }
-            if (!ok) break;
-            ++steps[x];
-            if (i == left) tc_commit_warp(smem_u32(&bars->o_full[x]));
-          }
-          if (i < left) {
-            tc_fence_after();
-            issue_qk(x, ks);
-          }
-        }
-        if (!ok) break;
-        if (i > 0) tc_commit_warp(smem_u32(&bars->v_empty[vs]));
-        if (i < n) tc_commit_warp(smem_u32(&bars->k_empty[ks]));
-        if (i == n - 1) tc_commit_warp(smem_u32(&bars->q_empty));
+    // The two Q tiles are independent streams of products, each waiting for
+    // its own rows: one tile's next unit starts while the other still ends
+    // its last.  While both wait for their rows they are served in turn.
+    enum Need { kUnit, kQK, kP, kNone };
+    struct Stream {
+      Need need = kUnit;
+      uint32_t unit = 0, g = 0, q = 0, steps = 0;  // units, K / V tiles, Q tiles begun; P taken
+      int i = 0, left = 0, n = 0, other = 0;       // step; steps of this tile, the unit, the other tile
+    } st0, st1;
+    // stage released by this tile, and for the other one where it has no such step
+    auto release = [&](uint64_t *empty, const Stream &s) {
+      tc_commit_warp(smem_u32(empty));
+      if (s.i >= s.other && lane == 0) mbar_arrive(smem_u32(empty));
+    };
+    // whatever needs no rows: the next unit, the next scores
+    auto feed = [&](int x, Stream &s) -> bool {
+      bool moved = false;
+      while (s.need == kUnit) {
+        const uint32_t slot = s.unit & 1u;
+        if (!ready(&bars->work_full[slot], (s.unit >> 1) & 1u)) return moved;
+        const Work &w = bars->work[slot];
+        const bool none = w.kvh < 0;
+        s.g += s.n;
+        s.i = 0;
+        s.n = none ? 0 : w.j1 - w.j0;
+        s.left = none ? 0 : w.end[x] - w.j0;
+        s.other = none ? 0 : w.end[x ^ 1] - w.j0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->work_empty[slot]));
+        ++s.unit;
+        s.need = none ? kNone : (s.left > 0 ? kQK : kUnit);
+        moved = true;
       }
-      g += n;
+      if (s.need == kQK) {
+        const uint32_t t = s.g + s.i, ks = t % PL::kKStages;
+        if (s.i == 0 && !ready(&bars->q_full[x], s.q & 1u)) return moved;
+        if (!ready(&bars->k_full[ks], (t / PL::kKStages) & 1u)) return moved;
+        tc_fence_after();
+        issue_qk(x, ks);
+        release(&bars->k_empty[ks], s);
+        if (s.i == s.left - 1) {
+          tc_commit_warp(smem_u32(&bars->q_empty[x]));
+          ++s.q;
+        }
+        s.need = kP;
+        moved = true;
+      }
+      return moved;
+    };
+    auto wait = [&](const uint64_t *bar, uint32_t parity) {
+      return warp_wait(smem_u32(bar), parity, abort_flag, p.status, kDevTimeoutMma);
+    };
+    // the first part of this step's P is there (or waited for); then its value
+    // product and the next scores
+    auto serve = [&](int x, Stream &s) -> bool {
+      const uint32_t t = s.g + s.i, vs = t % PL::kVStages;
+      if (!wait(&bars->p_full[x][0], s.steps & 1u)) return false;
+      tc_fence_after();
+      issue_pv(x, vs, 0, s.i == 0);
+      if (!wait(&bars->p_full[x][1], s.steps & 1u)) return false;
+      tc_fence_after();
+      issue_pv(x, vs, 1, false);
+      ++s.steps;
+      if (s.i == s.left - 1) tc_commit_warp(smem_u32(&bars->o_full[x]));
+      release(&bars->v_empty[vs], s);
+      s.need = ++s.i < s.left ? kQK : kUnit;
+      feed(x, s);
+      return true;
+    };
+    int turn = 0;
+    long long idle = 0;  // since when nothing has moved (0: it has)
+    while (st0.need != kNone || st1.need != kNone) {
+      // A tile can be served once its V tile is there: a tile that is ahead of
+      // the other waits for stages the other has yet to release, so the issuer
+      // must not block on it.
+      auto v_ready = [&](const Stream &s) {
+        const uint32_t t = s.g + s.i;
+        return ready(&bars->v_full[t % PL::kVStages], (t / PL::kVStages) & 1u);
+      };
+      const bool w0 = st0.need == kP && v_ready(st0), w1 = st1.need == kP && v_ready(st1);
+      // serve tile 0 / 1 (blocking on its rows): its turn while both could be,
+      // or the other has no work left; otherwise only when its rows are done
+      const bool go0 = w0 && (w1 ? turn == 0 : st1.need == kNone ||
+                                                   ready(&bars->p_full[0][0], st0.steps & 1u));
+      const bool go1 = !go0 && w1 && (w0 ? turn == 1 : st0.need == kNone ||
+                                                           ready(&bars->p_full[1][0], st1.steps & 1u));
+      if (go0) {
+        if (!serve(0, st0)) break;
+        turn = 1;
+      } else if (go1) {
+        if (!serve(1, st1)) break;
+        turn = 0;
+      }
+      bool moved = go0 || go1;
+      if (st0.need < kP) moved |= feed(0, st0);
+      if (st1.need < kP) moved |= feed(1, st1);
+      if (moved) {
+        idle = 0;
+        continue;
+      }
+      const long long now = clock64();
+      if (idle == 0) idle = now;
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+      if (__any_sync(0xffffffffu, now - idle > kWaitLimitCycles)) {
+        *abort_flag = 1;
+        if (lane == 0 && p.status) atomicExch(p.status, kDevTimeoutMma);
+        break;
+      }
     }
+    __syncwarp();
     // every issued MMA must finish before TMEM is released
     tc_commit_warp(smem_u32(&bars->drain));
     volatile int never = 0;
