@@ -39,9 +39,6 @@ namespace prompt {
 // registers to the row warps: 16 * 112 + 4 * 32 = 20 * 96, the launch's.
 constexpr int kThreads = 640, kRowRegs = 112, kOtherRegs = 32;
 constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17, kSchedulerWarp = 18;
-// Of every 8 pairs of columns this many take their exponentials on the FMA
-// pipes instead of the special-function unit.
-constexpr int kFmaPairs = 2;
 constexpr int kTile = 128;                 // rows of a Q tile, keys of a K / V tile
 constexpr uint32_t kTmemCols = 512;
 // O is rescaled only when the maximum grows by more than this (log2 units):
@@ -81,7 +78,7 @@ struct Bars {
   uint64_t q_full[2], q_empty[2];  // per Q tile
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t s_full[2], o_full[2];
-  uint64_t p_full[2][2];  // [Q tile][first / last 32 columns of both halves]
+  uint64_t p_full[2][2];  // [Q tile][first 48 / last 16 columns of both halves]
   uint64_t work_full[2], work_empty[2];
   uint64_t cancel_full;
   uint64_t drain;
@@ -152,40 +149,6 @@ __device__ __forceinline__ void give_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-// 2^x for kN pairs of x >= -126 without the special-function unit: x = n + f
-// with n the nearest integer (adding 1.5 * 2^23 leaves n in the low mantissa
-// bits), 2^f by a polynomial of degree 4 (minimax in relative error on [-1/2,
-// 1/2], Remez exchange: 2.6e-6, below the rounding of P to 16 bits), n added
-// to the exponent field.  Written step by step over all pairs: the chains are
-// independent and hide one another's latency.
-template <int kN>
-__device__ __forceinline__ void exp2_pairs(uint64_t (&x)[kN]) {
-  constexpr float kMagic = 12582912.f;
-  const float k[5] = {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f,
-                      0.05591785907745361f, 0.009570102207362652f};
-  const uint64_t magic = f32x2(kMagic, kMagic);
-  uint64_t r[kN], y[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) r[i] = fadd2(x[i], magic);
-#pragma unroll
-  for (int i = 0; i < kN; ++i) y[i] = fadd2(r[i], f32x2(-kMagic, -kMagic));
-#pragma unroll
-  for (int i = 0; i < kN; ++i) x[i] = ffma2(y[i], f32x2(-1.f, -1.f), x[i]);
-#pragma unroll
-  for (int i = 0; i < kN; ++i) y[i] = ffma2(x[i], f32x2(k[4], k[4]), f32x2(k[3], k[3]));
-#pragma unroll
-  for (int d = 2; d >= 0; --d)
-#pragma unroll
-    for (int i = 0; i < kN; ++i) y[i] = ffma2(y[i], x[i], f32x2(k[d], k[d]));
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    float r0, r1, y0, y1;
-    f32x2_split(r[i], r0, r1);
-    f32x2_split(y[i], y0, y1);
-    x[i] = f32x2(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(r0) << 23)),
-                 __uint_as_float(__float_as_uint(y1) + (__float_as_uint(r1) << 23)));
-  }
-}
 // Named barrier that returns whether any of its threads' predicates holds.
 __device__ __forceinline__ bool barrier_any(int id, int threads, bool pred) {
   uint32_t any;
@@ -266,14 +229,14 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
     // The two halves of a row share one maximum.  It is exchanged through
     // shared memory only when some row of the two warps needs a new one; the
     // barrier itself tells.
-    bool resc = false;
-    float alpha = 1.f;
     if (barrier_any(meet, 64, j == it.j0 || m_row * p.scale_log2 > m_use + kRescaleThreshold)) {
       *mine = m_row;
       named_bar_sync(meet, 64);
       m_row = max3_nan(m_row, *other, *other);
       named_bar_sync(meet, 64);  // read before the next exchange writes
       const float m_tile = m_row * p.scale_log2;
+      bool resc = false;
+      float alpha = 1.f;
       if (j == it.j0) {
         m_use = m_tile;
       } else if (m_tile > m_use + kRescaleThreshold) {
@@ -282,18 +245,18 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
         l *= alpha;
         m_use = m_tile;
       }
-    }
-    if (__any_sync(0xffffffffu, resc)) {
-      const float a = resc ? alpha : 1.f;
+      if (__any_sync(0xffffffffu, resc)) {
+        const float a = resc ? alpha : 1.f;
 #pragma unroll 1
-      for (int c = 0; c < kOCols / 16; ++c) {
-        float v[16];
-        uint32_t u[16];
-        tmem_ld16(t_o + 16 * c, v);
-        tmem_wait_ld();
+        for (int c = 0; c < kOCols / 16; ++c) {
+          float v[16];
+          uint32_t u[16];
+          tmem_ld16(t_o + 16 * c, v);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i] * a);
-        tmem_st16(t_o + 16 * c, u);
+          for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i] * a);
+          tmem_st16(t_o + 16 * c, u);
+        }
       }
     }
     // Value rows past the sequence's end belong to the next sequence and may
@@ -318,33 +281,17 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
     const uint64_t nm2 = f32x2(-msafe, -msafe);
     uint64_t acc2 = f32x2(0.f, 0.f), acc2b = f32x2(0.f, 0.f);
     // P over S in place, 32 columns at a time
-    // kPairs pairs of columns of v from the first on, to words of w
-    auto exps = [&](auto fma_pairs, const float *v, uint32_t *w) {
-      constexpr int kF = decltype(fma_pairs)::value;  // the first pairs go to the FMA pipes
-      constexpr int kPairs = 8;
-      uint64_t y[kPairs];
+    // 16 columns of v to 8 words of w
+    auto exps = [&](const float *v, uint32_t *w) {
+      uint64_t y[8];
 #pragma unroll
-      for (int c = 0; c < kPairs; ++c) y[c] = ffma2(f32x2(v[2 * c], v[2 * c + 1]), c2, nm2);
-#pragma unroll
-      for (int c = kF; c < kPairs; ++c) {
+      for (int c = 0; c < 8; ++c) {
         float x0, x1;
-        f32x2_split(y[c], x0, x1);
+        f32x2_split(ffma2(f32x2(v[2 * c], v[2 * c + 1]), c2, nm2), x0, x1);
         y[c] = f32x2(fast_exp2(x0), fast_exp2(x1));
       }
-      if constexpr (kF > 0) {
-        uint64_t z[kF];
 #pragma unroll
-        for (int c = 0; c < kF; ++c) {
-          float x0, x1;
-          f32x2_split(y[c], x0, x1);
-          z[c] = f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-        }
-        exp2_pairs<kF>(z);
-#pragma unroll
-        for (int c = 0; c < kF; ++c) y[c] = z[c];
-      }
-#pragma unroll
-      for (int c = 0; c < kPairs; ++c) {
+      for (int c = 0; c < 8; ++c) {
         float p0, p1;
         f32x2_split(y[c], p0, p1);
         w[c] = Elem<T>::pack2(p0, p1);
@@ -354,29 +301,24 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
           acc2 = fadd2(acc2, y[c]);
       }
     };
-    // P of 32 columns (and the rescaled O, the cleared V) is there: the value
-    // product of the first columns starts while the last are computed
+    // P of the first 48 or the last 16 columns (and the rescaled O, the cleared
+    // V) is there: most of the value product runs while the last are computed
     auto hand_over = [&](int part) {
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars->p_full[x][part]));
     };
-    auto all = [&](auto fma_pairs) {
-      uint32_t w[16], w2[16];
-      exps(fma_pairs, s, w);
-      exps(fma_pairs, s + 16, w + 8);
-      tmem_st16p(t_s, w);
-      exps(fma_pairs, s2, w2);  // hides the store's latency
-      hand_over(0);
-      exps(fma_pairs, s2 + 16, w2 + 8);
-      tmem_st16p(t_s + 16, w2);
-      hand_over(1);
-    };
-    if (masked)  // a masked weight has to be exactly 0
-      all(std::integral_constant<int, 0>());
-    else
-      all(std::integral_constant<int, kFmaPairs>());
+    uint32_t w[16], w2[16];
+    exps(s, w);
+    exps(s + 16, w + 8);
+    tmem_st16p(t_s, w);
+    exps(s2, w2);
+    tmem_st8p(t_s + 16, w2);
+    hand_over(0);
+    exps(s2 + 16, w2 + 8);
+    tmem_st8p(t_s + 24, w2 + 8);
+    hand_over(1);
     float a0, a1;
     f32x2_split(fadd2(acc2, acc2b), a0, a1);
     l += a0 + a1;
@@ -791,18 +733,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       tc_commit_warp(smem_u32(&bars->s_full[x]));
     };
-    // value product with the tile in stage st, K steps of the first (part 0)
-    // or last 32 columns of each half
+    // value product with the tile in stage st: K steps (16 keys each) 0 to 2 of
+    // both halves (part 0), or the last ones
     auto issue_pv = [&](int x, uint32_t st, int part, bool first) {
       const uint64_t vd = v_desc + static_cast<uint64_t>((st * PL::kVBytes) >> 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kk = (i / 2) * 4 + part * 2 + i % 2;  // 16 keys each
-        umma_ts_warp(tmem + PL::kColO + x * kDv,
-                     tmem + PL::kColS + x * kTile + (kk / 4) * (kTile / 2) + (kk % 4) * 8,
-                     vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
-                     (first && part == 0 && i == 0) ? 0u : 1u);
-      }
+      for (int i = part ? 3 : 0; i < (part ? 4 : 3); ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          umma_ts_warp(tmem + PL::kColO + x * kDv,
+                       tmem + PL::kColS + x * kTile + half * (kTile / 2) + i * 8,
+                       vd + static_cast<uint64_t>(((half * 4 + i) * 16 * 128) >> 4), kIdescPV,
+                       (first && i == 0 && half == 0) ? 0u : 1u);
     };
     // The two Q tiles are independent streams of products, each waiting for
     // its own rows: one tile's next unit starts while the other still ends
