@@ -55,13 +55,17 @@ __host__ __device__ constexpr int value_unit(int t, int u, int r, int half) {
   return (idx / 4) * 512 + (r * 4 + q) * 16 + (idx % 4) * 4 + (t % 2) * 2;
 }
 
-// Where a pool slot (block * block_size + offset) lives.
+// A pool of `slots` = num_blocks * block_size token slots, below 2^32, and
+// fewer than 2^31 tiles (either would be larger than the GPU's memory).
 struct Pool {
   uint8_t *data;
-  int64_t slots;  // num_blocks * block_size
-  int block_size, heads, tile_bytes;
-  __device__ __forceinline__ uint8_t *tile(int64_t block, int head, int tile_in_block) const {
-    return data + ((block * heads + head) * (block_size / kTileTokens) + tile_in_block) * tile_bytes;
+  uint32_t slots;
+  int block_size, tiles_per_block, heads, tile_bytes;
+  // x / tiles_per_block for x < 2^28, as (x * div_mul) >> div_shift
+  uint32_t div_mul, div_shift;
+  __device__ __forceinline__ uint8_t *tile(uint32_t block, int head, uint32_t tile_in_block) const {
+    const uint32_t at = (block * heads + head) * tiles_per_block + tile_in_block;
+    return data + static_cast<uint64_t>(at) * static_cast<uint32_t>(tile_bytes);
   }
 };
 

@@ -7,11 +7,15 @@
 // result does not depend on the launch.  A group that holds a NaN or an
 // infinity keeps lo = NaN and reads back as NaN: it is not lost silently.
 //
-// One segment of D / 8 lanes takes one row (token, kv head, keys or values):
-// a lane holds eight dims (one 16-byte load), a group's minimum and maximum
-// are shuffles inside the segment, and a lane's eight codes are one 32-bit
-// word of the tile (kv4.cuh).  Byte-bound: 2 D bytes of a row in, D / 2 + 4 D
-// / G out.
+// One segment of D / 8 lanes takes a token of one kv head, keys and values: a
+// lane holds eight dims of each (two 16-byte loads), a group's minimum and
+// maximum are shuffles inside the segment, and a lane's eight codes are one
+// 32-bit word of keys and two 16-bit units of values (kv4.cuh).  4 D bytes in,
+// D + 8 D / G out per token and head (the read in reverse).  At the HBM rate
+// the schedulers have about 200 instructions per 16 elements of a lane, the
+// integer pipes half of that, so per-element work is kept small: minima and
+// maxima two at a time in T, divisions as products with the group's
+// reciprocal corrected to the exact quotient, codes moved by multiply-adds.
 #include "kv4.cuh"
 #include "flagattn_b200.h"
 
@@ -20,7 +24,7 @@ int record_error(int status, const char *msg);  // capi.cu: message for fa_last_
 
 namespace kv4 {
 
-constexpr int kWarpsPerBlock = 8;
+constexpr int kThreadsPerBlock = 256;
 
 struct RowsIn {
   const void *k, *v;
@@ -31,141 +35,213 @@ struct RowsOut {
   int64_t k_st, k_sh, v_st, v_sh;
 };
 
-// Row of the calling lane: segment of D / 8 lanes = (token, head, keys / values).
-template <int kD>
-__device__ __forceinline__ bool locate(int64_t n, int heads, int64_t &tok, int &head, int &is_v,
-                                       int &j) {
-  constexpr int kSeg = kD / 8;
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * (32 * kWarpsPerBlock) + threadIdx.x;
-  const int64_t row = thread / kSeg;
-  j = static_cast<int>(thread % kSeg);
-  is_v = static_cast<int>(row & 1);
-  head = static_cast<int>((row >> 1) % heads);
-  tok = (row >> 1) / heads;
-  return tok < n;
+// Elementwise minimum of two packed pairs that keeps a NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
-// kD dims, groups of kG.
-template <typename T, int kD, int kG>
-__global__ void __launch_bounds__(32 * kWarpsPerBlock)
-    append_kernel(RowsIn in, const int64_t *__restrict__ slots, int64_t n, Pool pool) {
-  constexpr int kSeg = kD / 8, kGroups = kD / kG, kLanes = kG / 8;  // lanes of a group
-  int64_t tok;
-  int head, is_v, j;
-  const bool inside = locate<kD>(n, pool.heads, tok, head, is_v, j);
-  const int64_t slot = inside ? __ldg(slots + tok) : -1;
-  const bool live = slot >= 0 && slot < pool.slots;
-  float x[8];
-  bool bad = false;
-  float lo = INFINITY, hi = -INFINITY;
-  if (live) {
-    const T *src = is_v ? static_cast<const T *>(in.v) + tok * in.v_st + head * in.v_sh
-                        : static_cast<const T *>(in.k) + tok * in.k_st + head * in.k_sh;
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src) + j);
-    const T *e = reinterpret_cast<const T *>(&u);
+// Tile and row of a pool slot; false for a slot outside the pool.
+__device__ __forceinline__ bool find_slot(const Pool &pool, int64_t slot, int head, uint8_t *&tile,
+                                          int &t) {
+  if (static_cast<uint64_t>(slot) >= pool.slots) return false;  // negative ones too
+  const uint32_t x = static_cast<uint32_t>(slot) / kTileTokens;
+  const uint32_t block =
+      static_cast<uint32_t>((static_cast<uint64_t>(x) * pool.div_mul) >> pool.div_shift);
+  t = static_cast<int>(static_cast<uint32_t>(slot) % kTileTokens);
+  tile = pool.tile(block, head, x - block * pool.tiles_per_block);
+  return true;
+}
+
+// d / s correctly rounded, given r = 1 / s rounded: two corrections by the exact
+// remainder (Markstein's theorem, for an s whose significand is not all
+// ones and results away from underflow).
+__device__ __forceinline__ float quotient(float d, float s, float r) {
+  float q = d * r;
+  q = fmaf(fmaf(-q, s, d), r, q);
+  return fmaf(fmaf(-q, s, d), r, q);
+}
+
+// Codes of the lane's eight dims (u, 16 bits each), nibble i = dim i, and the
+// group's (lo, scale) pair.  All lanes of the warp take part.
+template <typename T, int kG>
+__device__ __forceinline__ uint32_t quantise(const uint4 &u, uint32_t &pair) {
+  constexpr int kLanes = kG / 8;  // of a group
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, half to even
+  constexpr uint32_t kSigns = 0x80008000u;
+  // {minimum, -maximum}: the minima of x and of -x
+  const uint32_t lows = min2_nan<T>(min2_nan<T>(u.x, u.y), min2_nan<T>(u.z, u.w));
+  const uint32_t highs = min2_nan<T>(min2_nan<T>(u.x ^ kSigns, u.y ^ kSigns),
+                                     min2_nan<T>(u.z ^ kSigns, u.w ^ kSigns));
+  uint32_t ends = min2_nan<T>(__byte_perm(lows, highs, 0x5410), __byte_perm(lows, highs, 0x7632));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = Elem<T>::to_f(e[i]);
-      bad |= !(fabsf(x[i]) < INFINITY);
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  }
-#pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad |= __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), o) != 0;
-  }
+  for (int o = 1; o < kLanes; o <<= 1)
+    ends = min2_nan<T>(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+  const T *end = reinterpret_cast<const T *>(&ends);
+  const float lo = Elem<T>::to_f(end[0]), hi = -Elem<T>::to_f(end[1]);
+  const bool finite = hi < INFINITY && lo > -INFINITY;  // false when a NaN came through
   // halves: max - min of finite bf16 values may pass the f32 range
-  const T scale = Elem<T>::from_f(__fdiv_rn(hi * 0.5f - lo * 0.5f, 7.5f));
-  const float s = Elem<T>::to_f(scale);
-  uint32_t word = 0;
-  if (!bad && s != 0.f) {
+  const float lo2 = lo * 0.5f, range2 = hi * 0.5f - lo2;
+  const bool normal = range2 >= 0x1p-90f;
+  const T scale =
+      Elem<T>::from_f(normal ? quotient(range2, 7.5f, 1.f / 7.5f) : __fdiv_rn(range2, 7.5f));
+  const float s2 = Elem<T>::to_f(scale) * 0.5f;
+  T both[2] = {finite ? end[0] : Elem<T>::from_f(NAN), finite ? scale : Elem<T>::from_f(0.f)};
+  pair = *reinterpret_cast<const uint32_t *>(both);
+  if (!finite || s2 == 0.f) return 0u;
+  const T *e = reinterpret_cast<const T *>(&u);
+  float n[8];
+  if (normal && s2 >= 0x1p-100f) {
+    // rint((x - lo) / s), at most 15: the scale is off by 2^-8 of itself at most
+    const float r = __frcp_rn(s2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(x[i] * 0.5f - lo * 0.5f, s * 0.5f));
-      word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
-    }
+    for (int i = 0; i < 8; ++i)
+      n[i] = (quotient(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2, r) + kMagic) - kMagic;
+  } else {  // a subnormal scale may be off by half: the quotient may pass 15
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      n[i] = rintf(fminf(__fdiv_rn(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2), 15.f));
   }
-  // the units (u, r, 0 / 1) gather four dims from each 32-dim half of their 64
-  const int r = j % 8;
-  const uint32_t w0 = __shfl_sync(0xffffffffu, word, (j & ~7) + r / 2, kSeg);
-  const uint32_t w1 = __shfl_sync(0xffffffffu, word, (j & ~7) + 4 + r / 2, kSeg);
-  if (!live) return;
-  const int64_t block = slot / pool.block_size;
-  const int off = static_cast<int>(slot % pool.block_size), t = off % kTileTokens;
-  uint8_t *tile = pool.tile(block, head, off / kTileTokens);
-  if (is_v) {  // byte `half` of the chosen 16-bit halves of w0, then of w1
+  // four codes to a 16-bit number in f32, exactly
+  const float a = fmaf(fmaf(fmaf(n[3], 16.f, n[2]), 16.f, n[1]), 16.f, n[0]);
+  const float b = fmaf(fmaf(fmaf(n[7], 16.f, n[6]), 16.f, n[5]), 16.f, n[4]);
+  return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
+}
+
+// kD dims, groups of kG.  Grid: token strides x kv heads; a segment takes every
+// gridDim.x-th block's token and loads the next one's rows ahead.
+template <typename T, int kD, int kG>
+__global__ void __launch_bounds__(kThreadsPerBlock)
+    append_kernel(RowsIn in, const int64_t *__restrict__ slots, int64_t n, Pool pool) {
+  constexpr int kSeg = kD / 8, kGroups = kD / kG, kLanes = kG / 8, kTok = kThreadsPerBlock / kSeg;
+  const int head = blockIdx.y, j = threadIdx.x % kSeg, r = j % 8, seg = threadIdx.x / kSeg;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTok;
+  int64_t tok = static_cast<int64_t>(blockIdx.x) * kTok + seg;
+  const T *k = static_cast<const T *>(in.k) + tok * in.k_st + head * in.k_sh + 8 * j;
+  const T *v = static_cast<const T *>(in.v) + tok * in.v_st + head * in.v_sh + 8 * j;
+  uint4 ku = make_uint4(0u, 0u, 0u, 0u), vu = ku;
+  int64_t slot = -1;
+  auto load = [&] {
+    slot = -1;
+    if (tok < n) {
+      slot = __ldg(slots + tok);
+      ku = __ldg(reinterpret_cast<const uint4 *>(k));
+      vu = __ldg(reinterpret_cast<const uint4 *>(v));
+    }
+  };
+  load();
+  // all lanes of a warp stay while its first segment has a token
+  for (int64_t first = tok - seg % (32 / kSeg); first < n; first += step) {
+    const uint4 kc = ku, vc = vu;
+    const int64_t at = slot;
+    tok += step;
+    k += step * in.k_st;
+    v += step * in.v_st;
+    load();
+    uint32_t kpair, vpair;
+    const uint32_t kword = quantise<T, kG>(kc, kpair), vword = quantise<T, kG>(vc, vpair);
+    // the units (u, r, 0 / 1) gather four dims from each 32-dim half of their 64
+    const uint32_t w0 = __shfl_sync(0xffffffffu, vword, (j & ~7) + r / 2, kSeg);
+    const uint32_t w1 = __shfl_sync(0xffffffffu, vword, (j & ~7) + 4 + r / 2, kSeg);
+    uint8_t *tile;
+    int t;
+    if (!find_slot(pool, at, head, tile, t)) continue;
+    *reinterpret_cast<uint32_t *>(tile + key_word<kD>(t, j)) = kword;
+    // byte `half` of the chosen 16-bit halves of w0, then of w1
     const uint32_t w = __byte_perm(w0, w1, (r & 1) ? 0x7362 : 0x5140);
 #pragma unroll
     for (int half = 0; half < 2; ++half)
       *reinterpret_cast<uint16_t *>(tile + code_bytes(kD) + value_unit<kD>(t, j / 8, r, half)) =
           static_cast<uint16_t>(w >> (16 * half));
-  } else {
-    *reinterpret_cast<uint32_t *>(tile + key_word<kD>(t, j)) = word;
-  }
-  if (j % kLanes == 0) {
-    T pair[2] = {bad ? Elem<T>::from_f(NAN) : Elem<T>::from_f(lo),
-                 bad ? Elem<T>::from_f(0.f) : scale};
-    *reinterpret_cast<uint32_t *>(tile + 2 * code_bytes(kD) + t * (8 * kGroups) +
-                                  (is_v * kGroups + j / kLanes) * 4) =
-        *reinterpret_cast<const uint32_t *>(pair);
+    if (j % kLanes == 0) {
+      uint32_t *pairs = reinterpret_cast<uint32_t *>(tile + 2 * code_bytes(kD) + t * (8 * kGroups));
+      pairs[j / kLanes] = kpair;
+      pairs[kGroups + j / kLanes] = vpair;
+    }
   }
 }
 
-template <typename T, int kD, int kG>
-__global__ void __launch_bounds__(32 * kWarpsPerBlock)
-    read_kernel(Pool pool, const int64_t *__restrict__ slots, int64_t n, RowsOut out) {
-  constexpr int kSeg = kD / 8, kGroups = kD / kG, kLanes = kG / 8;
-  int64_t tok;
-  int head, is_v, j;
-  const bool inside = locate<kD>(n, pool.heads, tok, head, is_v, j);
-  const int64_t slot = inside ? __ldg(slots + tok) : -1;
-  const bool live = slot >= 0 && slot < pool.slots;
-  uint32_t word = 0;
-  float lo = 0.f, s = 0.f;
-  const int r = j % 8;
-  if (live) {
-    const int64_t block = slot / pool.block_size;
-    const int off = static_cast<int>(slot % pool.block_size), t = off % kTileTokens;
-    const uint8_t *tile = pool.tile(block, head, off / kTileTokens);
-    if (is_v) {
-      const uint8_t *codes = tile + code_bytes(kD);
-      word = *reinterpret_cast<const uint16_t *>(codes + value_unit<kD>(t, j / 8, r, 0)) |
-             static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(
-                 codes + value_unit<kD>(t, j / 8, r, 1))) << 16;
-    } else {
-      word = *reinterpret_cast<const uint32_t *>(tile + key_word<kD>(t, j));
-    }
-    const uint32_t pair = *reinterpret_cast<const uint32_t *>(
-        tile + 2 * code_bytes(kD) + t * (8 * kGroups) + (is_v * kGroups + j / kLanes) * 4);
-    const T *e = reinterpret_cast<const T *>(&pair);
-    lo = Elem<T>::to_f(e[0]);
-    s = Elem<T>::to_f(e[1]);
-  }
-  // values: dims 8 j .. + 3 are one byte of both units of r = 2 (j % 4), the
-  // next four of r + 1; the byte is the 32-dim half p = (j / 4) % 2
-  const uint32_t w0 = __shfl_sync(0xffffffffu, word, (j & ~7) + 2 * (j % 4), kSeg);
-  const uint32_t w1 = __shfl_sync(0xffffffffu, word, (j & ~7) + 2 * (j % 4) + 1, kSeg);
-  if (!inside) return;
-  if (is_v) word = __byte_perm(w0, w1, ((j >> 2) & 1) ? 0x7531 : 0x6420);
+// Eight values lo + scale * code in T.
+template <typename T>
+__device__ __forceinline__ uint4 expand(uint32_t word, uint32_t pair) {
+  const T *e = reinterpret_cast<const T *>(&pair);
+  const float lo = Elem<T>::to_f(e[0]), s = Elem<T>::to_f(e[1]);
   // lo + 15 * scale may pass the type's largest number by the scale's rounding
   const float top = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
-  auto value = [&](int i) {
-    const float x = fmaf(static_cast<float>((word >> (4 * i)) & 15u), s, lo);
-    return x > top ? top : x;  // false for a NaN
-  };
-  uint4 u;
-  uint32_t *o = reinterpret_cast<uint32_t *>(&u);
+  const bool over = fmaf(15.f, s, lo) > top;
+  // nibbles 0 to 4 are masked in place: 16^i c in the mantissa under the
+  // exponent of 2^23, with 16^i taken off the scale (exact); 5 to 7 after a shift
+  float si[5] = {s};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = Elem<T>::pack2(value(2 * i), value(2 * i + 1));
-  T *dst = is_v ? static_cast<T *>(out.v) + tok * out.v_st + head * out.v_sh
-                : static_cast<T *>(out.k) + tok * out.k_st + head * out.k_sh;
-  reinterpret_cast<uint4 *>(dst)[j] = u;
+  for (int i = 1; i < 5; ++i) si[i] = si[i - 1] * 0.0625f;
+  const uint32_t upper = word >> 20;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = i < 5 ? i : i - 5;
+    const float c = __uint_as_float(((i < 5 ? word : upper) & (15u << (4 * k))) | 0x4b000000u) - 8388608.f;
+    x[i] = fmaf(c, si[k], lo);
+  }
+  if (over) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] > top ? top : x[i];
+  }
+  return make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]),
+                    Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
+}
+
+template <typename T, int kD, int kG>
+__global__ void __launch_bounds__(kThreadsPerBlock)
+    read_kernel(Pool pool, const int64_t *__restrict__ slots, int64_t n, RowsOut out) {
+  constexpr int kSeg = kD / 8, kGroups = kD / kG, kLanes = kG / 8, kTok = kThreadsPerBlock / kSeg;
+  const int head = blockIdx.y, j = threadIdx.x % kSeg, r = j % 8, seg = threadIdx.x / kSeg;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTok;
+  int64_t tok = static_cast<int64_t>(blockIdx.x) * kTok + seg;
+  T *k = static_cast<T *>(out.k) + tok * out.k_st + head * out.k_sh + 8 * j;
+  T *v = static_cast<T *>(out.v) + tok * out.v_st + head * out.v_sh + 8 * j;
+  int64_t slot = tok < n ? __ldg(slots + tok) : -1;
+  uint32_t kword, kpair, vpair;
+  uint16_t v0, v1;
+  auto load = [&] {  // of `slot`; zeros for a slot outside the pool
+    kword = kpair = vpair = 0u;
+    v0 = v1 = 0;
+    uint8_t *tile;
+    int t;
+    if (!find_slot(pool, slot, head, tile, t)) return;
+    kword = *reinterpret_cast<const uint32_t *>(tile + key_word<kD>(t, j));
+    const uint8_t *codes = tile + code_bytes(kD);
+    v0 = *reinterpret_cast<const uint16_t *>(codes + value_unit<kD>(t, j / 8, r, 0));
+    v1 = *reinterpret_cast<const uint16_t *>(codes + value_unit<kD>(t, j / 8, r, 1));
+    const uint32_t *pairs =
+        reinterpret_cast<const uint32_t *>(tile + 2 * code_bytes(kD) + t * (8 * kGroups));
+    kpair = pairs[j / kLanes];
+    vpair = pairs[kGroups + j / kLanes];
+  };
+  load();
+  slot = tok + step < n ? __ldg(slots + tok + step) : -1;
+  for (int64_t first = tok - seg % (32 / kSeg); first < n; first += step) {
+    const uint32_t kw = kword, kp = kpair, vp = vpair, vword = v0 | static_cast<uint32_t>(v1) << 16;
+    const bool live = tok < n;
+    T *kd = k, *vd = v;
+    tok += step;
+    k += step * out.k_st;
+    v += step * out.v_st;
+    load();  // the next token's words, and the slot of the one after it
+    slot = tok + step < n ? __ldg(slots + tok + step) : -1;
+    // values: dims 8 j .. + 3 are one byte of both units of r = 2 (j % 4), the
+    // next four of r + 1; the byte is the 32-dim half p = (j / 4) % 2
+    const uint32_t w0 = __shfl_sync(0xffffffffu, vword, (j & ~7) + 2 * (j % 4), kSeg);
+    const uint32_t w1 = __shfl_sync(0xffffffffu, vword, (j & ~7) + 2 * (j % 4) + 1, kSeg);
+    if (!live) continue;
+    *reinterpret_cast<uint4 *>(kd) = expand<T>(kw, kp);
+    *reinterpret_cast<uint4 *>(vd) =
+        expand<T>(__byte_perm(w0, w1, ((j >> 2) & 1) ? 0x7531 : 0x6420), vp);
+  }
 }
 
 // Calls fn with (T, head size, group size) as types / constants of the cache.
@@ -201,6 +277,9 @@ int validate_cache(const fa_kv4_cache *c) {
     return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: block / head count");
   if (c->block_size <= 0 || c->block_size % kTileTokens)
     return record_error(FA_ERR_UNSUPPORTED, "kv4: block size must be a multiple of 16 tokens");
+  const int64_t slots = static_cast<int64_t>(c->num_blocks) * c->block_size;
+  if (slots > 0xffffffffll || slots / kTileTokens > 0x7fffffffll / c->num_kv_heads)
+    return record_error(FA_ERR_UNSUPPORTED, "kv4: pool of 2^32 slots or 2^31 tiles");
   if (reinterpret_cast<uintptr_t>(c->data) & 15u)
     return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: the pool must be 16-byte aligned");
   return FA_OK;
@@ -209,19 +288,26 @@ int validate_cache(const fa_kv4_cache *c) {
 Pool pool_of(const fa_kv4_cache *c) {
   Pool p;
   p.data = static_cast<uint8_t *>(c->data);
-  p.slots = static_cast<int64_t>(c->num_blocks) * c->block_size;
+  p.slots = static_cast<uint32_t>(static_cast<int64_t>(c->num_blocks) * c->block_size);
   p.block_size = c->block_size;
+  p.tiles_per_block = c->block_size / kTileTokens;
   p.heads = c->num_kv_heads;
   p.tile_bytes = tile_bytes(c->head_size, c->head_size / c->group_size);
+  // x < 2^28 and 2^(l - 1) < d <= 2^l: m = floor(2^(28 + l) / d) + 1 is below
+  // 2^30 and x * m >> (28 + l) is x / d, since m d - 2^(28 + l) <= d <= 2^l
+  uint32_t l = 0;
+  while ((1u << l) < static_cast<uint32_t>(p.tiles_per_block)) ++l;
+  p.div_shift = 28 + l;
+  p.div_mul = static_cast<uint32_t>((uint64_t{1} << p.div_shift) / p.tiles_per_block + 1);
   return p;
 }
 
 // Checks and grid shared by append and read: rows in either direction.
 int validate_rows(const fa_kv4_cache *c, const void *k, int64_t k_st, int64_t k_sh, const void *v,
-                  int64_t v_st, int64_t v_sh, const int64_t *slots, int64_t n, unsigned *grid) {
+                  int64_t v_st, int64_t v_sh, const int64_t *slots, int64_t n, dim3 *grid) {
   const int st = validate_cache(c);
   if (st != FA_OK) return st;
-  *grid = 0;
+  *grid = dim3(0);
   if (n < 0) return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: negative row count");
   if (n == 0) return FA_OK;
   if (!k || !v || !slots || (!c->data && c->num_blocks > 0))
@@ -232,12 +318,18 @@ int validate_rows(const fa_kv4_cache *c, const void *k, int64_t k_st, int64_t k_
                         "kv4: rows must be 16-byte aligned, slots 8-byte aligned");
   if (k_st % 8 || k_sh % 8 || v_st % 8 || v_sh % 8)
     return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: strides must be multiples of 8 elements");
-  const int64_t per_block = 32 * kWarpsPerBlock / (c->head_size / 8);
-  if (n > (int64_t{1} << 40) / c->num_kv_heads)
-    return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: too many rows");
-  const int64_t blocks = (n * c->num_kv_heads * 2 + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffLL) return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: too many rows");
-  *grid = static_cast<unsigned>(blocks);
+  const int64_t per_block = kThreadsPerBlock / (c->head_size / 8);
+  if (n > 0x7fffffffLL * per_block || c->num_kv_heads > 65535)
+    return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: too many rows or kv heads");
+  // at most eight blocks per SM (all resident): the rest of the tokens in strides
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
+  const int64_t most = (8 * sms + c->num_kv_heads - 1) / c->num_kv_heads;
+  const int64_t want = (n + per_block - 1) / per_block;
+  *grid = dim3(static_cast<unsigned>(want < most ? want : most),
+               static_cast<unsigned>(c->num_kv_heads));
   return FA_OK;
 }
 
@@ -262,14 +354,14 @@ extern "C" int fa_kv4_append(const fa_kv4_cache *c, const void *k, int64_t k_str
                              int64_t k_stride_h, const void *v, int64_t v_stride_t,
                              int64_t v_stride_h, const int64_t *slots, int64_t n, void *stream) {
   using namespace fa::kv4;
-  unsigned grid = 0;
+  dim3 grid;
   const int st = validate_rows(c, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, slots, n,
                                &grid);
-  if (st != FA_OK || grid == 0) return st;
+  if (st != FA_OK || grid.x == 0) return st;
   const RowsIn in{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h};
   return dispatch(c, [&](auto t, auto d, auto g) {
     append_kernel<decltype(t), d.value, g.value>
-        <<<grid, 32 * kWarpsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(in, slots, n,
+        <<<grid, kThreadsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(in, slots, n,
                                                                             pool_of(c));
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? FA_OK : fa::record_error(FA_ERR_CUDA, cudaGetErrorString(e));
@@ -280,14 +372,14 @@ extern "C" int fa_kv4_read(const fa_kv4_cache *c, void *k, int64_t k_stride_t, i
                            void *v, int64_t v_stride_t, int64_t v_stride_h, const int64_t *slots,
                            int64_t n, void *stream) {
   using namespace fa::kv4;
-  unsigned grid = 0;
+  dim3 grid;
   const int st = validate_rows(c, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, slots, n,
                                &grid);
-  if (st != FA_OK || grid == 0) return st;
+  if (st != FA_OK || grid.x == 0) return st;
   const RowsOut out{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h};
   return dispatch(c, [&](auto t, auto d, auto g) {
     read_kernel<decltype(t), d.value, g.value>
-        <<<grid, 32 * kWarpsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(pool_of(c), slots,
+        <<<grid, kThreadsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(pool_of(c), slots,
                                                                             n, out);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? FA_OK : fa::record_error(FA_ERR_CUDA, cudaGetErrorString(e));

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
 
     // every 32 tiles lane i looks up the pool tile of the warp's i-th next one
     // (-1: past the end, or a block outside the pool), one batch ahead
-    const int tiles_per_page = p.pool.block_size / kTileTokens;
+    const int tiles_per_page = p.pool.tiles_per_block;
     auto look_up = [&](int i0) {
       const int mine = (j0 + i0 + lane) * kWarps + warp;
       if (mine >= tiles_end || i0 + lane >= n) return -1;
@@ -736,10 +736,6 @@ int validate_attention(const fa_kv4_attention_args *a) {
   if (a->batch < 0 || a->num_q_heads <= 0 || a->num_q_heads % a->cache.num_kv_heads)
     return record_error(FA_ERR_INVALID_ARGUMENT,
                         "kv4 attention: query heads must be a multiple of the cache's kv heads");
-  int64_t bytes = 0;
-  fa_kv4_cache_bytes(&a->cache, &bytes);
-  if (bytes / tile_bytes(a->cache.head_size, a->cache.head_size / a->cache.group_size) > INT32_MAX)
-    return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: pool of more than 2^31 tiles");
   if (a->bt_width < 0 || a->bt_stride < 0)
     return record_error(FA_ERR_INVALID_ARGUMENT, "kv4 attention: block table shape");
   if (!(a->scale > 0.f) || std::isinf(a->scale))

@@ -119,6 +119,17 @@ def test_constant_extreme_and_non_finite_groups(dtype):
         assert (got[7].float() - x[7].float()).abs().max() <= 1 / 30 + 0.5 * (dtype == torch.bfloat16)
 
 
+def test_subnormal_ranges():
+    """Groups whose range is a few subnormal steps: the scale rounds to one too."""
+    cache = fa.Int4KVCache(1, 1, 16, 64)
+    steps = torch.arange(64, device="cuda") % torch.tensor([2, 7, 16, 40], device="cuda")[:, None]
+    x = (steps * 2.0 ** -133).to(torch.bfloat16)[:, None]  # bf16's smallest numbers
+    assert x.float().max() > 0
+    fa.append_kv_int4(x, x, cache, torch.arange(4, device="cuda"))
+    for got in fa.read_kv_int4(cache, torch.arange(4, device="cuda")):
+        assert same(got, values(x, 64).to(x.dtype))
+
+
 def build(lens, hq, hk, d, group, block, dtype, seed=0, size=1.0, pool_extra=3):
     """Cache with shuffled pages whose unused slots hold NaN scales and any
     codes, the query, and the rows of each sequence."""
