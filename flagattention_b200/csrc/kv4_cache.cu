@@ -24,7 +24,7 @@ int record_error(int status, const char *msg);  // capi.cu: message for fa_last_
 
 namespace kv4 {
 
-constexpr int kThreadsPerBlock = 256;
+constexpr int kThreadsPerBlock = 256, kBlocksPerSm = 4;
 
 struct RowsIn {
   const void *k, *v;
@@ -58,13 +58,20 @@ __device__ __forceinline__ bool find_slot(const Pool &pool, int64_t slot, int he
   return true;
 }
 
-// d / s correctly rounded, given r = 1 / s rounded: two corrections by the exact
-// remainder (Markstein's theorem, for an s whose significand is not all
-// ones and results away from underflow).
+// d / s correctly rounded, given r = 1 / s to about an ulp, for an s of at most
+// 11 significant bits and results away from underflow: d * r is off by less
+// than two ulp, and adding the exact remainder times r rounds a number that is
+// off by 2^-22 ulp, while d / s is no nearer than 2^-12 ulp to a rounding boundary
+// (it is a multiple of 2^-k / s, and no boundary: that has 25 significant bits).
 __device__ __forceinline__ float quotient(float d, float s, float r) {
-  float q = d * r;
-  q = fmaf(fmaf(-q, s, d), r, q);
+  const float q = d * r;
   return fmaf(fmaf(-q, s, d), r, q);
+}
+// 1 / s to about an ulp (one Newton step), s normal.
+__device__ __forceinline__ float reciprocal(float s) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fmaf(fmaf(-s, r, 1.f), r, r);
 }
 
 // Codes of the lane's eight dims (u, 16 bits each), nibble i = dim i, and the
@@ -98,7 +105,7 @@ __device__ __forceinline__ uint32_t quantise(const uint4 &u, uint32_t &pair) {
   float n[8];
   if (normal && s2 >= 0x1p-100f) {
     // rint((x - lo) / s), at most 15: the scale is off by 2^-8 of itself at most
-    const float r = __frcp_rn(s2);
+    const float r = reciprocal(s2);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       n[i] = (quotient(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2, r) + kMagic) - kMagic;
@@ -116,7 +123,7 @@ __device__ __forceinline__ uint32_t quantise(const uint4 &u, uint32_t &pair) {
 // kD dims, groups of kG.  Grid: token strides x kv heads; a segment takes every
 // gridDim.x-th block's token and loads the next one's rows ahead.
 template <typename T, int kD, int kG>
-__global__ void __launch_bounds__(kThreadsPerBlock)
+__global__ void __launch_bounds__(kThreadsPerBlock, kBlocksPerSm)
     append_kernel(RowsIn in, const int64_t *__restrict__ slots, int64_t n, Pool pool) {
   constexpr int kSeg = kD / 8, kGroups = kD / kG, kLanes = kG / 8, kTok = kThreadsPerBlock / kSeg;
   const int head = blockIdx.y, j = threadIdx.x % kSeg, r = j % 8, seg = threadIdx.x / kSeg;
@@ -196,7 +203,7 @@ __device__ __forceinline__ uint4 expand(uint32_t word, uint32_t pair) {
 }
 
 template <typename T, int kD, int kG>
-__global__ void __launch_bounds__(kThreadsPerBlock)
+__global__ void __launch_bounds__(kThreadsPerBlock, kBlocksPerSm)
     read_kernel(Pool pool, const int64_t *__restrict__ slots, int64_t n, RowsOut out) {
   constexpr int kSeg = kD / 8, kGroups = kD / kG, kLanes = kG / 8, kTok = kThreadsPerBlock / kSeg;
   const int head = blockIdx.y, j = threadIdx.x % kSeg, r = j % 8, seg = threadIdx.x / kSeg;
@@ -321,12 +328,12 @@ int validate_rows(const fa_kv4_cache *c, const void *k, int64_t k_st, int64_t k_
   const int64_t per_block = kThreadsPerBlock / (c->head_size / 8);
   if (n > 0x7fffffffLL * per_block || c->num_kv_heads > 65535)
     return record_error(FA_ERR_INVALID_ARGUMENT, "kv4: too many rows or kv heads");
-  // at most eight blocks per SM (all resident): the rest of the tokens in strides
+  // as many blocks as are resident at once: the rest of the tokens in strides
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
-  const int64_t most = (8 * sms + c->num_kv_heads - 1) / c->num_kv_heads;
+  const int64_t most = (kBlocksPerSm * sms + c->num_kv_heads - 1) / c->num_kv_heads;
   const int64_t want = (n + per_block - 1) / per_block;
   *grid = dim3(static_cast<unsigned>(want < most ? want : most),
                static_cast<unsigned>(c->num_kv_heads));
