@@ -81,17 +81,18 @@ struct Plan {
   static constexpr int kHeads = 8 * kNT;
   static constexpr int kORow = kD + 4;  // f32 row pitch of the merge buffer (bank spread)
   static constexpr int kMergeBytes = kWarps * kHeads * kORow * 4;
+  static_assert(kMergeBytes <= 48 * 1024, "merge buffer");
 };
-// Shared memory holds the schedule's scan (batch + 1 int64), then the merge
-// buffer: sequences a call can take.
-constexpr int kMaxBatch = 6000;
-// Tiles a warp asks L2 to fetch ahead of the one it loads: 16 warps x 6 x 2304
+// Tiles a warp asks L2 to fetch ahead of the one it loads: 16 warps x 3 x 2304
 // bytes in flight cover the latency of HBM (44 KB per SM) several times over.
-constexpr int kAhead = 6;
+constexpr int kAhead = 3;
 
+// Units [a0, a1) of the CTA; the first belongs to entry `entry` of sequence b
+// (kv heads x head tiles), whose own first unit is x.  CTA p of `parts` starts
+// at unit p * chunk + min(p, extra).
 struct Share {
-  long long a0, a1, x_lo, total;
-  int e_lo, e_hi, parts;
+  long long a0, a1, x, chunk;
+  int b, entry, parts, extra;
 };
 
 struct Control {
@@ -107,15 +108,27 @@ __device__ __forceinline__ int seq_len_of(const Params &p, int b) {
 }
 __device__ __forceinline__ int blocks_of(int len) { return (len + kBlockTokens - 1) / kBlockTokens; }
 
-// The CTA's share of the work: entry costs 1 + blocks, in entry order, cut in
-// `parts` equal runs (the unit before an entry's blocks stands for its
-// per-piece overhead).  scan: batch + 1 int64 of shared memory.
-__device__ __noinline__ void compute_share(const Params &p, long long *scan, Control *ctl) {
+// Cost of an entry in units of one block: the blocks, and the start and end of
+// a piece (table, first tiles, Q, the warps' merge: about 3 us, three blocks).
+constexpr int kPieceCost = 3;
+
+// a / b where the quotient or both numbers are small; the 64-bit division is
+// an order of magnitude slower.
+__device__ __forceinline__ long long divide(long long a, int b) {
+  return a < (1ll << 31) ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
+}
+
+// The CTA's share of the work: the entries' costs in entry order, cut into
+// `parts` runs that differ by at most one unit.  A thread adds up its run of
+// sequences; the one that holds unit a0 finds the entry.
+__device__ __forceinline__ void compute_share(const Params &p, Control *ctl) {
   const int B = p.batch, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per_seq = p.hkv * p.head_tiles;
   const int per = (B + kThreads - 1) / kThreads;
   const int b0 = min(B, tid * per), b1 = min(B, b0 + per);
   long long local = 0;
-  for (int b = b0; b < b1; ++b) local += 1 + blocks_of(seq_len_of(p, b));
+  for (int b = b0; b < b1; ++b) local += kPieceCost + blocks_of(seq_len_of(p, b));
+  local *= per_seq;
   long long incl = local;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -124,46 +137,42 @@ __device__ __noinline__ void compute_share(const Params &p, long long *scan, Con
   }
   if (lane == 31) ctl->warp_sum[warp] = incl;
   __syncthreads();
-  long long run = incl - local;
-  for (int w = 0; w < warp; ++w) run += ctl->warp_sum[w];
-  for (int b = b0; b < b1; ++b) {
-    scan[b] = run;
-    run += 1 + blocks_of(seq_len_of(p, b));
+  long long total = 0, run = incl - local;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) run += ctl->warp_sum[w];
+    total += ctl->warp_sum[w];
   }
-  if (b1 == B && b0 < b1) scan[B] = run;
-  __syncthreads();
-  if (tid == 0) {
-    Share sh;
-    const long long per_seq = static_cast<long long>(p.hkv) * p.head_tiles;
-    sh.total = per_seq * scan[B];
-    sh.parts = static_cast<int>(min(static_cast<long long>(gridDim.x), sh.total));
-    sh.e_lo = 0;
-    sh.e_hi = -1;
-    sh.x_lo = sh.a0 = sh.a1 = 0;
-    if (static_cast<int>(blockIdx.x) < sh.parts) {
-      sh.a0 = blockIdx.x * sh.total / sh.parts;
-      sh.a1 = (blockIdx.x + 1) * sh.total / sh.parts;
-      auto locate = [&](long long u, int &e, long long &x) {
-        int lo = 0, hi = B - 1;  // last sequence with per_seq * scan[b] <= u
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (per_seq * scan[mid] <= u) lo = mid; else hi = mid - 1;
-        }
-        const long long c = scan[lo + 1] - scan[lo];
-        const long long in = u - per_seq * scan[lo];  // 32-bit division where it fits
-        const long long h = in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(c)
-                                             : in / c;
-        e = static_cast<int>(lo * per_seq + h);
-        x = per_seq * scan[lo] + h * c;
-      };
-      long long x_hi;
-      locate(sh.a0, sh.e_lo, sh.x_lo);
-      locate(sh.a1 - 1, sh.e_hi, x_hi);
+  const int parts = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  const int self = static_cast<int>(blockIdx.x);
+  const long long chunk = divide(total, parts);
+  const int extra = static_cast<int>(total - chunk * parts);
+  const long long a0 = self * chunk + min(self, extra);
+  if (self >= parts) {
+    if (tid == 0) ctl->share = Share{0, 0, 0, 1, 0, 0, parts, 0};
+  } else if (a0 >= run && a0 < run + local) {
+    int b = b0;
+    long long cost = 0;
+    for (;; ++b) {  // ends: a0 lies in this thread's sequences
+      cost = kPieceCost + blocks_of(seq_len_of(p, b));
+      if (a0 < run + cost * per_seq) break;
+      run += cost * per_seq;
     }
-    ctl->share = sh;
+    const int entry = static_cast<int>(divide(a0 - run, static_cast<int>(cost)));
+    ctl->share = Share{a0, a0 + chunk + (self < extra ? 1 : 0), run + entry * cost, chunk,
+                       b, entry, parts, extra};
   }
   __syncthreads();
 }
+
+// A run of one entry's 64-token blocks.
+struct Piece {
+  int b, entry;    // entry of the sequence: kv head * head tiles + head tile
+  int len, j0, nb; // tokens; first block; blocks of the entry
+  int blocks;      // of the piece
+  int n;           // this warp's 16-token tiles
+  long long x;     // first unit of the entry
+};
 
 // Operand pair k (0..3) of w: nibble k of both 16-bit halves as f16 numbers c *
 // 2^-24 (k even) or 16 c * 2^-24 (k odd); w8 = w >> 8.
@@ -235,89 +244,115 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  compute_share(p, reinterpret_cast<long long *>(smem), &ctl);
+  compute_share(p, &ctl);
   const Share &sh = ctl.share;
   float *obuf = reinterpret_cast<float *>(smem);
 
-  long long x = sh.x_lo;
-  for (int e = sh.e_lo; e <= sh.e_hi; ++e) {
-    // ------------------------------------------------------------ the piece
-    const int per_seq = p.hkv * p.head_tiles;
-    const int b = e / per_seq, kvh = (e % per_seq) / p.head_tiles, ht = e % p.head_tiles;
-    const int len = seq_len_of(p, b), nb = blocks_of(len);
-    const long long j0l = min(max(sh.a0 - x - 1, 0ll), static_cast<long long>(nb));
-    const long long j1l = min(max(sh.a1 - x - 1, 0ll), static_cast<long long>(nb));
-    const long long x_e = x;
-    x += 1 + nb;
-    if (nb > 0 ? j1l <= j0l : x_e < sh.a0) continue;  // the entry's unit alone: no piece here
-    const int j0 = static_cast<int>(j0l), j1 = static_cast<int>(j1l);
-    const int self = static_cast<int>(blockIdx.x);
-    const bool final_out = j1 - j0 == nb;
-    if (j0 == 0 && threadIdx.x == 0) {
-      int last = self;  // CTA with the entry's last block
-      if (!final_out)
-        last = static_cast<int>(min(static_cast<long long>(sh.parts - 1),
-                                    ((x_e + nb + 1) * sh.parts + sh.total - 1) / sh.total - 1));
-      p.merge[e] = make_int4(final_out ? -1 : sh.parts + self, self + 1, last - self, 0);
-    }
-    const int slot = j0 == 0 ? sh.parts + self : self;
-    const int h0 = ht * kHeads;                      // first head inside the group
-    const int heads = min(kHeads, p.group - h0);
-    // this warp's tiles: block j holds its tile j * 4 + warp
-    const int tiles_end = (len + kTileTokens - 1) / kTileTokens;
-    int n = j1 - j0;
-    while (n > 0 && (j0 + n - 1) * kWarps + warp >= tiles_end) --n;
-
-    // every 32 tiles lane i looks up the pool tile of the warp's i-th next one
-    // (-1: past the end, or a block outside the pool), one batch ahead
-    const int tiles_per_page = p.pool.tiles_per_block;
-    auto look_up = [&](int i0) {
-      const int mine = (j0 + i0 + lane) * kWarps + warp;
-      if (mine >= tiles_end || i0 + lane >= n) return -1;
-      const int pg = mine / tiles_per_page;
-      const int page = __ldg(p.block_table + b * p.bt_stride + pg);
-      if (page < 0 || page >= p.num_blocks) return -1;
-      return (page * p.hkv + kvh) * tiles_per_page + (mine - pg * tiles_per_page);
-    };
-    int tiles_a = look_up(0), tiles_b = n > 32 ? look_up(32) : -1;  // tiles base .. + 31, + 32 .. + 63
-    auto tile_at = [&](int i) {  // i: relative to the current batch of 32, 0 .. 63
-      return __shfl_sync(0xffffffffu, i < 32 ? tiles_a : tiles_b, i & 31);
-    };
-    auto prefetch = [&](int at) {
-      if (at >= 0 && lane == 0)
-        bulk_prefetch_l2(p.pool.data + static_cast<int64_t>(at) * kTileB, kTileB);
-    };
-    constexpr int kLaneWords = kW < 4 ? kW : 4;
-    constexpr int kRowBytes = 16 * kLaneWords;
-    const int key_off = r * kRowBytes + q * 4 * kLaneWords;  // row r + 8: + 8 * kRowBytes
-    uint32_t ka[kW] = {}, kb[kW] = {}, sca[2 * kGroups] = {}, scb[2 * kGroups] = {}, vw[4 * kU] = {};
-    auto load_keys = [&](const uint8_t *tile) {
-#pragma unroll
-      for (int pl = 0; pl < kW / kLaneWords; ++pl) {
-        const uint8_t *plane = tile + pl * (kTileTokens * kRowBytes) + key_off;
-        load_words<kLaneWords>(plane, ka + pl * kLaneWords);
-        load_words<kLaneWords>(plane + 8 * kRowBytes, kb + pl * kLaneWords);
+  const int self = static_cast<int>(blockIdx.x), per_seq = p.hkv * p.head_tiles;
+  // the next piece of the share, from the entry at unit x on
+  int b = sh.b, entry = sh.entry, len = sh.a0 < sh.a1 ? seq_len_of(p, b) : 0;
+  long long x = sh.x;
+  auto next_piece = [&](Piece &pc) -> bool {
+    while (x < sh.a1) {
+      const int nb = blocks_of(len);
+      // block j of the entry is unit x + kPieceCost + j
+      const long long from = sh.a0 - x - kPieceCost, to = sh.a1 - x - kPieceCost;
+      pc.j0 = static_cast<int>(min(max(from, 0ll), static_cast<long long>(nb)));
+      pc.blocks = static_cast<int>(min(max(to, 0ll), static_cast<long long>(nb))) - pc.j0;
+      pc.b = b;
+      pc.entry = entry;
+      pc.len = len;
+      pc.nb = nb;
+      pc.x = x;
+      // an empty entry goes to the CTA that holds its first unit
+      const bool mine = nb > 0 ? pc.blocks > 0 : x >= sh.a0;
+      x += kPieceCost + nb;
+      if (++entry == per_seq) {
+        entry = 0;
+        if (++b < p.batch) len = seq_len_of(p, b);
       }
-    };
-    auto load_scales = [&](const uint8_t *tile) {  // all pairs of tokens r, r + 8
-      load_words<2 * kGroups>(tile + 2 * code_bytes(kD) + r * 8 * kGroups, sca);
-      load_words<2 * kGroups>(tile + 2 * code_bytes(kD) + (r + 8) * 8 * kGroups, scb);
-    };
-    auto load_values = [&](const uint8_t *tile) {  // [token pair][u][half]
+      if (mine) {
+        // block j holds this warp's tile j * 4 + warp
+        const int tiles = (pc.len + kTileTokens - 1) / kTileTokens;
+        pc.n = min(pc.blocks, max((tiles - warp + kWarps - 1) / kWarps - pc.j0, 0));
+        return true;
+      }
+    }
+    return false;
+  };
+
+  constexpr int kLaneWords = kW < 4 ? kW : 4;
+  constexpr int kRowBytes = 16 * kLaneWords;
+  const int key_off = r * kRowBytes + q * 4 * kLaneWords;  // row r + 8: + 8 * kRowBytes
+  const int tiles_per_page = p.pool.tiles_per_block;
+  uint32_t ka[kW] = {}, kb[kW] = {}, sca[2 * kGroups] = {}, scb[2 * kGroups] = {}, vw[4 * kU] = {};
+  auto load_keys = [&](const uint8_t *tile) {
 #pragma unroll
-      for (int pl = 0; pl < kU; ++pl)
-        load_words<4>(tile + code_bytes(kD) + pl * 512 + lane * 16, vw + 4 * pl);
-    };
-    int at = tile_at(0);
+    for (int pl = 0; pl < kW / kLaneWords; ++pl) {
+      const uint8_t *plane = tile + pl * (kTileTokens * kRowBytes) + key_off;
+      load_words<kLaneWords>(plane, ka + pl * kLaneWords);
+      load_words<kLaneWords>(plane + 8 * kRowBytes, kb + pl * kLaneWords);
+    }
+  };
+  auto load_scales = [&](const uint8_t *tile) {  // all pairs of tokens r, r + 8
+    load_words<2 * kGroups>(tile + 2 * code_bytes(kD) + r * 8 * kGroups, sca);
+    load_words<2 * kGroups>(tile + 2 * code_bytes(kD) + (r + 8) * 8 * kGroups, scb);
+  };
+  auto load_values = [&](const uint8_t *tile) {  // [token pair][u][half]
+#pragma unroll
+    for (int pl = 0; pl < kU; ++pl)
+      load_words<4>(tile + code_bytes(kD) + pl * 512 + lane * 16, vw + 4 * pl);
+  };
+  // every 32 tiles lane i looks up the pool tile of the warp's i-th next one
+  // (-1: past the end, or a block outside the pool), one batch ahead
+  auto look_up = [&](const Piece &pc, int i0) {
+    const int mine = (pc.j0 + i0 + lane) * kWarps + warp;
+    if (i0 + lane >= pc.n) return -1;
+    const int pg = mine / tiles_per_page;
+    const int page = __ldg(p.block_table + pc.b * p.bt_stride + pg);
+    if (page < 0 || page >= p.num_blocks) return -1;
+    return (page * p.hkv + pc.entry / p.head_tiles) * tiles_per_page + (mine - pg * tiles_per_page);
+  };
+  int tiles_a = -1, tiles_b = -1;  // tiles base .. + 31, + 32 .. + 63 of the piece
+  auto tile_at = [&](int i) {      // i: relative to base, 0 .. 63
+    return __shfl_sync(0xffffffffu, i < 32 ? tiles_a : tiles_b, i & 31);
+  };
+  auto tile_ptr = [&](int at) { return p.pool.data + static_cast<int64_t>(at) * kTileB; };
+  auto prefetch = [&](int at) {
+    if (at >= 0 && lane == 0) bulk_prefetch_l2(tile_ptr(at), kTileB);
+  };
+  // a piece's loads: Q rows, block table, its first tile into registers, the
+  // next ones into L2.  Issued before the previous piece is merged.
+  uint4 qraw[kNT][kW];
+  int at = -1;
+  auto begin = [&](const Piece &pc) {
+    const int h0 = pc.entry % p.head_tiles * kHeads;  // first head inside the group
+    const int heads = min(kHeads, p.group - h0);
+    const T *rows = static_cast<const T *>(p.q) + pc.b * p.q_sb +
+                    static_cast<int64_t>(pc.entry / p.head_tiles * p.group + h0) * p.q_sh;
+#pragma unroll
+    for (int t = 0; t < kNT; ++t)
+#pragma unroll
+      for (int i = 0; i < kW; ++i)
+        qraw[t][i] = t * 8 + r < heads
+                         ? __ldg(reinterpret_cast<const uint4 *>(rows + (t * 8 + r) * p.q_sh) + 4 * i + q)
+                         : make_uint4(0u, 0u, 0u, 0u);
+    tiles_a = look_up(pc, 0);
+    tiles_b = pc.n > 32 ? look_up(pc, 32) : -1;
+    at = tile_at(0);
     if (at >= 0) {
-      const uint8_t *tile = p.pool.data + static_cast<int64_t>(at) * kTileB;
-      load_keys(tile);
-      load_scales(tile);
-      load_values(tile);
+      load_keys(tile_ptr(at));
+      load_scales(tile_ptr(at));
+      load_values(tile_ptr(at));
     }
 #pragma unroll 1
-    for (int i = 1; i < kAhead; ++i) prefetch(tile_at(i));
+    for (int i = 1; i < min(kAhead, pc.n); ++i) prefetch(tile_at(i));
+  };
 
+  Piece pc;
+  bool have = next_piece(pc);
+  if (have) begin(pc);
+  while (have) {
     // Q as the B operand, times a power of two that brings the row's largest
     // magnitude to [2^13, 2^14): pair k of word i holds dims 32 i + 8 q + {k,
     // k + 4} of head r of each 8-head tile, over 16 for odd k
@@ -326,16 +361,10 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     float unit[kNT][2];         // log2 score per unit of the products' sum, ditto
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
-      const bool live = t * 8 + r < heads;
-      const uint4 *src = reinterpret_cast<const uint4 *>(
-          static_cast<const T *>(p.q) + b * p.q_sb +
-          static_cast<int64_t>(kvh * p.group + h0 + (live ? t * 8 + r : 0)) * p.q_sh);
-      uint4 v[kW];
       float mag = 0.f;
 #pragma unroll
       for (int i = 0; i < kW; ++i) {
-        v[i] = live ? __ldg(src + 4 * i + q) : make_uint4(0u, 0u, 0u, 0u);
-        const T *el = reinterpret_cast<const T *>(&v[i]);
+        const T *el = reinterpret_cast<const T *>(&qraw[t][i]);
 #pragma unroll
         for (int d = 0; d < 8; ++d) mag = fmaxf(mag, fabsf(Elem<T>::to_f(el[d])));
       }
@@ -348,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
       for (int g = 0; g < kGroups; ++g) sum[g] = 0.f;
 #pragma unroll
       for (int i = 0; i < kW; ++i) {
-        const T *el = reinterpret_cast<const T *>(&v[i]);
+        const T *el = reinterpret_cast<const T *>(&qraw[t][i]);
         float x[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -397,16 +426,16 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
     // the warp's next tile, as soon as its products are issued.
     int base = 0;  // of tiles_a
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const int left = at >= 0 ? len - ((j0 + i) * kWarps + warp) * kTileTokens : 0;
+    for (int i = 0; i < pc.n; ++i) {
+      const int left = at >= 0 ? pc.len - ((pc.j0 + i) * kWarps + warp) * kTileTokens : 0;
       if (i - base == 32) {
         base += 32;
         tiles_a = tiles_b;
-        tiles_b = base + 32 < n ? look_up(base + 32) : -1;
+        tiles_b = base + 32 < pc.n ? look_up(pc, base + 32) : -1;
       }
       at = tile_at(i + 1 - base);
       prefetch(tile_at(i + kAhead - base));
-      const uint8_t *next = p.pool.data + static_cast<int64_t>(at) * kTileB;
+      const uint8_t *next = tile_ptr(at);
       // ------------------------------------------------------------ scores
       float s[kNT][4];
 #pragma unroll
@@ -558,8 +587,23 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
       if (at >= 0) load_values(next);
     }
 
+    const Piece done = pc;
+
     // ------------------------------------------------ the warps' states meet
-    __syncthreads();  // the previous piece's merge (or the scan) is done with
+    const bool final_out = done.blocks == done.nb;
+    const int h0 = done.entry % p.head_tiles * kHeads, kvh = done.entry / p.head_tiles;
+    const int heads = min(kHeads, p.group - h0);
+    const int slot = done.j0 == 0 ? sh.parts + self : self;
+    if (done.j0 == 0 && threadIdx.x == 0) {
+      int last = self;  // CTA with the entry's last block
+      if (!final_out) {
+        const long long u = done.x + kPieceCost + done.nb - 1, big = sh.extra * (sh.chunk + 1);
+        last = static_cast<int>(u < big ? u / (sh.chunk + 1) : sh.extra + (u - big) / sh.chunk);
+      }
+      p.merge[static_cast<int64_t>(done.b) * per_seq + done.entry] =
+          make_int4(final_out ? -1 : sh.parts + self, self + 1, last - self, 0);
+    }
+    __syncthreads();  // the previous piece's merge is done with the buffer
 #pragma unroll
     for (int t = 0; t < kNT; ++t)
 #pragma unroll
@@ -617,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
           acc.w = fmaf(v.w, k, acc.w);
         }
         if (final_out)
-          store4<T>(static_cast<T *>(p.o) + b * p.o_sb + h * p.o_sh + d, acc);
+          store4<T>(static_cast<T *>(p.o) + done.b * p.o_sb + h * p.o_sh + d, acc);
         else
           store4<float>(p.part_o + (static_cast<int64_t>(slot) * kHeads + hh) * kD + d, acc);
       }
@@ -625,9 +669,11 @@ __global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
         if (!final_out)
           p.part_lse[static_cast<int64_t>(slot) * kHeads + hh] = lse;
         else if (p.lse)
-          p.lse[static_cast<int64_t>(b) * p.hq + h] = lse;
+          p.lse[static_cast<int64_t>(done.b) * p.hq + h] = lse;
       }
     }
+    have = next_piece(pc);
+    if (have) begin(pc);
   }
 }
 
@@ -682,13 +728,10 @@ int launch_t(const Params &p, int sms, cudaStream_t stream, int *grid_out, bool 
   constexpr int per_sm = kD * kNT <= 128 ? 4 : 2;
   *grid_out = sms * per_sm;
   if (query) return FA_OK;
-  if (p.batch > kMaxBatch)
-    return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: at most 6000 sequences per call");
-  const int scan = (p.batch + 1) * 8;  // at most 48 KB: no opt-in needed
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(*grid_out);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = scan > PL::kMergeBytes ? scan : PL::kMergeBytes;
+  cfg.dynamicSmemBytes = PL::kMergeBytes;  // below 48 KB: no opt-in needed
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
