@@ -83,6 +83,12 @@ struct Plan {
   static constexpr int kMergeBytes = kWarps * kHeads * kORow * 4;
   static_assert(kMergeBytes <= 48 * 1024, "merge buffer");
 };
+// CTAs per SM: as many as the registers hold without spills in the loop (64
+// short chats, head size 64, two head tiles: 34.6 us with four, 32.9 with three;
+// 8 long contexts, head size 128, one head tile: 88 us with four, 98 with three).
+__host__ __device__ constexpr int blocks_per_sm(int d, int nt) {
+  return nt == 1 && d <= 128 ? 4 : (d == 64 ? 3 : 2);
+}
 // Tiles a warp asks L2 to fetch ahead of the one it loads: 16 warps x 3 x 2304
 // bytes in flight cover the latency of HBM (44 KB per SM) several times over.
 constexpr int kAhead = 3;
@@ -230,7 +236,7 @@ __device__ __forceinline__ void pair_of(uint32_t w, float &lo, float &scale) {
 }
 
 template <typename T, int kD, int kGroups, int kNT>
-__global__ void __launch_bounds__(kThreads, kD * kNT <= 128 ? 4 : 2)
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
     kv4_decode_kernel(const __grid_constant__ Params p) {
   using PL = Plan<kD, kGroups, kNT>;
   constexpr int kG = kD / kGroups;
@@ -725,8 +731,7 @@ template <typename T, int kD, int kGroups, int kNT>
 int launch_t(const Params &p, int sms, cudaStream_t stream, int *grid_out, bool query) {
   using PL = Plan<kD, kGroups, kNT>;
   auto kern = kv4_decode_kernel<T, kD, kGroups, kNT>;
-  constexpr int per_sm = kD * kNT <= 128 ? 4 : 2;
-  *grid_out = sms * per_sm;
+  *grid_out = sms * blocks_per_sm(kD, kNT);
   if (query) return FA_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(*grid_out);
