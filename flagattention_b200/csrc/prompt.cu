@@ -261,8 +261,9 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
     }
     // Value rows past the sequence's end belong to the next sequence and may
     // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them
-    // (both Q tiles do, before their own products; either may come first).
-    if (quad == 0 && half == 0 && it.lk < (j + 1) * kTile) {
+    // (both Q tiles do, before their own products; either may come first), an
+    // eighth of the rows each warp.
+    if (it.lk < (j + 1) * kTile) {
       const uint32_t v_tile = tiles + (j - it.j0);
       const int st = v_tile % PL::kVStages;
       warp_wait(smem_u32(&bars->v_full[st]), (v_tile / PL::kVStages) & 1u, abort_flag, p.status,
@@ -270,7 +271,7 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
       const uint32_t tile = smem_u32(smem + PL::kOffV) + st * PL::kVBytes;
       const int r0 = it.lk - j * kTile;
       const int units = (kTile - r0) * 8;  // 16-byte units of a chunk's rows
-      for (int u = lane; u < units * PL::kVChunks; u += 32)
+      for (int u = (warp & 7) * 32 + lane; u < units * PL::kVChunks; u += 256)
         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
                          tile + (u / units) * PL::kChunkBytes + r0 * 128 + (u % units) * 16),
                      "r"(0u)
@@ -419,16 +420,15 @@ __device__ __forceinline__ int cancelled_block(uint32_t response) {
 struct Finder {
   const Params &p;
   const int lane, span;
-  int lq = 0, lk = 0, pairs = 0;  // of the lane's sequence
+  int q0 = 0, k0 = 0, lq = 0, lk = 0, pairs = 0;  // of the lane's sequence
   int c = -1;                     // key tiles of the current items
   int base = 0, first = 0;        // items before them / before sequence `first`
 
   __device__ __forceinline__ Finder(const Params &p_, int lane_) : p(p_), lane(lane_), span(2 * p_.tq) {
     if (p.batch > 32) return;
     if (lane < p.batch) {
-      int s;
-      seq_range(p.cu_q, lane, p.total_q, s, lq);
-      seq_range(p.cu_k, lane, p.total_k, s, lk);
+      seq_range(p.cu_q, lane, p.total_q, q0, lq);
+      seq_range(p.cu_k, lane, p.total_k, k0, lk);
       pairs = (lq + span - 1) / span;
     }
     restart();
@@ -456,7 +456,7 @@ struct Finder {
     }
     return v;
   }
-  __device__ __forceinline__ bool by_cost(int x, int &b, int &pair) {
+  __device__ __forceinline__ bool by_cost(int x, Work &w, int &pair) {
     if (x < base) restart();
     for (; c >= 0; --c) {
       const int more = at_least(c + 1), mine = (pairs > 0 ? at_least(c) : 0) - (pairs > 0 ? more : 0);
@@ -464,15 +464,18 @@ struct Finder {
       const int all = __shfl_sync(0xffffffffu, incl, 31);
       if (x < base + all) {
         const int at = __ffs(__ballot_sync(0xffffffffu, x < base + incl)) - 1;
-        b = at;
         pair = __shfl_sync(0xffffffffu, pairs - more - 1 + (incl - mine), at) - (x - base);
+        w.q0 = __shfl_sync(0xffffffffu, q0, at);
+        w.lq = __shfl_sync(0xffffffffu, lq, at);
+        w.k0 = __shfl_sync(0xffffffffu, k0, at);
+        w.lk = __shfl_sync(0xffffffffu, lk, at);
         return true;
       }
       base += all;
     }
     return false;  // the bound of the items is not tight
   }
-  __device__ __forceinline__ bool in_order(int x, int &b, int &pair) {
+  __device__ __forceinline__ bool in_order(int x, Work &w, int &pair) {
     if (x < base) base = first = 0;
     for (; first < p.batch; first += 32) {
       int s, n = 0;
@@ -481,16 +484,17 @@ struct Finder {
       const int all = __shfl_sync(0xffffffffu, incl, 31);
       if (x < base + all) {
         const int at = __ffs(__ballot_sync(0xffffffffu, x < base + incl)) - 1;
-        b = first + at;
         pair = base + __shfl_sync(0xffffffffu, incl, at) - 1 - x;
+        seq_range(p.cu_q, first + at, p.total_q, w.q0, w.lq);
+        seq_range(p.cu_k, first + at, p.total_k, w.k0, w.lk);
         return true;
       }
       base += all;
     }
     return false;
   }
-  __device__ __forceinline__ bool find(int x, int &b, int &pair) {
-    return p.batch <= 32 ? by_cost(x, b, pair) : in_order(x, b, pair);
+  __device__ __forceinline__ bool find(int x, Work &w, int &pair) {
+    return p.batch <= 32 ? by_cost(x, w, pair) : in_order(x, w, pair);
   }
 };
 
@@ -507,13 +511,11 @@ __device__ __forceinline__ void scheduler_role(const Params &p, Bars *bars, int 
     const int sec = idx / per_section, in = idx - sec * per_section;
     const int width = min(p.section, p.hkv - sec * p.section);
     const int x = in / (width * p.splits), rest = in - x * width * p.splits;
-    int b, pair;
-    if (finder.find(x, b, pair)) {
-      Work w;
+    Work w;
+    int pair;
+    if (finder.find(x, w, pair)) {
       w.kvh = sec * p.section + rest % width;
       w.split = rest / width;
-      seq_range(p.cu_q, b, p.total_q, w.q0, w.lq);
-      seq_range(p.cu_k, b, p.total_k, w.k0, w.lk);
       w.i0 = pair * 2 * p.tq;
       int n[2];
 #pragma unroll
@@ -525,8 +527,12 @@ __device__ __forceinline__ void scheduler_role(const Params &p, Bars *bars, int 
         n[t] = keys > 0 ? (keys + kTile - 1) / kTile : 0;
       }
       const int n_max = max(n[0], n[1]);
-      w.j0 = static_cast<int>(static_cast<int64_t>(w.split) * n_max / p.splits);
-      w.j1 = static_cast<int>(static_cast<int64_t>(w.split + 1) * n_max / p.splits);
+      w.j0 = 0;
+      w.j1 = n_max;
+      if (p.splits > 1) {  // at most 32 splits of 2^24 tiles
+        w.j0 = w.split * n_max / p.splits;
+        w.j1 = (w.split + 1) * n_max / p.splits;
+      }
       w.end[0] = min(w.j1, n[0]);
       w.end[1] = min(w.j1, n[1]);
       const uint32_t slot = count & 1u;
@@ -591,6 +597,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
 
+  // the scheduler's first reads, on their way while the CTA sets up
+  if (warp == kSchedulerWarp && lane < min(p.batch, 32)) {
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.cu_q + lane));
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.cu_k + lane));
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&bars->k_full[i]), 1);
