@@ -185,14 +185,6 @@ struct Piece {
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int k) {
   return (k < 2 ? w : w8) & ((k & 1) ? 0x00f000f0u : 0x000f000fu);
 }
-// The values' operands: byte k / 2 of both halves whole, c + 16 c' times 2^-24
-// (k even), or its upper code alone, 16 c' * 2^-24 (k odd).  The sums for the
-// lower code are their difference, taken once per piece: one instruction per
-// operand.  (The keys cannot: their two codes meet different query numbers.)
-__device__ __forceinline__ uint32_t code_bytes16(uint32_t w, int k) {
-  const uint32_t both = k < 2 ? w & 0x00ff00ffu : __byte_perm(w, 0u, 0x4341);
-  return (k & 1) ? (k < 2 ? w : both) & 0x00f000f0u : both;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -253,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
   compute_share(p, &ctl);
   const Share &sh = ctl.share;
   float *obuf = reinterpret_cast<float *>(smem);
+  float *kept = obuf + warp * kHeads * PL::kORow + lane;  // value sums of earlier tiles
 
   const int self = static_cast<int>(blockIdx.x), per_seq = p.hkv * p.head_tiles;
   // the next piece of the share, from the entry at unit x on
@@ -435,6 +428,21 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
     for (int i = 0; i < pc.n; ++i) {
       const int left = at >= 0 ? pc.len - ((pc.j0 + i) * kWarps + warp) * kTileTokens : 0;
       if (i - base == 32) {
+        // The tensor cores cut off what an f32 sum has no room for, and the
+        // codes' sums only grow (no sign): after 64 tiles they move to this
+        // warp's part of the buffer, where they are added with rounding.
+        if (base & 32) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int i2 = 0; i2 < kD / 16; ++i2)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float &sum = kept[((t * (kD / 16) + i2) * 4 + c) * 32];
+                sum = base >= 64 ? sum + o[t][i2][c] : o[t][i2][c];
+                o[t][i2][c] = 0.f;
+              }
+        }
         base += 32;
         tiles_a = tiles_b;
         tiles_b = base + 32 < pc.n ? look_up(pc, base + 32) : -1;
@@ -540,6 +548,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
             for (int i2 = 0; i2 < kD / 16; ++i2) {
               o[t][i2][h] *= alpha * shrink;
               o[t][i2][h + 2] *= alpha * shrink;
+              if (base >= 64) {
+                kept[((t * (kD / 16) + i2) * 4 + h) * 32] *= alpha * shrink;
+                kept[((t * (kD / 16) + i2) * 4 + h + 2) * 32] *= alpha * shrink;
+              }
             }
           }
       }
@@ -577,11 +589,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
       for (int u = 0; u < kU; ++u) {
         const uint32_t w0 = vw[2 * u], w1 = vw[2 * u + 1], w2 = vw[2 * kU + 2 * u],
                        w3 = vw[2 * kU + 2 * u + 1];
+        const uint32_t s0 = w0 >> 8, s1 = w1 >> 8, s2 = w2 >> 8, s3 = w3 >> 8;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int g = (64 * u + 32 * (k >> 1)) / kG;
-          const uint32_t a0 = code_bytes16(w0, k), a1 = code_bytes16(w1, k),
-                         a2 = code_bytes16(w2, k), a3 = code_bytes16(w3, k);
+          const uint32_t a0 = code_pair(w0, s0, k), a1 = code_pair(w1, s1, k),
+                         a2 = code_pair(w2, s2, k), a3 = code_pair(w3, s3, k);
 #pragma unroll
           for (int t = 0; t < kNT; ++t) {
             mma16816(o[t][4 * u + k], a0, a1, a2, a3, pf[t][g][0], pf[t][g][1]);
@@ -593,6 +606,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
       if (at >= 0) load_values(next);
     }
 
+    if (base >= 64) {  // sums were moved
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int i2 = 0; i2 < kD / 16; ++i2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[t][i2][c] += kept[((t * (kD / 16) + i2) * 4 + c) * 32];
+      __syncwarp();  // the rows of the merge go over them
+    }
     const Piece done = pc;
 
     // ------------------------------------------------ the warps' states meet
@@ -609,7 +631,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
       p.merge[static_cast<int64_t>(done.b) * per_seq + done.entry] =
           make_int4(final_out ? -1 : sh.parts + self, self + 1, last - self, 0);
     }
-    __syncthreads();  // the previous piece's merge is done with the buffer
 #pragma unroll
     for (int t = 0; t < kNT; ++t)
 #pragma unroll
@@ -631,12 +652,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
 #pragma unroll
           for (int pp = 0; pp < 2; ++pp) {
             const float ex = extra[t][(64 * u + 32 * pp) / kG][h];
-            const float unit_o = 0x1p24f / vnorm, odd = 0x1p20f / vnorm;
+            const float even = 0x1p24f / vnorm, odd = 0x1p20f / vnorm;
             const float *oa = o[t][4 * u + 2 * pp], *ob = o[t][4 * u + 2 * pp + 1];
             // codes 2 pp and 2 pp + 1 of rows m < 8, then of rows m >= 8
             *reinterpret_cast<float4 *>(row + 64 * u + 32 * pp + 4 * r) =
-                make_float4(fmaf(oa[h] - ob[h], unit_o, ex), fmaf(ob[h], odd, ex),
-                            fmaf(oa[h + 2] - ob[h + 2], unit_o, ex), fmaf(ob[h + 2], odd, ex));
+                make_float4(fmaf(oa[h], even, ex), fmaf(ob[h], odd, ex), fmaf(oa[h + 2], even, ex),
+                            fmaf(ob[h + 2], odd, ex));
           }
       }
     __syncthreads();
@@ -678,6 +699,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
           p.lse[static_cast<int64_t>(done.b) * p.hq + h] = lse;
       }
     }
+    __syncthreads();  // the buffer is free for the next piece's sums
     have = next_piece(pc);
     if (have) begin(pc);
   }

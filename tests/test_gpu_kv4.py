@@ -4,10 +4,10 @@ Quantisation is defined in f32 with IEEE division, so append + read is compared
 for equality with the same formula in torch.  The attention's bound is derived:
 with p the softmax weights, c / lo / s the codes, minima and scales, u the unit
 roundoff of the output type (2^-8 bf16, 2^-11 f16):
-  * p * s is rounded to bf16 before the value product (f16 caches: to two bf16
-    parts, 2^-16): u_p * sum p s c, u_p = 2^-8 or 2^-16;
+  * p * s is rounded to f16 before the value product (f16 caches: to two f16
+    parts, at least 2^-16): u_p * sum p s c, u_p = 2^-11 or 2^-16;
   * the output is rounded: u |o|;
-  * f32 accumulation of codes with their offset 16: 2^-20 sum p (|lo| + 47 s);
+  * f32 accumulation: 2^-20 sum p (|lo| + 47 s);
   * scores are off by at most e = 2^-21 (3 S + 2), S = scale * sum_d |q_d| (47 s
     + |lo|): a weight by 2 e.
 """
@@ -22,7 +22,7 @@ from flagattention_b200._torch import read_status
 pytestmark = pytest.mark.gpu
 
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
-UP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16}
+UP = {torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -16}
 SHAPES = [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32), (256, 128), (256, 64)]
 
 
@@ -207,6 +207,34 @@ def test_decode_pages(block):
                                   [1 + (i * 53) % 300 for i in range(400)]])
 def test_decode_long_split_and_many(lens):
     check(*build(lens, 8, 2, 64, 32, 16, torch.bfloat16, seed=4))
+
+
+@pytest.mark.parametrize("d, group", [(128, 64), (64, 32), (256, 128)])
+@pytest.mark.parametrize("dtype, bound", [(torch.bfloat16, 3e-3), (torch.float16, 1e-3)])
+def test_decode_long_context_keeps_its_accuracy(d, group, dtype, bound):
+    """Over many tokens the output is the small difference of large sums (codes
+    and minima are not centred): 2-norm against 64 bits, one sequence spread over
+    the GPU and a batch of which every CTA holds whole ones (one sequence's sums
+    run over hundreds of tiles in one warp).  Expected: the output's
+    rounding (at most 2^-8 or 2^-11, 2^-8 / sqrt(3) = 2.3e-3 or 2.8e-4 over the
+    mantissas), P' rounded to 16 bits (independent: 2^-11 / sqrt(3) * rms(s c) /
+    rms(v) = 7e-4, or nothing), and f32 sums of n / 64 products per warp, each off
+    by 2^-24 of a sum about 2 / rms(o) = 60 times the output: below 5e-4.  Sums that a
+    warp lets grow further have to be split."""
+    cache, table, q, data, lens = build([40000], 8, 1, d, group, 64, dtype, seed=12)
+    k, v = (_exact(x[:, 0], group) for x in data[0])
+    p = torch.softmax(q[0].double() @ k.T * d ** -0.5, -1)
+    want = p @ v
+    for batch in (1, 1500):                               # the same pages for all
+        out = fa.paged_attention_int4(q.expand(batch, -1, -1), cache, lens.expand(batch),
+                                      table.expand(batch, -1))
+        for b in {0, batch // 2, batch - 1}:
+            assert (out[b].double() - want).norm() / want.norm() <= bound
+
+
+def _exact(x, group):
+    c, lo, s = (t.double() for t in quantise(x, group))
+    return (lo[..., None] + c * s[..., None]).flatten(-2)
 
 
 def test_decode_sharp_scores():
