@@ -71,6 +71,36 @@ def test_append_then_read_is_exact(d, group, heads, block, n, dtype):
         assert not got.any()
 
 
+@pytest.mark.parametrize("d, group", SHAPES)
+def test_tile_layout(d, group):
+    """The bytes of a tile are where csrc/kv4.cuh says: key words, value units,
+    (lo, scale) pairs."""
+    cache = fa.Int4KVCache(1, 1, 16, d, group_size=group)
+    k, v = rows(16, 1, d, torch.bfloat16, 3)
+    fa.append_kv_int4(k, v, cache, torch.arange(16, device="cuda"))
+    tile = cache.data[0, 0, 0].cpu().numpy()
+    (ck, lk, sk), (cv, lv, sv) = ([t[:, 0].cpu() for t in quantise(x, group)] for x in (k, v))
+    ck, cv = (c.flatten(-2).numpy().astype(np.uint8) for c in (ck, cv))
+    want = np.zeros_like(tile)
+    plane, half_bytes = min(d, 128), 8 * d
+    for t in range(16):
+        for dim in range(0, d, 2):                        # two codes a byte
+            j = dim // 8                                   # key word: dims 8 j .. 8 j + 7
+            pl, jj = j // (plane // 8), j % (plane // 8)
+            at = pl * 8 * plane + t * (plane // 2) + ((jj % 4) * (plane // 32) + jj // 4) * 4
+            want[at + dim % 8 // 2] = ck[t, dim] | ck[t, dim + 1] << 4
+            # value dim 64 u + 32 p + 4 r + 2 half + (n & 1), n = 2 p + (n & 1)
+            u, p, r, half = dim // 64, dim // 32 % 2, dim % 32 // 4, dim % 4 // 2
+            idx = ((t // 8) * (d // 64) + u) * 2 + half
+            at = idx // 4 * 512 + (r * 4 + t % 8 // 2) * 16 + idx % 4 * 4 + t % 2 * 2
+            want[half_bytes + at + p] = cv[t, dim] | cv[t, dim + 1] << 4
+        pairs = torch.stack([torch.cat([lk[t], lv[t]]), torch.cat([sk[t], sv[t]])], -1)
+        n = pairs.numel() * 2
+        want[2 * half_bytes + t * n:2 * half_bytes + (t + 1) * n] = \
+            pairs.to(torch.bfloat16).view(torch.uint8).numpy().ravel()
+    assert np.array_equal(tile, want)
+
+
 def test_skipped_slots_overwrites_and_strides():
     cache = fa.Int4KVCache(4, 2, 32, 128)
     qkv = torch.randn(50, 8, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
