@@ -14,7 +14,8 @@ import math
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import raw_stream, require_cuda
+from flagattention_b200._torch import (empty, launch_lock, raw_stream, require_cuda,
+                                       stream_workspace)
 
 
 class Int4KVCache:
@@ -128,11 +129,11 @@ def read_kv_int4(cache, slot_mapping):
     a slot outside the pool."""
     slot_mapping = _check_slots(slot_mapping, cache)
     n, heads, d = slot_mapping.shape[0], cache.num_kv_heads, cache.head_size
-    k = slot_mapping.new_empty((n, heads, d), dtype=cache.dtype)
-    v = torch.empty_like(k)
+    dev = slot_mapping.get_device()
+    k, v = empty((n, heads, d), cache.dtype, dev), empty((n, heads, d), cache.dtype, dev)
     st = _lib.lib().fa_kv4_read(ctypes.byref(cache.struct()), k.data_ptr(), heads * d, d,
                                 v.data_ptr(), heads * d, d, slot_mapping.data_ptr(), n,
-                                raw_stream(slot_mapping.get_device()))
+                                raw_stream(dev))
     if st:
         _lib.check(st, "fa_kv4_read")
     return k, v
@@ -152,7 +153,8 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
         require_cuda(query, context_lens, block_tables)
     if query.dim() != 3 or query.shape[2] != cache.head_size:
         raise _lib.InvalidArgument("query must be [num_seqs, num_q_heads, head_size of the cache]")
-    if query.dtype != cache.dtype:
+    c_dtype = cache.dtype
+    if query.dtype != c_dtype:
         raise _lib.InvalidArgument(f"the query must be in the cache's dtype ({cache.dtype})")
     num_seqs, hq, d = query.shape
     if hq == 0 or hq % cache.num_kv_heads != 0:
@@ -170,20 +172,22 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
     if block_tables.stride(1) != 1:
         block_tables = block_tables.contiguous()
     c = cache.struct()
-    out = query.new_empty((num_seqs, hq, d))
-    lse = query.new_empty((num_seqs, hq), dtype=torch.float32) if return_lse else None
+    out = empty((num_seqs, hq, d), c_dtype, dev)
+    lse = empty((num_seqs, hq), torch.float32, dev) if return_lse else None
     po, pl, mg = _workspace_bytes(dev, num_seqs, hq, c.num_kv_heads, d, c.group_size, c.dtype)
-    ws = query.new_empty((po + pl + mg,), dtype=torch.uint8)
-    base = ws.data_ptr()
+    stream = raw_stream(dev)
     q_b, q_h, _ = query.stride()
-    # field order of fa_kv4_attention_args
-    a = _lib.Kv4AttentionArgs(query.data_ptr(), q_b, q_h, c, block_tables.data_ptr(),
-                              block_tables.stride(0), block_tables.shape[1],
-                              context_lens.data_ptr(), num_seqs, hq,
-                              1.0 / math.sqrt(d) if attn_scale is None else attn_scale,
-                              out.data_ptr(), hq * d, d, lse.data_ptr() if return_lse else None,
-                              base, base + po, base + po + pl)
-    st = _lib.lib().fa_kv4_attention(ctypes.byref(a), raw_stream(dev))
+    with launch_lock:
+        ws, base = stream_workspace(po + pl + mg, dev, stream)
+        # field order of fa_kv4_attention_args
+        a = _lib.Kv4AttentionArgs(query.data_ptr(), q_b, q_h, c, block_tables.data_ptr(),
+                                  block_tables.stride(0), block_tables.shape[1],
+                                  context_lens.data_ptr(), num_seqs, hq,
+                                  1.0 / math.sqrt(d) if attn_scale is None else attn_scale,
+                                  out.data_ptr(), hq * d, d,
+                                  lse.data_ptr() if return_lse else None,
+                                  base, base + po, base + po + pl)
+        st = _lib.lib().fa_kv4_attention(ctypes.byref(a), stream)
     if st:
         _lib.check(st, "fa_kv4_attention")
     return (out, lse) if return_lse else out

@@ -16,16 +16,21 @@ import math
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import dtype_code, raw_stream, require_cuda, status_ptr
+from flagattention_b200._torch import (dtype_code, empty, launch_lock, raw_stream,
+                                       require_cuda, status_ptr, stream_workspace)
 
 
-def _rows16(x):
-    """x, or a contiguous copy where the kernel cannot address its rows
-    (inner stride, broadcast dims, 16-byte alignment)."""
+def _rows(x):
+    """(x, address, token stride, head stride): x, or a contiguous copy where the
+    kernel cannot address its rows (inner stride, broadcast dims, 16-byte
+    alignment)."""
     t, h, d = x.stride()
-    if d == 1 and t and h and not (t | h | (x.data_ptr() >> 1)) & 7:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    p = x.data_ptr()
+    if d != 1 or not t or not h or (t | h | (p >> 1)) & 7:
+        x = x.clone(memory_format=torch.contiguous_format)
+        t, h, _ = x.stride()
+        p = x.data_ptr()
+    return x, p, t, h
 
 
 @functools.lru_cache(maxsize=4096)
@@ -80,22 +85,23 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
     code = dtype_code(q)
     batch = cu_seqlens_q.shape[0] - 1
     causal = 1 if causal else 0
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    (q, q_p, q_t, q_h), (k, k_p, k_t, k_h), (v, v_p, v_t, v_h) = _rows(q), _rows(k), _rows(v)
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
-    out = q.new_empty((total_q, hq, d_v))
-    lse = q.new_empty((hq, total_q), dtype=torch.float32) if return_lse else None
+    out = empty((total_q, hq, d_v), dtype, dev)
+    lse = empty((hq, total_q), torch.float32, dev) if return_lse else None
     size = _workspace_bytes(dev, batch, total_q, total_k, hq, hk, d_v, causal) \
         if hq // hk <= 128 and 0 < d_v <= 128 else 0
-    ws = q.new_empty((size,), dtype=torch.uint8) if size else None
-    (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _) = q.stride(), k.stride(), v.stride()
-    # field order of fa_prompt_args
-    a = _lib.PromptArgs(q.data_ptr(), q_t, q_h, k.data_ptr(), k_t, k_h, v.data_ptr(), v_t, v_h,
-                        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-                        batch, total_q, total_k, hq, hk, d, d_v, causal, code,
-                        1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
-                        out.data_ptr(), hq * d_v, d_v, lse.data_ptr() if return_lse else None,
-                        ws.data_ptr() if size else None, status_ptr(dev))
-    st = _lib.lib().fa_prompt_attention(ctypes.byref(a), raw_stream(dev))
+    stream = raw_stream(dev)
+    with launch_lock:
+        ws, base = stream_workspace(size, dev, stream) if size else (None, None)
+        # field order of fa_prompt_args
+        a = _lib.PromptArgs(q_p, q_t, q_h, k_p, k_t, k_h, v_p, v_t, v_h,
+                            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+                            batch, total_q, total_k, hq, hk, d, d_v, causal, code,
+                            1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
+                            out.data_ptr(), hq * d_v, d_v, lse.data_ptr() if return_lse else None,
+                            base, status_ptr(dev))
+        st = _lib.lib().fa_prompt_attention(ctypes.byref(a), stream)
     if st:
         _lib.check(st, "fa_prompt_attention")
     return (out, lse) if return_lse else out
