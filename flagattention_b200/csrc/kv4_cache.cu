@@ -16,6 +16,13 @@
 // integer pipes half of that, so per-element work is kept small: minima and
 // maxima two at a time in T, divisions as products with the group's
 // reciprocal corrected to the exact quotient, codes moved by multiply-adds.
+// A thread takes every grid-th token and loads the next ones' rows while it
+// works on one; four blocks of 256 threads per SM.
+//
+// Measured: 16383 tokens of 8 kv heads of 128, groups of 64, bf16, written and
+// read back: 53 us for 172 MB (3.2 TB/s; schedulers issue in 80% / 70% of the
+// cycles of the write / the read: the instruction count binds).  64
+// tokens: 4.6 us for both launches.
 #include "kv4.cuh"
 #include "flagattn_b200.h"
 

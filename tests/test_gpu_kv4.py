@@ -299,6 +299,21 @@ def test_decode_nan_stays_and_does_not_spread():
     assert out[0, 2:].isfinite().all() and out[1].isfinite().all() and lse[1].isfinite().all()
 
 
+@pytest.mark.parametrize("lens", [[9000], [2500] * 12])    # wide and narrow merges
+def test_decode_nan_stays_when_entries_are_split(lens):
+    cache, table, q, data, n = build(lens, 16, 2, 128, 64, 16, torch.bfloat16, seed=17)
+    k = data[0][0].clone()
+    k[20, 0, 3] = float("nan")                                       # in one piece of kv head 0
+    fa.append_kv_int4(k[20:21], data[0][1][20:21], cache,
+                      (table[0, 1].long() * 16 + 4).reshape(1))
+    q[0, 9] = float("nan")                                           # in every piece of its row
+    out, lse = fa.paged_attention_int4(q, cache, n, table, return_lse=True)
+    bad = torch.zeros(len(lens), 16, dtype=torch.bool, device="cuda")
+    bad[0, :8] = bad[0, 9] = True
+    assert torch.equal(out.isnan().all(-1), bad) and torch.equal(out.isnan().any(-1), bad)
+    assert torch.equal(lse.isnan(), bad) and lse[~bad].isfinite().all()
+
+
 def test_decode_table_entries_outside_the_pool_and_short_tables():
     cache, table, q, data, lens = build([100, 64, 40], 4, 2, 64, 32, 16, torch.bfloat16, seed=8)
     live = [torch.ones(n, dtype=torch.bool, device="cuda") for n in (100, 64, 40)]

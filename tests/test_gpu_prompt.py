@@ -149,6 +149,21 @@ def test_neighbours_do_not_leak(value):
     check(q, k, v, lens, lens, causal=True, skip=(1,))
 
 
+def test_nan_stays_when_keys_are_split():
+    """Few queries over many keys: a NaN in one range of the keys, and one in a
+    query, which meets it in every range."""
+    n, m = 100, 9000
+    q, k, v = tensors([n], [m], 16, 2, 128, 128, torch.bfloat16, seed=14)
+    k[5000, 0] = float("nan")
+    q[7, 9] = float("nan")
+    cu = lambda x: torch.tensor([0, x], dtype=torch.int32, device="cuda")  # noqa: E731
+    out, lse = fa.prompt_attention(q, k, v, cu(n), cu(m), return_lse=True)
+    bad = torch.zeros(n, 16, dtype=torch.bool, device="cuda")
+    bad[:, :8] = bad[7, 9] = True
+    assert torch.equal(out.isnan().all(-1), bad) and torch.equal(out.isnan().any(-1), bad)
+    assert torch.equal(lse.isnan(), bad.T) and lse.T[~bad].isfinite().all()
+
+
 def test_values_of_the_lowest_type_value():
     lens = [100, 260]
     q, k, v = tensors(lens, lens, 4, 2, 64, 64, torch.bfloat16, seed=5)
