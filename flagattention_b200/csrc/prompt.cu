@@ -74,7 +74,7 @@ struct Plan {
   static constexpr int kKStages = kDqk == 192 ? 2 : (kDqk == 128 ? 3 : 4);
   static constexpr int kVStages = kDqk == 192 ? 1 : (kDqk == 128 ? 2 : 4);
   static constexpr int kOffX = 1024;
-  static constexpr int kOffQ = 3072;
+  static constexpr int kOffQ = kOffX + 2048;  // past the exchange block
   static constexpr int kOffK = kOffQ + 2 * kQBytes;
   static constexpr int kOffV = kOffK + kKStages * kKBytes;
   static constexpr int kSmemUsed = kOffV + kVStages * kVBytes;

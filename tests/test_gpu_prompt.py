@@ -184,6 +184,18 @@ def test_views_of_a_fused_projection():
     check(t, t, t, lens, lens)                        # heads outside tokens
 
 
+def test_views_past_32_bit_offsets():
+    """Rows 2^20 elements apart: the last ones lie past 2^31 elements."""
+    n = 2100
+    g = torch.Generator(device="cuda").manual_seed(15)
+    base = torch.empty(n, 1 << 20, dtype=torch.bfloat16, device="cuda")
+    base[:, :1536] = torch.randn(n, 1536, generator=g, device="cuda").to(torch.bfloat16)
+    base[:, 1536:1664] = float("nan")
+    q, k, v = base[:, :1024].view(n, 8, 128), base[:, 1024:1280].view(n, 2, 128), \
+        base[:, 1280:1536].view(n, 2, 128)
+    check(q, k, v, [2000, 100], [2000, 100])
+
+
 def test_many_sequences_and_long_ones():
     lens = [1 + (i * 37) % 90 for i in range(700)]
     check(*tensors(lens, lens, 4, 1, 64, 64, torch.bfloat16, seed=7), lens, lens)
