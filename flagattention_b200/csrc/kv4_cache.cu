@@ -15,7 +15,7 @@
 // the schedulers have about 200 instructions per 16 elements of a lane, the
 // integer pipes half of that, so per-element work is kept small: minima and
 // maxima two at a time in T, divisions as products with the group's
-// reciprocal corrected to the exact quotient, codes moved by multiply-adds.
+// reciprocal corrected to the exact quotient, codes summed up as integers.
 // A thread takes every grid-th token and loads the next ones' rows while it
 // works on one; four blocks of 256 threads per SM.
 //
@@ -109,22 +109,26 @@ __device__ __forceinline__ uint32_t quantise(const uint4 &u, uint32_t &pair) {
   pair = *reinterpret_cast<const uint32_t *>(both);
   if (!finite || s2 == 0.f) return 0u;
   const T *e = reinterpret_cast<const T *>(&u);
-  float n[8];
+  // codes as integers in the mantissa of kMagic
+  constexpr uint32_t kMagicBits = 0x4b400000u;
+  uint32_t n[8];
   if (normal && s2 >= 0x1p-100f) {
     // rint((x - lo) / s), at most 15: the scale is off by 2^-8 of itself at most
     const float r = reciprocal(s2);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      n[i] = (quotient(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2, r) + kMagic) - kMagic;
+      n[i] = __float_as_uint(quotient(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2, r) + kMagic);
   } else {  // a subnormal scale may be off by half: the quotient may pass 15
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      n[i] = rintf(fminf(__fdiv_rn(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2), 15.f));
+      n[i] = __float_as_uint(
+          fminf(__fdiv_rn(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2), 15.f) + kMagic);
   }
-  // four codes to a 16-bit number in f32, exactly
-  const float a = fmaf(fmaf(fmaf(n[3], 16.f, n[2]), 16.f, n[1]), 16.f, n[0]);
-  const float b = fmaf(fmaf(fmaf(n[7], 16.f, n[6]), 16.f, n[5]), 16.f, n[4]);
-  return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
+  // sum of 16^i (kMagicBits + code) modulo 2^32, less what kMagicBits gives
+  uint32_t word = n[7];
+#pragma unroll
+  for (int i = 6; i >= 0; --i) word = word * 16u + n[i];
+  return word - kMagicBits * 0x11111111u;
 }
 
 // kD dims, groups of kG.  Grid: token strides x kv heads; a segment takes every
@@ -180,33 +184,46 @@ __global__ void __launch_bounds__(kThreadsPerBlock, kBlocksPerSm)
   }
 }
 
-// Eight values lo + scale * code in T.
+template <typename T>
+__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
+// Eight values lo + scale * code, rounded once to T: two at a time in T, whose
+// fused multiply-add takes exact operands.  A code is one AND-OR into the
+// mantissa of a power of two (128 in bf16, 1024 in f16), which is then taken off.
 template <typename T>
 __device__ __forceinline__ uint4 expand(uint32_t word, uint32_t pair) {
-  const T *e = reinterpret_cast<const T *>(&pair);
-  const float lo = Elem<T>::to_f(e[0]), s = Elem<T>::to_f(e[1]);
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr uint32_t kPower = kHalf ? 0x64006400u : 0x43004300u, kMinusPower = kPower | 0x80008000u;
+  const uint32_t lo = __byte_perm(pair, 0u, 0x1010), s = __byte_perm(pair, 0u, 0x3232);
+  uint32_t x[4];  // dims i and i + 4
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = fma2<T>(add2<T>(((word >> (4 * i)) & 0x000f000fu) | kPower, kMinusPower), s, lo);
   // lo + 15 * scale may pass the type's largest number by the scale's rounding
-  const float top = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
-  const bool over = fmaf(15.f, s, lo) > top;
-  // nibbles 0 to 4 are masked in place: 16^i c in the mantissa under the
-  // exponent of 2^23, with 16^i taken off the scale (exact); 5 to 7 after a shift
-  float si[5] = {s};
+  const T *e = reinterpret_cast<const T *>(&pair);
+  constexpr float top = kHalf ? 65504.f : 3.38953139e38f;
+  if (fmaf(15.f, Elem<T>::to_f(e[1]), Elem<T>::to_f(e[0])) > top) {
 #pragma unroll
-  for (int i = 1; i < 5; ++i) si[i] = si[i - 1] * 0.0625f;
-  const uint32_t upper = word >> 20;
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int k = i < 5 ? i : i - 5;
-    const float c = __uint_as_float(((i < 5 ? word : upper) & (15u << (4 * k))) | 0x4b000000u) - 8388608.f;
-    x[i] = fmaf(c, si[k], lo);
+    for (int i = 0; i < 4; ++i) x[i] = min2_nan<T>(x[i], kHalf ? 0x7bff7bffu : 0x7f7f7f7fu);
   }
-  if (over) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] > top ? top : x[i];
-  }
-  return make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]),
-                    Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
+  return make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
+                    __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
 }
 
 template <typename T, int kD, int kG>
