@@ -216,12 +216,8 @@ __device__ __forceinline__ uint4 expand(uint32_t word, uint32_t pair) {
   for (int i = 0; i < 4; ++i)
     x[i] = fma2<T>(add2<T>(((word >> (4 * i)) & 0x000f000fu) | kPower, kMinusPower), s, lo);
   // lo + 15 * scale may pass the type's largest number by the scale's rounding
-  const T *e = reinterpret_cast<const T *>(&pair);
-  constexpr float top = kHalf ? 65504.f : 3.38953139e38f;
-  if (fmaf(15.f, Elem<T>::to_f(e[1]), Elem<T>::to_f(e[0])) > top) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = min2_nan<T>(x[i], kHalf ? 0x7bff7bffu : 0x7f7f7f7fu);
-  }
+  for (int i = 0; i < 4; ++i) x[i] = min2_nan<T>(x[i], kHalf ? 0x7bff7bffu : 0x7f7f7f7fu);
   return make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
                     __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
 }
