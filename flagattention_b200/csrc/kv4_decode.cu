@@ -716,43 +716,41 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
 }
 
 // Merge of split entries: entry e = (sequence, kv head, run of head tiles),
-// partials f32 [slot][rows][kD].  Narrow: one warp per row.  Wide: the four
-// warps of a block take every fourth partial of one row, for entries cut
-// into many pieces.
-template <typename T, bool kWide>
-__global__ void __launch_bounds__(128)
+// partials f32 [slot][rows][kD], o = sum_s exp(lse_s - lse) o_s.  What it costs is
+// round trips to L2, so a warp loads eight partials of a row before it uses the
+// first.  Narrow: one warp per row.  Wide, for entries cut into many pieces
+// (one context of 8000 tokens: 74): eight warps per row take every eighth
+// partial, and meet in shared memory.
+template <typename T, int kD, bool kWide>
+__global__ void __launch_bounds__(kWide ? 256 : 128)
     kv4_combine_kernel(const float *__restrict__ part_o, const float *__restrict__ part_lse,
                        const int4 *__restrict__ merge, int rows, int group, int head_tiles,
-                       int hkv, int hq, int d, T *__restrict__ out, int64_t o_sb, int64_t o_sh,
+                       int hkv, int hq, T *__restrict__ out, int64_t o_sb, int64_t o_sh,
                        float *__restrict__ lse) {
-  __shared__ MergeState states[kWide ? 4 : 1][32];
+  constexpr int kVec = kD > 128 ? 2 : 1, kAtOnce = 8, kRowWarps = kWide ? 8 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = kWide ? rows : rows / 4;  // blocks of an entry
-  const int e = blockIdx.x / per;
+  const int e = blockIdx.x / per, w = kWide ? warp : 0;
   const int row = kWide ? blockIdx.x % per : (blockIdx.x % per) * 4 + warp;
   const int ht = e % head_tiles, kvh = (e / head_tiles) % hkv, b = e / (head_tiles * hkv);
   const int in_group = ht * rows + row;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 mg = merge[e];
   if (mg.x < 0 || in_group >= group) return;  // of all threads when wide
-  const int64_t os = static_cast<int64_t>(rows) * d, off = static_cast<int64_t>(row) * d;
-  MergeState st;
-  st.init();
-  if (!kWide || warp == 0)
-    fold_parts<false, 1>(st, part_o, part_lse, mg.x, 0, 1, 1, os, rows, off, row, d, lane);
-  fold_parts<false, 2>(st, part_o, part_lse, mg.y, kWide ? warp : 0, kWide ? 4 : 1, mg.z, os, rows,
-                       off, row, d, lane);
+  RowSum<kVec> st;
+  st.template fold<kAtOnce>(part_o, part_lse, w, kRowWarps, 1 + mg.z, kD, lane, [&](int s) {
+    return static_cast<int64_t>(s == 0 ? mg.x : mg.y + s - 1) * rows + row;
+  });
   if constexpr (kWide) {
+    __shared__ RowSum<kVec> states[kRowWarps][32];
     states[warp][lane] = st;
     __syncthreads();
     if (warp != 0) return;
-#pragma unroll
-    for (int w = 1; w < 4; ++w) fold_state(st, states[w][lane]);
+    st.join(&states[0][lane], 32, kRowWarps);
   }
   const int h = kvh * group + in_group;
-  const float l = finish_row<T>(st, d, out + b * o_sb + h * o_sh, lane);
-  // a piece of infinite lse (NaN) left a NaN in the sums, and so in the row
-  if (lse && lane == 0) lse[static_cast<int64_t>(b) * hq + h] = st.z == st.z ? l : NAN;
+  const float l = st.finish(out + b * o_sb + h * o_sh, kD, lane);
+  if (lse && lane == 0) lse[static_cast<int64_t>(b) * hq + h] = l;
 }
 
 // Run of query heads one entry serves, as 8-head tiles: two where a group has
@@ -778,19 +776,21 @@ int launch_t(const Params &p, int sms, cudaStream_t stream, int *grid_out, bool 
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
-  // about grid / entries pieces per entry
+  // about grid / entries pieces per entry; from 16 on the wide merge (8000 tokens
+  // a context, 8 kv heads: 4 contexts 24.5 us wide, 26.6 narrow; 8 contexts 34.8 / 32.7)
   const int64_t entries = static_cast<int64_t>(p.batch) * p.hkv * p.head_tiles;
-  const bool wide = entries * 8 <= *grid_out;
+  const bool wide = entries * 16 <= *grid_out;
   const int64_t blocks = entries * (wide ? PL::kHeads : PL::kHeads / 4);
   if (blocks > INT32_MAX) return record_error(FA_ERR_UNSUPPORTED, "kv4 attention: too many rows");
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(wide ? 256 : 128);
   cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, wide ? kv4_combine_kernel<T, true> : kv4_combine_kernel<T, false>,
+  e = cudaLaunchKernelEx(&cfg,
+                         wide ? kv4_combine_kernel<T, kD, true> : kv4_combine_kernel<T, kD, false>,
                          static_cast<const float *>(p.part_o),
                          static_cast<const float *>(p.part_lse),
                          static_cast<const int4 *>(p.merge), PL::kHeads, p.group, p.head_tiles,
-                         p.hkv, p.hq, kD, static_cast<T *>(p.o), p.o_sb, p.o_sh, p.lse);
+                         p.hkv, p.hq, static_cast<T *>(p.o), p.o_sb, p.o_sh, p.lse);
   if (e != cudaSuccess) return record_error(FA_ERR_CUDA, cudaGetErrorString(e));
   return FA_OK;
 }

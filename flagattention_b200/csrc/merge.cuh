@@ -187,6 +187,86 @@ __device__ __forceinline__ void mla_row_state(MergeState &st, const TP *__restri
   }
 }
 
+// The same merge for rows of up to 128 * kVec f32 columns (lane l owns 4 l + 128
+// c .. + 3), many partials of which are loaded before the first is used: what it
+// costs is round trips to L2.  A partial of infinite lse stands for one that is
+// NaN, which a maximum would drop; it makes the row and its lse NaN.
+template <int kVec>
+struct RowSum {
+  float m = -INFINITY, z = 0.f;
+  float4 acc[kVec];
+  __device__ __forceinline__ RowSum() {
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  static __device__ __forceinline__ void add(float4 &a, float ka, const float4 &v, float kv) {
+    a.x = a.x * ka + v.x * kv;
+    a.y = a.y * ka + v.y * kv;
+    a.z = a.z * ka + v.z * kv;
+    a.w = a.w * ka + v.w * kv;
+  }
+  // partials first, first + step, ... below n; at(s): which row of part_o ([row][d]
+  // f32) and part_lse is partial s
+  template <int kAtOnce, typename At>
+  __device__ __forceinline__ void fold(const float *part_o, const float *part_lse, int first,
+                                       int step, int n, int d, int lane, At at) {
+    for (int s0 = first; s0 < n; s0 += step * kAtOnce) {
+      float ls[kAtOnce];
+      float4 v[kAtOnce][kVec];
+#pragma unroll
+      for (int g = 0; g < kAtOnce; ++g) {
+        const int s = s0 + g * step;
+        const int64_t i = at(s);
+        ls[g] = s < n ? __ldg(part_lse + i) : -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c)
+          v[g][c] = s < n && c * 128 + lane * 4 < d
+                        ? __ldg(reinterpret_cast<const float4 *>(part_o + i * d + c * 128) + lane)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float top = m;
+#pragma unroll
+      for (int g = 0; g < kAtOnce; ++g) top = fmaxf(top, ls[g]);
+      if (top == -INFINITY) continue;  // nothing but empty partials so far
+      const float keep = m == -INFINITY ? 0.f : __expf(m - top);
+      z *= keep;
+#pragma unroll
+      for (int g = 0; g < kAtOnce; ++g) {
+        const float k = ls[g] == -INFINITY ? 0.f : __expf(ls[g] - top);
+        z += k;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) add(acc[c], g == 0 ? keep : 1.f, v[g][c], k);
+      }
+      m = top;
+    }
+  }
+  // join with n - 1 further states, others[i * stride], i = 1 .. n - 1, of the row
+  __device__ __forceinline__ void join(const RowSum *others, int stride, int n) {
+    for (int i = 1; i < n; ++i) {
+      const RowSum &o = others[i * stride];
+      const float top = fmaxf(m, o.m);
+      if (top == -INFINITY) continue;
+      const float k = m == -INFINITY ? 0.f : __expf(m - top);
+      const float ko = o.m == -INFINITY ? 0.f : __expf(o.m - top);
+      z = z * k + o.z * ko;
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) add(acc[c], k, o.acc[c], ko);
+      m = top;
+    }
+  }
+  // writes the row (d columns) and returns its lse
+  template <typename T>
+  __device__ __forceinline__ float finish(T *out, int d, int lane) const {
+    const float inv = z > 0.f ? 1.f / z : 0.f;  // a NaN is in acc as well
+#pragma unroll
+    for (int c = 0; c < kVec; ++c)
+      if (c * 128 + lane * 4 < d)
+        store4<T>(out + c * 128 + lane * 4, make_float4(acc[c].x * inv, acc[c].y * inv,
+                                                        acc[c].z * inv, acc[c].w * inv));
+    return z > 0.f ? m + __logf(z) : (z == z ? -INFINITY : NAN);
+  }
+};
+
 // Normalised output row and merged LSE of a state whose partials had type TP
 // (which fixes the lane's columns, acc_col).
 template <typename T, typename TP = float>

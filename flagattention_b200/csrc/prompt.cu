@@ -911,14 +911,12 @@ __global__ void __launch_bounds__(128) prompt_merge_kernel(const __grid_constant
   const int head = static_cast<int>(row / p.total_q), tok = static_cast<int>(row % p.total_q);
   if (tok >= __ldg(p.cu_q + p.batch)) return;  // of no sequence: not written
   const int lane = threadIdx.x & 31;
-  MergeState st;
-  st.init();
-  fold_parts<false, 2>(st, p.part_o, p.part_lse, 0, 0, 1, p.splits, rows * p.d_v, rows, row * p.d_v,
-                       row, p.d_v, lane);
-  const float l = finish_row<T>(
-      st, p.d_v, static_cast<T *>(p.o) + static_cast<int64_t>(tok) * p.o_st + head * p.o_sh, lane);
-  // a part of infinite lse (NaN) left a NaN in the sums, and so in the row
-  if (p.lse && lane == 0) p.lse[row] = st.z == st.z ? l : NAN;
+  RowSum<1> st;
+  st.fold<4>(p.part_o, p.part_lse, 0, 1, p.splits, p.d_v, lane,
+             [&](int s) { return static_cast<int64_t>(s) * rows + row; });
+  const float l = st.finish(
+      static_cast<T *>(p.o) + static_cast<int64_t>(tok) * p.o_st + head * p.o_sh, p.d_v, lane);
+  if (p.lse && lane == 0) p.lse[row] = l;
 }
 
 template <typename T, int kDqk, int kDv>
