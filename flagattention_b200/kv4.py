@@ -18,6 +18,9 @@ from flagattention_b200._torch import (empty, launch_lock, raw_stream, require_c
                                        stream_workspace)
 
 
+_pack_attention, _attention_args = _lib.packer(_lib.Kv4AttentionArgs)
+
+
 class Int4KVCache:
     """Pool of num_blocks blocks of block_size tokens, num_kv_heads heads of
     head_size dims (64, 128 or 256), keys and values.
@@ -41,9 +44,9 @@ class Int4KVCache:
         if device.type != "cuda":
             raise _lib.InvalidArgument("flagattention_b200 operators take CUDA tensors only "
                                        "(there is no CPU path)")
-        code = _lib.FA_DTYPE_F16 if dtype == torch.float16 else _lib.FA_DTYPE_BF16
+        self.dtype_code = _lib.FA_DTYPE_F16 if dtype == torch.float16 else _lib.FA_DTYPE_BF16
         self._struct = _lib.Kv4Cache(None, self.num_blocks, self.num_kv_heads, self.block_size,
-                                     self.head_size, self.group_size, code)
+                                     self.head_size, self.group_size, self.dtype_code)
         size = ctypes.c_int64(0)
         _lib.check(_lib.lib().fa_kv4_cache_bytes(ctypes.byref(self._struct), ctypes.byref(size)),
                    "fa_kv4_cache_bytes")
@@ -56,6 +59,11 @@ class Int4KVCache:
     @property
     def device(self):
         return self.data.device
+
+    def fields(self):
+        """The values of the library's ``fa_kv4_cache``, in order."""
+        return (self.data.data_ptr(), self.num_blocks, self.num_kv_heads, self.block_size,
+                self.head_size, self.group_size, self.dtype_code)
 
     def struct(self):
         """The pool as the library's ``fa_kv4_cache``."""
@@ -149,8 +157,11 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
     also the log-sum-exp f32 [num_seqs, num_q_heads].  A sequence without
     cached tokens gets zeros and -inf.
     """
-    if not (query.is_cuda and context_lens.is_cuda and block_tables.is_cuda):
+    dev = query.get_device()
+    if dev < 0 or cache.data.get_device() != dev or context_lens.get_device() != dev or \
+            block_tables.get_device() != dev:
         require_cuda(query, context_lens, block_tables)
+        raise _lib.InvalidArgument("all tensors must be on the cache's device")
     if query.dim() != 3 or query.shape[2] != cache.head_size:
         raise _lib.InvalidArgument("query must be [num_seqs, num_q_heads, head_size of the cache]")
     c_dtype = cache.dtype
@@ -164,30 +175,24 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
     if context_lens.shape != (num_seqs,) or block_tables.dim() != 2 or \
             block_tables.shape[0] != num_seqs:
         raise _lib.InvalidArgument("context_lens [num_seqs] and block_tables [num_seqs, width]")
-    dev = query.get_device()
-    if cache.data.get_device() != dev or context_lens.get_device() != dev or \
-            block_tables.get_device() != dev:
-        raise _lib.InvalidArgument("all tensors must be on the cache's device")
     query, context_lens = _rows16(query), context_lens.contiguous()
     if block_tables.stride(1) != 1:
         block_tables = block_tables.contiguous()
-    c = cache.struct()
     out = empty((num_seqs, hq, d), c_dtype, dev)
     lse = empty((num_seqs, hq), torch.float32, dev) if return_lse else None
-    po, pl, mg = _workspace_bytes(dev, num_seqs, hq, c.num_kv_heads, d, c.group_size, c.dtype)
+    po, pl, mg = _workspace_bytes(dev, num_seqs, hq, cache.num_kv_heads, d, cache.group_size,
+                                  cache.dtype_code)
     stream = raw_stream(dev)
     q_b, q_h, _ = query.stride()
     with launch_lock:
         ws, base = stream_workspace(po + pl + mg, dev, stream)
         # field order of fa_kv4_attention_args
-        a = _lib.Kv4AttentionArgs(query.data_ptr(), q_b, q_h, c, block_tables.data_ptr(),
-                                  block_tables.stride(0), block_tables.shape[1],
-                                  context_lens.data_ptr(), num_seqs, hq,
-                                  1.0 / math.sqrt(d) if attn_scale is None else attn_scale,
-                                  out.data_ptr(), hq * d, d,
-                                  lse.data_ptr() if return_lse else None,
-                                  base, base + po, base + po + pl)
-        st = _lib.lib().fa_kv4_attention(ctypes.byref(a), stream)
+        _pack_attention(query.data_ptr(), q_b, q_h, *cache.fields(), block_tables.data_ptr(),
+                        block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
+                        num_seqs, hq, 1.0 / math.sqrt(d) if attn_scale is None else attn_scale,
+                        out.data_ptr(), hq * d, d, lse.data_ptr() if return_lse else 0,
+                        base, base + po, base + po + pl)
+        st = _lib.lib().fa_kv4_attention(_attention_args, stream)
     if st:
         _lib.check(st, "fa_kv4_attention")
     return (out, lse) if return_lse else out

@@ -20,6 +20,9 @@ from flagattention_b200._torch import (dtype_code, empty, launch_lock, raw_strea
                                        require_cuda, status_ptr, stream_workspace)
 
 
+_pack, _args = _lib.packer(_lib.PromptArgs)
+
+
 def _rows(x):
     """(x, address, token stride, head stride): x, or a contiguous copy where the
     kernel cannot address its rows (inner stride, broadcast dims, 16-byte
@@ -61,9 +64,11 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
     """
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
-    if not (q.is_cuda and k.is_cuda and v.is_cuda and cu_seqlens_q.is_cuda and
-            cu_seqlens_k.is_cuda):
+    dev = q.get_device()
+    if dev < 0 or k.get_device() != dev or v.get_device() != dev or \
+            cu_seqlens_q.get_device() != dev or cu_seqlens_k.get_device() != dev:
         require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
+        raise _lib.InvalidArgument("all tensors must be on one device")
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise _lib.InvalidArgument("q, k, v must be [tokens, heads, head size]")
     (total_q, hq, d), (total_k, hk, d_k), (total_v, hv, d_v) = q.shape, k.shape, v.shape
@@ -78,14 +83,14 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
             cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] < 1 or \
             cu_seqlens_k.shape != cu_seqlens_q.shape:
         raise _lib.InvalidArgument("cu_seqlens must be int32 [batch + 1]")
-    dev = q.get_device()
-    if k.get_device() != dev or v.get_device() != dev or cu_seqlens_q.get_device() != dev or \
-            cu_seqlens_k.get_device() != dev:
-        raise _lib.InvalidArgument("all tensors must be on one device")
     code = dtype_code(q)
     batch = cu_seqlens_q.shape[0] - 1
     causal = 1 if causal else 0
-    (q, q_p, q_t, q_h), (k, k_p, k_t, k_h), (v, v_p, v_t, v_h) = _rows(q), _rows(k), _rows(v)
+    (q_t, q_h, q_d), (k_t, k_h, k_d), (v_t, v_h, v_d) = q.stride(), k.stride(), v.stride()
+    q_p, k_p, v_p = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not (q_d == k_d == v_d == 1 and q_t and q_h and k_t and k_h and v_t and v_h) or \
+            (q_t | q_h | k_t | k_h | v_t | v_h | (q_p | k_p | v_p) >> 1) & 7:
+        (q, q_p, q_t, q_h), (k, k_p, k_t, k_h), (v, v_p, v_t, v_h) = _rows(q), _rows(k), _rows(v)
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     out = empty((total_q, hq, d_v), dtype, dev)
     lse = empty((hq, total_q), torch.float32, dev) if return_lse else None
@@ -93,15 +98,15 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
         if hq // hk <= 128 and 0 < d_v <= 128 else 0
     stream = raw_stream(dev)
     with launch_lock:
-        ws, base = stream_workspace(size, dev, stream) if size else (None, None)
+        ws, base = stream_workspace(size, dev, stream) if size else (None, 0)
         # field order of fa_prompt_args
-        a = _lib.PromptArgs(q_p, q_t, q_h, k_p, k_t, k_h, v_p, v_t, v_h,
-                            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-                            batch, total_q, total_k, hq, hk, d, d_v, causal, code,
-                            1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
-                            out.data_ptr(), hq * d_v, d_v, lse.data_ptr() if return_lse else None,
-                            base, status_ptr(dev))
-        st = _lib.lib().fa_prompt_attention(ctypes.byref(a), stream)
+        _pack(q_p, q_t, q_h, k_p, k_t, k_h, v_p, v_t, v_h,
+              cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+              batch, total_q, total_k, hq, hk, d, d_v, causal, code,
+              1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
+              out.data_ptr(), hq * d_v, d_v, lse.data_ptr() if return_lse else 0,
+              base, status_ptr(dev))
+        st = _lib.lib().fa_prompt_attention(_args, stream)
     if st:
         _lib.check(st, "fa_prompt_attention")
     return (out, lse) if return_lse else out
