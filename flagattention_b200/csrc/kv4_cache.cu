@@ -4,7 +4,8 @@
 // lo) / 15 rounded to the row's type (lo is an element of the row, so exact),
 // and codes c = rint((x - lo) / s) clamped to 0 .. 15 (0 where s is 0); it
 // stands for lo + s * c.  All arithmetic is f32 with IEEE division, so the
-// result does not depend on the launch.  A group that holds a NaN or an
+// result does not depend on the launch (reads: one fused
+// multiply-add in the row's type, rounded once).  A group that holds a NaN or an
 // infinity keeps lo = NaN and reads back as NaN: it is not lost silently.
 //
 // One segment of D / 8 lanes takes a token of one kv head, keys and values: a
@@ -13,16 +14,16 @@
 // 32-bit word of keys and two 16-bit units of values (kv4.cuh).  4 D bytes in,
 // D + 8 D / G out per token and head (the read in reverse).  At the HBM rate
 // the schedulers have about 200 instructions per 16 elements of a lane, the
-// integer pipes half of that, so per-element work is kept small: minima and
-// maxima two at a time in T, divisions as products with the group's
-// reciprocal corrected to the exact quotient, codes summed up as integers.
+// integer pipes half of that, so per-element work is kept small: minima,
+// maxima and expanded codes two at a time in T, divisions as products with the
+// group's reciprocal corrected to the exact quotient, codes summed up as integers.
 // A thread takes every grid-th token and loads the next ones' rows while it
 // works on one; four blocks of 256 threads per SM.
 //
 // Measured: 16383 tokens of 8 kv heads of 128, groups of 64, bf16, written and
-// read back: 53 us for 172 MB (3.2 TB/s; schedulers issue in 80% / 70% of the
-// cycles of the write / the read: the instruction count binds).  64
-// tokens: 4.6 us for both launches.
+// read back: 46-50 us for 172 MB (3.5 TB/s; schedulers issue in 75% / 60% of the
+// cycles of the write / the read, the integer pipe is 60% / 64% busy: the
+// instruction count binds).  64 tokens: 4.2 us for both launches.
 #include "kv4.cuh"
 #include "flagattn_b200.h"
 

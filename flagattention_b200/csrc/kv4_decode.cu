@@ -44,7 +44,8 @@
 // Measured at 64 query / 8 kv heads of 128, groups of 64, bf16: 8 contexts of
 // 20001 to 65536 tokens 89-92 us (390 MB read from HBM, 4.3 TB/s; schedulers
 // issue in 57% of the cycles, the integer pipe is 52% busy: the instruction count binds
-// before HBM does), 32 of 1000 to 4096 tokens 29.9 us, one of 700 tokens 9.3 us;
+// before HBM does), 32 of 1000 to 4096 tokens 29.9 us, one of 700 tokens 9.3 us (of
+// 8000: 18.3 with a cold L2);
 // 64 of 1 to 4001 tokens, 64 / 4 heads of 64, f16: 31.3 us.
 #include "kv4.cuh"
 #include "flagattn_b200.h"
