@@ -267,6 +267,12 @@ def _exact(x, group):
     return (lo[..., None] + c * s[..., None]).flatten(-2)
 
 
+@pytest.mark.parametrize("lens", [[4001], [900] * 9, [33, 5000, 0, 1]])
+@pytest.mark.parametrize("d, group, hq", [(64, 32, 4), (64, 64, 40), (128, 128, 4), (256, 64, 6)])
+def test_decode_merges_of_many_and_few_pieces(d, group, hq, lens):
+    check(*build(lens, hq, 2, d, group, 16, torch.bfloat16, seed=18))
+
+
 def test_decode_sharp_scores():
     """Scores spread over hundreds, rising and falling along the context."""
     cache, table, q, data, lens = build([900, 640], 8, 2, 128, 64, 16, torch.bfloat16, seed=5)
