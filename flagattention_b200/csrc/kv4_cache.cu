@@ -113,13 +113,15 @@ __device__ __forceinline__ uint32_t quantise(const uint4 &u, uint32_t &pair) {
   // codes as integers in the mantissa of kMagic
   constexpr uint32_t kMagicBits = 0x4b400000u;
   uint32_t n[8];
-  if (normal && s2 >= 0x1p-100f) {
+  // Half of a scale that is normal in T (bf16: far above subnormal in f32 too).
+  constexpr float kNormalHalf = std::is_same<T, __half>::value ? 0x1p-15f : 0x1p-100f;
+  if (normal && s2 >= kNormalHalf) {
     // rint((x - lo) / s), at most 15: the scale is off by 2^-8 of itself at most
     const float r = reciprocal(s2);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       n[i] = __float_as_uint(quotient(fmaf(Elem<T>::to_f(e[i]), 0.5f, -lo2), s2, r) + kMagic);
-  } else {  // a subnormal scale may be off by half: the quotient may pass 15
+  } else {  // a scale subnormal in T may be off by half: the quotient may pass 15
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       n[i] = __float_as_uint(

@@ -160,6 +160,24 @@ def test_subnormal_ranges():
         assert same(got, values(x, 64).to(x.dtype))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_subnormal_scales(dtype):
+    """Ranges of 1 .. 255 of the type's smallest steps: a scale of a few steps is
+    off by up to half a step (22 steps: 1.47 rounds to 1), so the largest quotient
+    passes 15 by up to half again and is cut there."""
+    step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    tops = torch.arange(1, 256, device="cuda")[:, None]
+    dim = torch.arange(64, device="cuda")
+    n = torch.where(dim % 9 == 4, tops, dim * dim % (tops + 1))   # the largest beside others
+    x = (n.double() * step).to(dtype)[:, None]
+    assert torch.equal(x.double()[:, 0], n.double() * step)
+    cache = fa.Int4KVCache(16, 1, 16, 64, dtype=dtype)
+    slots = torch.arange(255, device="cuda")
+    fa.append_kv_int4(x, -x, cache, slots)
+    for got, rows_ in zip(fa.read_kv_int4(cache, slots), (x, -x)):
+        assert same(got, values(rows_, 64).to(dtype))
+
+
 def build(lens, hq, hk, d, group, block, dtype, seed=0, size=1.0, pool_extra=3):
     """Cache with shuffled pages whose unused slots hold NaN scales and any
     codes, the query, and the rows of each sequence."""
