@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&bars->k_full[i]), 1);
-      mbar_init(smem_u32(&bars->k_empty[i]), 2);  // once per Q tile
+      mbar_init(smem_u32(&bars->k_empty[i]), 2);  // by each Q tile's stream
       mbar_init(smem_u32(&bars->v_full[i]), 1);
       mbar_init(smem_u32(&bars->v_empty[i]), 2);
     }
@@ -779,43 +779,69 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The two Q tiles are independent streams of products, each waiting for
     // its own rows: one tile's next unit starts while the other still ends
     // its last.  While both wait for their rows they are served in turn.
+    //
+    // A parity wait tells a phase from the one before it only, so a stream sees
+    // every K and every V tile land, in order, and releases each itself: those it
+    // multiplies when their products are done, those it has no step for
+    // as soon as they land (walk).  Scores of tile t are issued once V tile t -
+    // kVStages has been seen, so the rows' own wait for V tile t can not be
+    // answered by an earlier phase either.
     enum Need { kUnit, kQK, kP, kNone };
     struct Stream {
       Need need = kUnit;
-      uint32_t unit = 0, g = 0, q = 0, steps = 0;  // units, K / V tiles, Q tiles begun; P taken
-      int i = 0, left = 0, n = 0, other = 0;       // step; steps of this tile, the unit, the other tile
+      uint32_t unit = 0, q = 0, steps = 0;  // units, Q tiles begun; P taken
+      uint32_t g = 0, k = 0, v = 0;  // first tile of the unit; next K, V tile to see
+      int i = 0, left = 0, n = 0;    // step; steps of this tile, of the unit
     } st0, st1;
-    // stage released by this tile, and for the other one where it has no such step
-    auto release = [&](uint64_t *empty, const Stream &s) {
-      tc_commit_warp(smem_u32(empty));
-      if (s.i >= s.other && lane == 0) mbar_arrive(smem_u32(empty));
+    auto k_landed = [&](uint32_t t) {
+      return ready(&bars->k_full[t % PL::kKStages], (t / PL::kKStages) & 1u);
+    };
+    auto v_landed = [&](uint32_t t) {
+      return ready(&bars->v_full[t % PL::kVStages], (t / PL::kVStages) & 1u);
+    };
+    // tiles before the unit's first that the stream has no step for
+    auto walk = [&](Stream &s) -> bool {
+      bool moved = false;
+      while (s.k < s.g && k_landed(s.k)) {
+        if (lane == 0) mbar_arrive(smem_u32(&bars->k_empty[s.k % PL::kKStages]));
+        ++s.k;
+        moved = true;
+      }
+      while (s.v < s.g && v_landed(s.v)) {
+        if (lane == 0) mbar_arrive(smem_u32(&bars->v_empty[s.v % PL::kVStages]));
+        ++s.v;
+        moved = true;
+      }
+      return moved;
     };
     // whatever needs no rows: the next unit, the next scores
     auto feed = [&](int x, Stream &s) -> bool {
       bool moved = false;
       while (s.need == kUnit) {
         const uint32_t slot = s.unit & 1u;
-        if (!ready(&bars->work_full[slot], (s.unit >> 1) & 1u)) return moved;
+        if (!ready(&bars->work_full[slot], (s.unit >> 1) & 1u)) break;
         const Work &w = bars->work[slot];
         const bool none = w.kvh < 0;
-        s.g += s.n;
         s.i = 0;
         s.n = none ? 0 : w.j1 - w.j0;
-        s.left = none ? 0 : w.end[x] - w.j0;
-        s.other = none ? 0 : w.end[x ^ 1] - w.j0;
+        s.left = none ? 0 : max(w.end[x] - w.j0, 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars->work_empty[slot]));
         ++s.unit;
         s.need = none ? kNone : (s.left > 0 ? kQK : kUnit);
+        if (s.need == kUnit) s.g += s.n;
         moved = true;
       }
+      moved |= walk(s);
       if (s.need == kQK) {
-        const uint32_t t = s.g + s.i, ks = t % PL::kKStages;
+        const uint32_t t = s.g + s.i;
+        if (s.k < t || s.v + PL::kVStages <= t) return moved;
         if (s.i == 0 && !ready(&bars->q_full[x], s.q & 1u)) return moved;
-        if (!ready(&bars->k_full[ks], (t / PL::kKStages) & 1u)) return moved;
+        if (!k_landed(t)) return moved;
         tc_fence_after();
-        issue_qk(x, ks);
-        release(&bars->k_empty[ks], s);
+        issue_qk(x, t % PL::kKStages);
+        tc_commit_warp(smem_u32(&bars->k_empty[t % PL::kKStages]));
+        ++s.k;
         if (s.i == s.left - 1) {
           tc_commit_warp(smem_u32(&bars->q_empty[x]));
           ++s.q;
@@ -831,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the first part of this step's P is there (or waited for); then its value
     // product and the next scores
     auto serve = [&](int x, Stream &s) -> bool {
-      const uint32_t t = s.g + s.i, vs = t % PL::kVStages;
+      const uint32_t vs = s.v % PL::kVStages;
       if (!wait(&bars->p_full[x][0], s.steps & 1u)) return false;
       tc_fence_after();
       issue_pv(x, vs, 0, s.i == 0);
@@ -840,8 +866,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       issue_pv(x, vs, 1, false);
       ++s.steps;
       if (s.i == s.left - 1) tc_commit_warp(smem_u32(&bars->o_full[x]));
-      release(&bars->v_empty[vs], s);
+      tc_commit_warp(smem_u32(&bars->v_empty[vs]));
+      ++s.v;
       s.need = ++s.i < s.left ? kQK : kUnit;
+      if (s.need == kUnit) s.g += s.n;
       feed(x, s);
       return true;
     };
@@ -851,10 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A tile can be served once its V tile is there: a tile that is ahead of
       // the other waits for stages the other has yet to release, so the issuer
       // must not block on it.
-      auto v_ready = [&](const Stream &s) {
-        const uint32_t t = s.g + s.i;
-        return ready(&bars->v_full[t % PL::kVStages], (t / PL::kVStages) & 1u);
-      };
+      auto v_ready = [&](const Stream &s) { return s.v == s.g + s.i && v_landed(s.v); };
       const bool w0 = st0.need == kP && v_ready(st0), w1 = st1.need == kP && v_ready(st1);
       // serve tile 0 / 1 (blocking on its rows): its turn while both could be,
       // or the other has no work left; otherwise only when its rows are done
@@ -870,8 +895,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         turn = 0;
       }
       bool moved = go0 || go1;
-      if (st0.need < kP) moved |= feed(0, st0);
-      if (st1.need < kP) moved |= feed(1, st1);
+      moved |= feed(0, st0);
+      moved |= feed(1, st1);
       if (moved) {
         idle = 0;
         continue;

@@ -196,6 +196,19 @@ def test_views_past_32_bit_offsets():
     check(q, k, v, [2000, 100], [2000, 100])
 
 
+@pytest.mark.parametrize("d, dv", [(192, 128), (128, 128), (64, 64)])
+def test_units_with_uneven_tiles_and_short_ones_in_turn(d, dv):
+    """Pairs of Q tiles of which one ends a key tile early or has no token,
+    followed on their SM by sequences of less than one key tile; the keys of
+    some are more than the queries'.  Bit-identical when repeated."""
+    lens_q = [200, 60, 129, 17, 256, 100, 90, 1] * 25
+    lens_k = [200, 60, 500, 17, 256, 100, 700, 3] * 25
+    case = tensors(lens_q, lens_k, 16, 16, d, dv, torch.bfloat16, seed=16)
+    first = check(*case, lens_q, lens_k)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, check(*case, lens_q, lens_k)))
+
+
 def test_many_sequences_and_long_ones():
     lens = [1 + (i * 37) % 90 for i in range(700)]
     check(*tensors(lens, lens, 4, 1, 64, 64, torch.bfloat16, seed=7), lens, lens)
