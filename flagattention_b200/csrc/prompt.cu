@@ -799,7 +799,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto v_landed = [&](uint32_t t) {
       return ready(&bars->v_full[t % PL::kVStages], (t / PL::kVStages) & 1u);
     };
-    // tiles before the unit's first that the stream has no step for
+    // tiles before the unit's first that the stream has no step for, V after K:
+    // none is left when v has come to g
     auto walk = [&](Stream &s) -> bool {
       bool moved = false;
       while (s.k < s.g && k_landed(s.k)) {
@@ -807,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++s.k;
         moved = true;
       }
-      while (s.v < s.g && v_landed(s.v)) {
+      while (s.v < s.g && s.v < s.k && v_landed(s.v)) {
         if (lane == 0) mbar_arrive(smem_u32(&bars->v_empty[s.v % PL::kVStages]));
         ++s.v;
         moved = true;
@@ -895,8 +896,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         turn = 0;
       }
       bool moved = go0 || go1;
-      moved |= feed(0, st0);
-      moved |= feed(1, st1);
+      // only what each can do now: the loop's length is in every step's chain
+      if (st0.need < kP) moved |= feed(0, st0);
+      else if (st0.v < st0.g) moved |= walk(st0);
+      if (st1.need < kP) moved |= feed(1, st1);
+      else if (st1.v < st1.g) moved |= walk(st1);
       if (moved) {
         idle = 0;
         continue;

@@ -141,7 +141,8 @@ class Model:
 
         def walk(s):
             for key, stages in (("k", self.k), ("v", self.v)):
-                while s[key] < s["g"] and (self.on_behalf or landed(stages, s[key])):
+                while s[key] < s["g"] and (key == "k" or s["v"] < s["k"]) and \
+                        (self.on_behalf or landed(stages, s[key])):
                     if not self.on_behalf:
                         stages[s[key] % len(stages)].empty.arrive()
                     s[key] += 1
@@ -210,7 +211,10 @@ class Model:
                 yield from serve(streams[go])
                 turn = go ^ 1
             for s in streams:
-                feed(s)
+                if s["need"] in ("unit", "qk"):
+                    feed(s)
+                elif s["v"] < s["g"]:
+                    walk(s)
             yield
 
     # --------------------------------------------------------- the hardware
