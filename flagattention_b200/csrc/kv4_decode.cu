@@ -27,9 +27,13 @@
 // contexts of up to 65536 tokens from 147 us to 107.
 //
 // f16 operands hold Q and P' = p * s exactly enough because both are brought
-// near the top of its range by a power of two: Q by its row's largest
-// magnitude (bf16 and f16 queries then lose nothing above 2^-27 of it), P' by
-// the largest value scale a warp has met.
+// into its range by a power of two: Q by its row's largest magnitude (bf16 and
+// f16 queries then lose nothing above 2^-23 of it), P' by the largest product
+// that a warp has met for the head and group of dims.  Small ones are then off by
+// 2^-28 of that at most, so neither a large token that has no weight, nor one that only
+// another head attends to, nor another group of large values costs accuracy (one
+// unit for all heads and groups, by the largest scale: 9% off beside a
+// token 10^5 times larger that has no weight).
 //
 // Four warps of a CTA share a piece (a run of 64-token blocks of one entry),
 // one 16-token tile each per block, loaded straight into registers one tile
@@ -60,8 +64,11 @@ Pool pool_of(const fa_kv4_cache *c);
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlockTokens = kWarps * kTileTokens;  // schedule unit: one tile per warp
-constexpr float kRescaleThreshold = 8.0f;           // log2 units (factor 256): p <= 2^8
-constexpr float kValueScaleTop = 64.f;              // normalised value scales: P' <= 2^14
+// P' = p * s * unit, the unit a power of two for each head and group: the largest
+// p * s met lands in [2^3, 2^4), and maxima and units move when p passes 2^7 or
+// a scale times its unit 2^8, so P' stays below 2^15.
+constexpr float kRescaleThreshold = 7.f;
+constexpr int kUnitTop = 3, kLimitTop = 8, kUnitMost = 100;
 // Stands for "no key yet" as a running maximum: below every finite score, and
 // finite, so that differences with it need no special case.
 constexpr float kNoMax = -3.0e38f;
@@ -413,18 +420,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
     }
 
     // running state; lanes of equal q agree on m; l and extra are partial sums
-    // over the lane's tokens; vnorm normalises the value scales (warp-uniform)
-    float vnorm = 1.f;
-    bool fresh = true;
-    float m[kNT][2], l[kNT][2], extra[kNT][kGroups][2], o[kNT][kD / 16][4];
+    // over the lane's tokens; pu: P' per p * s, a power of two
+    float o[kNT][kD / 16][4];
+    uint64_t pu[kNT][kGroups], m[kNT], l[kNT], extra[kNT][kGroups];  // heads 2 q, 2 q + 1
+    float limit[kGroups];  // of value scales: 2^kLimitTop over the lane's largest unit
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) limit[g] = 0.f;
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
+      m[t] = f32x2(kNoMax, kNoMax);
+      l[t] = 0u;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m[t][h] = kNoMax;
-        l[t][h] = 0.f;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) extra[t][g][h] = 0.f;
+      for (int g = 0; g < kGroups; ++g) {
+        extra[t][g] = 0u;
+        pu[t][g] = f32x2(pow2(kUnitMost), pow2(kUnitMost));
       }
 #pragma unroll
       for (int i = 0; i < kD / 16; ++i)
@@ -517,71 +526,110 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
         }
       }
       // --------------------------------------------------- running softmax
-      float top = -INFINITY, big = 0.f;  // excess over the maxima; largest value scale
+      uint64_t pa[kNT], pb[kNT];  // p of tokens r and r + 8
+      auto weights = [&](int t) {
+        float m0, m1;
+        f32x2_split(m[t], m0, m1);
+        pa[t] = f32x2(fast_exp2(s[t][0] - m0), fast_exp2(s[t][1] - m1));
+        pb[t] = f32x2(fast_exp2(s[t][2] - m0), fast_exp2(s[t][3] - m1));
+      };
+      float top = -INFINITY;  // excess over the maxima
+      bool over = false;      // a value scale past its limit
 #pragma unroll
-      for (int t = 0; t < kNT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(s[t][h], s[t][h + 2]) - m[t][h]);
-#pragma unroll
-      for (int g = kGroups; g < 2 * kGroups; ++g) {
-        float lo, sa, sb;
-        pair_of<T>(sca[g], lo, sa);
-        pair_of<T>(scb[g], lo, sb);
-        big = fmax3(big, sa, sb);
+      for (int t = 0; t < kNT; ++t) {
+        float m0, m1;
+        f32x2_split(m[t], m0, m1);
+        top = fmax3(top, fmaxf(s[t][0], s[t][2]) - m0, fmaxf(s[t][1], s[t][3]) - m1);
       }
-      if (__any_sync(0xffffffffu, top > kRescaleThreshold || big * vnorm > kValueScaleTop)) {
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1)
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-        float shrink = 1.f;  // of what the value products hold
-        if (fresh || big * vnorm > kValueScaleTop) {
-          fresh = false;
-          // scales up to `big` land below 32: room for the next to be larger
-          const float larger = pow2(min(max(4 - exponent_of(big), -100), 100));
-          shrink = larger / vnorm;
-          vnorm = larger;
-        }
+      for (int g = 0; g < kGroups; ++g) {
+        float lo, sa, sb;
+        pair_of<T>(sca[kGroups + g], lo, sa);
+        pair_of<T>(scb[kGroups + g], lo, sb);
+        over |= fmaxf(sa, sb) > limit[g];
+      }
+      if (__any_sync(0xffffffffu, over || top > kRescaleThreshold)) {
+        // Maxima are whole numbers: held sums move by powers of two, and a unit
+        // stays that of the largest product met, in this tile or before.
+        float most[kGroups];  // the lane's largest units
 #pragma unroll
-        for (int t = 0; t < kNT; ++t)
+        for (int g = 0; g < kGroups; ++g) most[g] = 0.f;
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          float mh[2], up[2], alpha[2];  // 2^n and 2^-n where the maximum grows by n
+          f32x2_split(m[t], mh[0], mh[1]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float mx = fmaxf(s[t][h], s[t][h + 2]);
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1)
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            const float mn = fmaxf(m[t][h], mx);
-            const float alpha = fast_exp2(m[t][h] - mn);
-            m[t][h] = mn;
-            l[t][h] *= alpha;
+            const float mn = fmaxf(mh[h], ceilf(mx));
+            up[h] = pow2(static_cast<int>(fminf(mn - mh[h], 127.f)));
+            alpha[h] = fast_exp2(mh[h] - mn);
+            mh[h] = mn;
+          }
+          m[t] = f32x2(mh[0], mh[1]);
+          weights(t);
+          const uint64_t alpha2 = f32x2(alpha[0], alpha[1]);
+          l[t] = fmul2(l[t], alpha2);
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) extra[t][g][h] *= alpha;
+          for (int g = 0; g < kGroups; ++g) {
+            float lo, sa, sb, x0, x1, x2, x3, unit[2];
+            pair_of<T>(sca[kGroups + g], lo, sa);
+            pair_of<T>(scb[kGroups + g], lo, sb);
+            f32x2_split(fmul2(pa[t], f32x2(sa, sa)), x0, x1);
+            f32x2_split(fmul2(pb[t], f32x2(sb, sb)), x2, x3);
+            // exponent fields (bias 127) of both heads' largest products
+            uint32_t big = __float_as_uint(fmaxf(x0, x2)) >> 23 |
+                           __float_as_uint(fmaxf(x1, x3)) >> 23 << 16;
 #pragma unroll
-            for (int i2 = 0; i2 < kD / 16; ++i2) {
-              o[t][i2][h] *= alpha * shrink;
-              o[t][i2][h + 2] *= alpha * shrink;
-              if (base >= 64) {
-                kept[((t * (kD / 16) + i2) * 4 + h) * 32] *= alpha * shrink;
-                kept[((t * (kD / 16) + i2) * 4 + h + 2) * 32] *= alpha * shrink;
+            for (int off = 4; off < 32; off <<= 1)
+              big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, off));
+            f32x2_split(pu[t][g], unit[0], unit[1]);
+            extra[t][g] = fmul2(extra[t][g], alpha2);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int field = static_cast<int>(h ? big >> 16 : big & 0xffffu);
+              const float now =
+                  fminf(unit[h] * up[h], pow2(min(127 + kUnitTop - field, kUnitMost)));
+              // 1 / 2^e: the exponent field mirrored about 127
+              const float inv = __uint_as_float(0x7f000000u - __float_as_uint(unit[h]));
+              const float held = alpha[h] * (now * inv);
+              unit[h] = now;
+              most[g] = fmaxf(most[g], now);
+#pragma unroll
+              for (int i2 = 0; i2 < kD / 16; ++i2) {
+                if ((64 * (i2 / 4) + 32 * (i2 % 4 / 2)) / kG != g) continue;
+                o[t][i2][h] *= held;
+                o[t][i2][h + 2] *= held;
+                if (base >= 64) {
+                  kept[((t * (kD / 16) + i2) * 4 + h) * 32] *= held;
+                  kept[((t * (kD / 16) + i2) * 4 + h + 2) * 32] *= held;
+                }
               }
             }
+            pu[t][g] = f32x2(unit[0], unit[1]);
           }
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          limit[g] = __uint_as_float(0x7f000000u + (kLimitTop << 23) - __float_as_uint(most[g]));
       }
       // ---------------------------------------------------------- P and P V
       uint32_t pf[kNT][kGroups][kSplitP ? 4 : 2];  // B operands (high, then low parts)
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
-        const float p0 = fast_exp2(s[t][0] - m[t][0]), p1 = fast_exp2(s[t][1] - m[t][1]);
-        const float p2 = fast_exp2(s[t][2] - m[t][0]), p3 = fast_exp2(s[t][3] - m[t][1]);
-        l[t][0] += p0 + p2;
-        l[t][1] += p1 + p3;
+        weights(t);
+        l[t] = fadd2(l[t], fadd2(pa[t], pb[t]));
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-          float loa, sa, lob, sb;
+          float loa, sa, lob, sb, x0, x1, x2, x3;
           pair_of<T>(sca[kGroups + g], loa, sa);
           pair_of<T>(scb[kGroups + g], lob, sb);
-          sa *= vnorm;
-          sb *= vnorm;
-          const float x0 = p0 * sa, x1 = p1 * sa, x2 = p2 * sb, x3 = p3 * sb;
+          // in this order: p = 0 stays 0 whatever the unit and the scale
+          f32x2_split(fmul2(fmul2(pa[t], pu[t][g]), f32x2(sa, sa)), x0, x1);
+          f32x2_split(fmul2(fmul2(pb[t], pu[t][g]), f32x2(sb, sb)), x2, x3);
           const uint32_t wa = Elem<__half>::pack2(x0, x1), wb = Elem<__half>::pack2(x2, x3);
           pf[t][g][0] = transpose8(wa);
           pf[t][g][1] = transpose8(wb);
@@ -591,8 +639,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
             pf[t][g][2] = transpose8(Elem<__half>::pack2(x0 - __low2float(ha), x1 - __high2float(ha)));
             pf[t][g][3] = transpose8(Elem<__half>::pack2(x2 - __low2float(hb), x3 - __high2float(hb)));
           }
-          extra[t][g][0] = fmaf(p0, loa, fmaf(p2, lob, extra[t][g][0]));
-          extra[t][g][1] = fmaf(p1, loa, fmaf(p3, lob, extra[t][g][1]));
+          extra[t][g] = ffma2(pa[t], f32x2(loa, loa), ffma2(pb[t], f32x2(lob, lob), extra[t][g]));
         }
       }
       if (at >= 0) load_scales(next);
@@ -643,34 +690,41 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
           make_int4(final_out ? -1 : sh.parts + self, self + 1, last - self, 0);
     }
 #pragma unroll
-    for (int t = 0; t < kNT; ++t)
+    for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[t] = fadd2(l[t], __shfl_xor_sync(0xffffffffu, l[t], off));
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          extra[t][g] = fadd2(extra[t][g], __shfl_xor_sync(0xffffffffu, extra[t][g], off));
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], off);
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-            extra[t][g][h] += __shfl_xor_sync(0xffffffffu, extra[t][g][h], off);
-        }
+        auto of_head = [&](uint64_t x) {
+          float x0, x1;
+          f32x2_split(x, x0, x1);
+          return h ? x1 : x0;
+        };
         if (r == 0) {
-          ctl.m[warp][t * 8 + 2 * q + h] = m[t][h];
-          ctl.l[warp][t * 8 + 2 * q + h] = l[t][h];
+          ctl.m[warp][t * 8 + 2 * q + h] = of_head(m[t]);
+          ctl.l[warp][t * 8 + 2 * q + h] = of_head(l[t]);
         }
         float *row = obuf + (warp * kHeads + t * 8 + 2 * q + h) * PL::kORow;
 #pragma unroll
         for (int u = 0; u < kU; ++u)
 #pragma unroll
           for (int pp = 0; pp < 2; ++pp) {
-            const float ex = extra[t][(64 * u + 32 * pp) / kG][h];
-            const float even = 0x1p24f / vnorm, odd = 0x1p20f / vnorm;
+            const float ex = of_head(extra[t][(64 * u + 32 * pp) / kG]);
+            const float inv = 1.f / of_head(pu[t][(64 * u + 32 * pp) / kG]);
+            constexpr float even = 0x1p24f, odd = 0x1p20f;
             const float *oa = o[t][4 * u + 2 * pp], *ob = o[t][4 * u + 2 * pp + 1];
             // codes 2 pp and 2 pp + 1 of rows m < 8, then of rows m >= 8
             *reinterpret_cast<float4 *>(row + 64 * u + 32 * pp + 4 * r) =
-                make_float4(fmaf(oa[h], even, ex), fmaf(ob[h], odd, ex), fmaf(oa[h + 2], even, ex),
-                            fmaf(ob[h + 2], odd, ex));
+                make_float4(fmaf(oa[h] * even, inv, ex), fmaf(ob[h] * odd, inv, ex),
+                            fmaf(oa[h + 2] * even, inv, ex), fmaf(ob[h + 2] * odd, inv, ex));
           }
       }
+    }
     __syncthreads();
     constexpr int kPer = kThreads / kHeads;       // threads of one head's row
     const int hh = threadIdx.x / kPer, part = threadIdx.x % kPer;

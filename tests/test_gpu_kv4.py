@@ -311,6 +311,46 @@ def test_decode_f16_range(size):
     check(*build([400, 33], 8, 1, 128, 64, 16, torch.float16, seed=6, size=size))
 
 
+@pytest.mark.parametrize("dtype, factor, bound", [(torch.bfloat16, 1e3, 3e-3), (torch.bfloat16, 1e5, 3e-3),
+                                                  (torch.float16, 1e4, 1e-3)])
+@pytest.mark.parametrize("d, group, hq", [(128, 64, 8), (64, 32, 8), (256, 64, 8), (128, 32, 40)])
+@pytest.mark.parametrize("kind", ["first token", "middle token", "group", "some heads' token"])
+def test_decode_values_of_very_different_sizes(kind, d, group, hq, dtype, factor, bound):
+    """Large value rows that nobody or only some heads attend to, or one large
+    group, take nothing from the rest.  2-norm against 64 bits of every head and
+    group by itself; the bound is that of
+    ``test_decode_long_context_keeps_its_accuracy``: what is added, products p * s
+    that are small next to the largest one of their head and group, is off by
+    15 * 2^-28 of that per token, 2^-28 * 15 sqrt(20000) = 8e-6 together.  One
+    sequence spread over the GPU, and a batch of which every CTA holds whole ones."""
+    n, hk = 20000, 2
+    cache, table, q, data, lens = build([n], hq, hk, d, group, 64, dtype, seed=19)
+    (k, v), = data
+    q *= 3                                                # scores of standard deviation 3
+    q[..., 0] = 8
+    if kind == "some heads' token":
+        q[:, 1::2, 0] = -8                                # the even heads see only that token
+    far = 40 * d ** 0.5 / 8                               # scores 40 apart
+    k[..., 0] = 0
+    if kind == "group":
+        v[..., :group] *= factor
+    else:
+        t = 0 if kind == "first token" else n // 2
+        k[t, :, 0] = far if kind == "some heads' token" else -far
+        v[t, :, :group if kind == "some heads' token" else d] *= factor
+    t = torch.arange(n, device="cuda")
+    fa.append_kv_int4(k, v, cache, table[0].long()[t // 64] * 64 + t % 64)
+    kk, vv = (_exact(x, group).transpose(0, 1).repeat_interleave(hq // hk, 0) for x in (k, v))
+    p = torch.softmax(d ** -0.5 * q[0].double()[:, None] @ kk.transpose(1, 2), -1)
+    want = (p @ vv)[:, 0].unflatten(-1, (-1, group))
+    for batch in (1, 600):                                # the same pages for all
+        out = fa.paged_attention_int4(q.expand(batch, -1, -1), cache, lens.expand(batch),
+                                      table.expand(batch, -1))
+        for b in {0, batch // 2, batch - 1}:
+            off = (out[b].double().unflatten(-1, (-1, group)) - want).norm(dim=-1) / want.norm(dim=-1)
+            assert (off <= bound).all(), off.max()
+
+
 def test_decode_nan_stays_and_does_not_spread():
     lens = [50, 70]
     cache, table, q, data, n = build(lens, 4, 2, 128, 64, 16, torch.bfloat16, seed=7)
