@@ -35,6 +35,12 @@
 //   warps 0-7 / 8-15: rows of Q tile 0 / 1 (two threads per row, S read from
 //     TMEM, P written over it as the A operand of P V)
 //   warp 16: MMA issuer    warp 17: TMA producer    warp 18: scheduler
+//   warp 19: value rows at the edge
+//
+// A weight of 0 does not hide a value: 0 * NaN is NaN.  In V tiles with keys
+// that not every row of the unit sees, warp 19 (with one V stage the row warps) clears
+// the rows that none sees, the next sequence's among them, and every infinity or NaN
+// that only some see, and notes its key; the rows that see it add it to what they store.
 //
 // TMEM: S0 S1 (128 columns each, P in place), O0 O1.  A tile's products are
 // issued in order, so the barrier that announces S of step j also says that P V of
@@ -54,10 +60,10 @@
 namespace fa {
 namespace prompt {
 
-// One warp beyond the roles fills up the last warpgroup, which gives its
-// registers to the row warps: 16 * 112 + 4 * 32 = 20 * 96, the launch's.
+// The last warpgroup gives registers to the row warps: 16 * 112 + 4 * 32 = 20 *
+// 96, the launch's (launch_t refuses any other: a split with a larger sum waits for ever).
 constexpr int kThreads = 640, kRowRegs = 112, kOtherRegs = 32;
-constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17, kSchedulerWarp = 18;
+constexpr int kRowWarps = 16, kMmaWarp = 16, kProducerWarp = 17, kSchedulerWarp = 18, kEdgeWarp = 19;
 constexpr int kTile = 128;                 // rows of a Q tile, keys of a K / V tile
 constexpr uint32_t kTmemCols = 512;
 // O is rescaled only when the maximum grows by more than this (log2 units):
@@ -73,6 +79,10 @@ struct Plan {
   static constexpr int kVBytes = kVChunks * kChunkBytes;
   static constexpr int kKStages = kDqk == 192 ? 2 : (kDqk == 128 ? 3 : 4);
   static constexpr int kVStages = kDqk == 192 ? 1 : (kDqk == 128 ? 2 : 4);
+  // With one stage a V tile lands when its products are due: its readers' 256
+  // threads clear it (a few hundred cycles) and not one warp (about 2000; 2 prompts
+  // of 1000 to 2048 tokens, 128 heads of 192 / 128: 395 us so, 363 by the rows).
+  static constexpr bool kRowsClear = kVStages == 1;
   static constexpr int kOffX = 1024;
   static constexpr int kOffQ = kOffX + 2048;  // past the exchange block
   static constexpr int kOffK = kOffQ + 2 * kQBytes;
@@ -96,6 +106,7 @@ struct Work {
 struct Bars {
   uint64_t q_full[2], q_empty[2];  // per Q tile
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t v_raw[4];               // a V tile that the edge warp has to look at first
   uint64_t s_full[2], o_full[2];
   uint64_t p_full[2][2];  // [Q tile][first 48 / last 16 columns of both halves]
   uint64_t work_full[2], work_empty[2];
@@ -105,6 +116,12 @@ struct Bars {
   Work work[2];
   uint32_t tmem_base;
   int abort_flag;
+  // Keys of unit k whose infinities or NaN were cleared, from the unit's first
+  // hidden key on, in marks[k % 3]: a unit is handed out when all warps have begun
+  // the last but one, so three are told apart.
+  struct Marks {
+    uint32_t any, keys[8];
+  } marks[3];
 };
 // Row maxima, at the end row sums, that the two threads of a row exchange.
 struct Exchange {
@@ -115,6 +132,8 @@ static_assert(sizeof(Bars) <= 1024, "barrier block");
 
 struct Params {
   const int32_t *cu_q, *cu_k;
+  const void *v;  // as the tensor map has it
+  int64_t v_st, v_sh;
   int32_t batch, total_q, total_k, hq, hkv, group, tq;  // tq: tokens of a Q tile
   int32_t items;     // upper bound of the (sequence, Q tile pair) items
   int32_t splits;    // units an item's keys are cut into
@@ -134,6 +153,16 @@ __device__ __forceinline__ void seq_range(const int32_t *cu, int b, int total, i
                                           int &len) {
   start = min(max(__ldg(cu + b), 0), total);
   len = min(max(__ldg(cu + b + 1), start), total) - start;
+}
+
+// Keys that every row, and that any row of a unit sees: [0, all), [0, some).
+struct Seen {
+  int all, some;
+};
+__device__ __forceinline__ Seen seen_keys(const Params &p, const Work &w) {
+  if (!p.causal) return {w.lk, w.lk};
+  const int last = min(w.i0 + 2 * p.tq, w.lq);  // past the last token
+  return {max(w.i0 + 1 + w.lk - w.lq, 0), max(last + w.lk - w.lq, 0)};
 }
 
 // mbar_wait without its out-of-line loop: setmaxnreg does not go with calls.
@@ -188,6 +217,60 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
+// 0 * x + y of two halves.
+template <typename T>
+__device__ __forceinline__ uint32_t zero_of(uint32_t x, uint32_t y) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0u), "r"(y));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0u), "r"(y));
+  return d;
+}
+
+// Clears what rows of a V tile may hold that its readers must not meet: rows r0 ..
+// r1 - 1 lose infinities and NaN, which are noted (key0: the tile's first key, from
+// the unit's first hidden one on), rows from r1 on everything.  Done by n threads, i
+// of which calls; 16-byte units, kLoads on their way at a time.
+template <typename T, int kChunks, int kChunkBytes, int kLoads>
+__device__ __forceinline__ void clear_hidden(uint8_t *tile, int r0, int r1, int key0,
+                                             Bars::Marks &marks, int i, int n) {
+  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  auto finite = [](uint32_t y) {  // its halves, 0 for an infinity or a NaN
+    if ((y & 0x7fffu) >= kInf) y &= 0xffff0000u;
+    if ((y >> 16 & 0x7fffu) >= kInf) y &= 0xffffu;
+    return y;
+  };
+#pragma unroll
+  for (int ch = 0; ch < kChunks; ++ch) {
+    uint4 *at = reinterpret_cast<uint4 *>(tile + ch * kChunkBytes);
+    for (int u0 = r0 * 8 + i; u0 < r1 * 8; u0 += n * kLoads) {
+      uint4 x[kLoads];
+      uint32_t none = 0u;  // 0 * x + 0 is 0 unless x is an infinity or a NaN
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) x[k] = at[min(u0 + n * k, r1 * 8 - 1)];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        none |= zero_of<T>(x[k].x, zero_of<T>(x[k].y, zero_of<T>(x[k].z, zero_of<T>(x[k].w, 0u))));
+      if (none == 0u) continue;
+#pragma unroll 1
+      for (int k = 0; k < kLoads && u0 + n * k < r1 * 8; ++k) {
+        const int u = u0 + n * k;
+        const uint4 y = at[u], z = make_uint4(finite(y.x), finite(y.y), finite(y.z), finite(y.w));
+        if (((y.x ^ z.x) | (y.y ^ z.y) | (y.z ^ z.z) | (y.w ^ z.w)) == 0u) continue;
+        const int key = key0 + u / 8;  // fewer than a unit's tokens
+        atomicOr(&marks.keys[key >> 5], 1u << (key & 31));
+        atomicOr(&marks.any, 1u);
+        __threadfence_block();  // who finds the element cleared finds its mark
+        at[u] = z;
+      }
+    }
+#pragma unroll 4
+    for (int u = r1 * 8 + i; u < kTile * 8; u += n) at[u] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+}
+
 // Rows of Q tile x: two threads per row, each with half of the key tile's
 // columns (`half`) and of O's.  A wait that gives up does not end the loop
 // (every wait returns at once from then on): the two warps of a row keep
@@ -195,7 +278,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 template <typename T, int kDqk, int kDv>
 __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *bars,
                                          uint8_t *smem, uint32_t tmem, int warp, int lane,
-                                         uint32_t &steps, uint32_t &outs, uint32_t tiles) {
+                                         uint32_t &steps, uint32_t &outs, uint32_t unit,
+                                         uint32_t tiles) {
   using PL = Plan<kDqk, kDv>;
   constexpr int kCols = kTile / 2, kOCols = kDv / 2;
   volatile int *abort_flag = &bars->abort_flag;
@@ -278,25 +362,6 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
         }
       }
     }
-    // Value rows past the sequence's end belong to the next sequence and may
-    // hold infinities or NaN; P is 0 there but 0 * NaN is not: clear them
-    // (both Q tiles do, before their own products; either may come first), an
-    // eighth of the rows each warp.
-    if (it.lk < (j + 1) * kTile) {
-      const uint32_t v_tile = tiles + (j - it.j0);
-      const int st = v_tile % PL::kVStages;
-      warp_wait(smem_u32(&bars->v_full[st]), (v_tile / PL::kVStages) & 1u, abort_flag, p.status,
-                kDevTimeoutSoftmax);
-      const uint32_t tile = smem_u32(smem + PL::kOffV) + st * PL::kVBytes;
-      const int r0 = it.lk - j * kTile;
-      const int units = (kTile - r0) * 8;  // 16-byte units of a chunk's rows
-      for (int u = (warp & 7) * 32 + lane; u < units * PL::kVChunks; u += 256)
-        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
-                         tile + (u / units) * PL::kChunkBytes + r0 * 128 + (u % units) * 16),
-                     "r"(0u)
-                     : "memory");
-      fence_proxy_async_smem();
-    }
     const float msafe = m_use == -INFINITY ? 0.f : m_use;
     const uint64_t nm2 = f32x2(-msafe, -msafe);
     uint64_t acc2 = f32x2(0.f, 0.f), acc2b = f32x2(0.f, 0.f);
@@ -321,8 +386,7 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
           acc2 = fadd2(acc2, y[c]);
       }
     };
-    // P of the first 48 or the last 16 columns (and the rescaled O, the cleared
-    // V) is there: most of the value product runs while the last are computed
+    // P of the first 48 or the last 16 columns (and the rescaled O) is there: most of the value product runs while the last are computed
     auto hand_over = [&](int part) {
       tmem_wait_st();
       tc_fence_before();
@@ -335,6 +399,18 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
     tmem_st16p(t_s, w);
     exps(s2, w2);
     tmem_st8p(t_s + 16, w2);
+    if constexpr (PL::kRowsClear) {
+      const Seen seen = seen_keys(p, it);
+      if ((j + 1) * kTile > seen.all) {  // each Q tile's warps, the first to come clears
+        warp_wait(smem_u32(&bars->v_full[0]), (tiles + (j - it.j0)) & 1u, abort_flag, p.status,
+                  kDevTimeoutSoftmax);
+        const int r0 = max(seen.all - j * kTile, 0), r1 = min(max(seen.some - j * kTile, r0), kTile);
+        clear_hidden<T, PL::kVChunks, PL::kChunkBytes, 4>(smem + PL::kOffV, r0, r1,
+                                                          j * kTile - seen.all,
+                                                          bars->marks[unit % 3],
+                                                          (warp & 7) * 32 + lane, 256);
+      }
+    }
     hand_over(0);
     exps(s2 + 16, w2 + 8);
     tmem_st8p(t_s + 24, w2 + 8);
@@ -359,6 +435,8 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
   const int64_t prow = (static_cast<int64_t>(it.split) * p.hq + head) * p.total_q + it.q0 + tok;
   T *orow = static_cast<T *>(p.o) + static_cast<int64_t>(it.q0 + tok) * p.o_st + head * p.o_sh + col0;
   float *po = p.part_o + prow * p.d_v + col0;
+  const Bars::Marks &marks = bars->marks[unit % 3];
+  const bool marked = any && *const_cast<const volatile uint32_t *>(&marks.any) != 0;
 #pragma unroll 1
   for (int c = 0; c < kOCols / 16; ++c) {
     float v[16];
@@ -372,6 +450,25 @@ __device__ __forceinline__ void row_role(const Params &p, const Work &it, Bars *
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] *= f;
+    if (marked) {
+      // the cleared values of keys that this row sees: an infinity, or a NaN
+      const int first = seen_keys(p, it).all;
+#pragma unroll 1
+      for (int key = 0; key < min(end - first, 256); ++key) {
+        if (!(const_cast<const volatile uint32_t *>(marks.keys)[key >> 5] >> (key & 31) & 1u)) {
+          continue;
+        }
+        const T *src = static_cast<const T *>(p.v) +
+                       static_cast<int64_t>(it.k0 + first + key) * p.v_st + it.kvh * p.v_sh + col0 +
+                       16 * c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (col0 + 16 * c + (i & 8) >= p.d_v) break;
+          const float x = Elem<T>::to_f(src[i]);
+          v[i] += fabsf(x) < INFINITY ? 0.f : x;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (col0 + 16 * c + 8 * i >= p.d_v) continue;
@@ -558,6 +655,8 @@ __device__ __forceinline__ void scheduler_role(const Params &p, Bars *bars, int 
       if (!warp_wait(smem_u32(&bars->work_empty[slot]), ((count >> 1) & 1u) ^ 1u, abort_flag,
                      p.status, kDevTimeoutProducer))
         return;  // nothing more is handed out: the others' waits run out
+      if (lane < 9) reinterpret_cast<uint32_t *>(&bars->marks[count % 3])[lane] = 0u;
+      __syncwarp();
       if (lane == 0) {
         bars->work[slot] = w;
         mbar_arrive(smem_u32(&bars->work_full[slot]));
@@ -599,6 +698,34 @@ __device__ __forceinline__ bool next_work(Bars *bars, uint32_t k, int lane, int 
   return w.kvh >= 0;
 }
 
+// Value tiles at the edge of what a unit's rows see, between their load (v_raw) and
+// the products (v_full).
+template <typename T, int kDqk, int kDv>
+__device__ __forceinline__ void edge_role(const Params &p, Bars *bars, uint8_t *smem, int lane) {
+  using PL = Plan<kDqk, kDv>;
+  volatile int *abort_flag = &bars->abort_flag;
+  uint32_t tile = 0, raw = 0;  // V tiles so far; bit st: parity of stage st's next v_raw phase
+  Work w;
+  for (uint32_t k = 0; next_work(bars, k, lane, p.status, w); ++k) {
+    if (PL::kRowsClear) continue;
+    const Seen seen = seen_keys(p, w);
+    for (int j = max(seen.all / kTile, w.j0); j < w.j1; ++j) {
+      const uint32_t st = (tile + (j - w.j0)) % PL::kVStages;
+      if (!warp_wait(smem_u32(&bars->v_raw[st]), (raw >> st) & 1u, abort_flag, p.status,
+                     kDevTimeoutProducer))
+        return;
+      raw ^= 1u << st;
+      const int r0 = max(seen.all - j * kTile, 0), r1 = min(max(seen.some - j * kTile, r0), kTile);
+      clear_hidden<T, PL::kVChunks, PL::kChunkBytes, 4>(smem + PL::kOffV + st * PL::kVBytes, r0, r1,
+                                                        j * kTile - seen.all, bars->marks[k % 3],
+                                                        lane, 32);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars->v_full[st]));
+    }
+    tile += max(w.j1 - w.j0, 0);
+  }
+}
+
 template <typename T, int kDqk, int kDv>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map,
@@ -626,6 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->k_full[i]), 1);
       mbar_init(smem_u32(&bars->k_empty[i]), 2);  // by each Q tile's stream
       mbar_init(smem_u32(&bars->v_full[i]), 1);
+      mbar_init(smem_u32(&bars->v_raw[i]), 1);
       mbar_init(smem_u32(&bars->v_empty[i]), 2);
     }
     for (int i = 0; i < 2; ++i) {
@@ -636,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bars->p_full[i][1]), 8);
       mbar_init(smem_u32(&bars->o_full[i]), 1);
       mbar_init(smem_u32(&bars->work_full[i]), 1);
-      mbar_init(smem_u32(&bars->work_empty[i]), kRowWarps + 3);  // rows, producer, MMA twice
+      mbar_init(smem_u32(&bars->work_empty[i]), kRowWarps + 4);  // rows, producer, edge, MMA twice
     }
     mbar_init(smem_u32(&bars->cancel_full), 1);
     mbar_init(smem_u32(&bars->drain), 1);
@@ -659,15 +787,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t steps = 0, outs = 0, tiles = 0;
     Work it;
     for (uint32_t k = 0; next_work(bars, k, lane, p.status, it); ++k) {
-      row_role<T, kDqk, kDv>(p, it, bars, smem, tmem, warp, lane, steps, outs, tiles);
-      tiles += it.j1 - it.j0;
+      row_role<T, kDqk, kDv>(p, it, bars, smem, tmem, warp, lane, steps, outs, k, tiles);
+      tiles += max(it.j1 - it.j0, 0);
     }
-  } else if (warp > kProducerWarp) {
+  } else if (warp == kSchedulerWarp) {
     give_registers<kOtherRegs>();
-    if (warp == kSchedulerWarp) scheduler_role(p, bars, lane);
+    scheduler_role(p, bars, lane);
+  } else if (warp == kEdgeWarp) {
+    give_registers<kOtherRegs>();
+    edge_role<T, kDqk, kDv>(p, bars, smem, lane);
   } else if (warp == kProducerWarp) {
     give_registers<kOtherRegs>();
     uint32_t g = 0, gv = 0, gq[2] = {0, 0};  // K tiles, V tiles, Q tiles issued
+    uint32_t raw = 0, to_raw = 0;  // bit st: v_raw phases of stage st (parity); its last tile's
     if (lane == 0) {
       tma_prefetch_desc(&q_map);
       tma_prefetch_desc(&k_map);
@@ -692,6 +824,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (uint32_t k = 0; ok && next_work(bars, k, lane, p.status, it); ++k) {
       if (it.j1 <= it.j0) continue;
+      // first tile that the edge warp has to look at
+      const int edge = PL::kRowsClear ? INT32_MAX : seen_keys(p, it).all / kTile;
       load_q(0);
       for (int j = it.j0; ok && j < it.j1; ++j) {
         const uint32_t ks = g % PL::kKStages, vs = gv % PL::kVStages;
@@ -714,8 +848,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = warp_wait(smem_u32(&bars->v_empty[vs]), ((gv / PL::kVStages) & 1u) ^ 1u,
                              abort_flag, p.status, kDevTimeoutProducer)))
           break;
+        to_raw = (to_raw & ~(1u << vs)) | static_cast<uint32_t>(j >= edge) << vs;
+        if (j >= edge) raw ^= 1u << vs;
         if (lane == 0) {
-          const uint32_t vf = smem_u32(&bars->v_full[vs]);
+          const uint32_t vf = smem_u32(j >= edge ? &bars->v_raw[vs] : &bars->v_full[vs]);
           mbar_arrive_expect_tx(vf, PL::kVBytes);
 #pragma unroll
           for (int ch = 0; ch < PL::kVChunks; ++ch)
@@ -733,9 +869,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t t = g > PL::kKStages ? g - PL::kKStages : 0; t < g; ++t)
         wait_inline(smem_u32(&bars->k_full[t % PL::kKStages]), (t / PL::kKStages) & 1u, &never,
                     nullptr, 0);
-      for (uint32_t t = gv > PL::kVStages ? gv - PL::kVStages : 0; t < gv; ++t)
-        wait_inline(smem_u32(&bars->v_full[t % PL::kVStages]), (t / PL::kVStages) & 1u, &never,
-                    nullptr, 0);
+      for (uint32_t t = gv > PL::kVStages ? gv - PL::kVStages : 0; t < gv; ++t) {
+        const uint32_t st = t % PL::kVStages;
+        if (to_raw >> st & 1u)
+          wait_inline(smem_u32(&bars->v_raw[st]), (raw >> st & 1u) ^ 1u, &never, nullptr, 0);
+        else
+          wait_inline(smem_u32(&bars->v_full[st]), (t / PL::kVStages) & 1u, &never, nullptr, 0);
+      }
     }
     __syncwarp();
   } else {
@@ -783,9 +923,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A parity wait tells a phase from the one before it only, so a stream sees
     // every K and every V tile land, in order, and releases each itself: those it
     // multiplies when their products are done, those it has no step for
-    // as soon as they land (walk).  Scores of tile t are issued once V tile t -
-    // kVStages has been seen, so the rows' own wait for V tile t can not be
-    // answered by an earlier phase either.
+    // as soon as they land (walk).  Where rows look at V tile t themselves, its
+    // scores are issued once tile t - 1 has been seen, so that an earlier phase can not
+    // answer their wait either.
     enum Need { kUnit, kQK, kP, kNone };
     struct Stream {
       Need need = kUnit;
@@ -836,7 +976,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       moved |= walk(s);
       if (s.need == kQK) {
         const uint32_t t = s.g + s.i;
-        if (s.k < t || s.v + PL::kVStages <= t) return moved;
+        if (s.k < t || (PL::kRowsClear && s.v < t)) return moved;
         if (s.i == 0 && !ready(&bars->q_full[x], s.q & 1u)) return moved;
         if (!k_landed(t)) return moved;
         tc_fence_after();
@@ -953,6 +1093,13 @@ cudaError_t launch_t(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
                      const Params &p, unsigned grid, cudaStream_t stream) {
   auto kern = prompt_attention_kernel<T, kDqk, kDv>;
   constexpr int smem = Plan<kDqk, kDv>::kSmemBytes;
+  // registers that the row warps take must have been given up by the others
+  static const bool fits = [&] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess &&
+           a.numRegs * kThreads >= 32 * (kRowWarps * kRowRegs + (kThreads / 32 - kRowWarps) * kOtherRegs);
+  }();
+  if (!fits) return cudaErrorInvalidConfiguration;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kern<<<grid, kThreads, smem, stream>>>(qm, km, vm, p);
@@ -1026,6 +1173,9 @@ cudaError_t launch_prompt(const CUtensorMap &qm, const CUtensorMap &km, const CU
   p.batch = a->batch;
   p.total_q = a->total_q;
   p.total_k = a->total_k;
+  p.v = a->v;
+  p.v_st = a->v_stride_t;
+  p.v_sh = a->v_stride_h;
   p.hq = a->num_q_heads;
   p.hkv = a->num_kv_heads;
   p.group = a->num_q_heads / a->num_kv_heads;

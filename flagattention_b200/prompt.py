@@ -60,7 +60,9 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
     masking is bottom-right aligned: query i of lq sees keys 0 .. lk - lq + i.
     Returns out [total_q, Hq, Dv]; with return_lse also the log-sum-exp of
     the scaled scores, f32 [Hq, total_q].  A row that sees no key gets zeros
-    and -inf; rows past cu_seqlens_q[-1] are not written.
+    and -inf; rows past cu_seqlens_q[-1] are not written.  Keys and values that
+    a row does not see do not reach it, whatever they hold; a NaN or an infinity
+    in a value that it sees makes that element of the row NaN or infinite.
     """
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q

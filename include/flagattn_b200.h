@@ -171,7 +171,8 @@ int fa_split_kv_attention(const fa_decode_args *args, void *stream);
  * head h reads kv head h / (num_q_heads / num_kv_heads).  Causal: query i of
  * lq sees keys [0, lk - lq + i] of lk (bottom-right).  A row that sees no key
  * gets o = 0 and lse = -inf.  Tokens from cu_q[batch] on belong to no sequence
- * and are not written.
+ * and are not written.  Keys and values that a row does not see do not reach it,
+ * whatever they hold.
  * bf16 / f16, head sizes multiples of 8: d_qk <= 192, d_v <= 128; at most 128
  * query heads per kv head; scale > 0; pointers 16-byte aligned, strides
  * multiples of 8 elements.  lse (nullable): f32 [num_q_heads][total_q].

@@ -149,6 +149,59 @@ def test_neighbours_do_not_leak(value):
     check(q, k, v, lens, lens, causal=True, skip=(1,))
 
 
+@pytest.mark.parametrize("hq, hk, d, dv, dtype", [(8, 8, 128, 128, torch.bfloat16),
+                                                  (16, 2, 128, 128, torch.float16),
+                                                  (64, 1, 64, 64, torch.bfloat16),
+                                                  (4, 4, 192, 128, torch.bfloat16),
+                                                  (24, 1, 96, 72, torch.bfloat16),
+                                                  (3, 3, 64, 64, torch.float16)])
+@pytest.mark.parametrize("lens_q, lens_k", [([300, 70, 130], [300, 70, 130]),
+                                            ([40, 260, 9], [515, 300, 5]),
+                                            ([100], [9000])])
+def test_later_tokens_do_not_reach_earlier_rows(lens_q, lens_k, hq, hk, d, dv, dtype):
+    """A causal row's output does not depend on any bit of the keys that it does not
+    see.  Infinities and NaN in value rows reach exactly the elements that weigh
+    them (an infinity, or a NaN where infinities cancel), NaN keys every element of the rows
+    that see them; every other element keeps its bits."""
+    q, k, v = tensors(lens_q, lens_k, hq, hk, d, dv, dtype, seed=20)
+    cu = lambda x: torch.tensor([0] + list(np.cumsum(x)), dtype=torch.int32, device="cuda")  # noqa: E731
+    args = cu(lens_q), cu(lens_k)
+    clean, clean_l = fa.prompt_attention(q, k, v, *args, return_lse=True)
+    inf, nan = float("inf"), float("nan")
+    plants = [(0, 3, inf), (0, 3, inf), (0, 5, -inf), (1, 5, inf), (2, 7, nan), (5, 0, nan), (1, dv - 1, nan),
+              (40, 9, -inf), (3, 9, -inf)]
+    want = clean.double().clone()
+    bad_v = v.clone()
+    a = b = 0
+    for n, m in zip(lens_q, lens_k):
+        row = torch.arange(n, device="cuda")
+        for back, dim, x in plants:                       # `back` tokens before the last
+            t = m - 1 - back * max(1, min(n, m) // 45)
+            if t < 0:
+                continue
+            bad_v[b + t, back % hk, dim] = x
+            sees = row + m - n >= t
+            heads = torch.arange(hq, device="cuda") // (hq // hk) == back % hk
+            want[a:a + n, :, dim] += torch.where(sees[:, None] & heads, x, 0.0)
+        a, b = a + n, b + m
+    got, got_l = fa.prompt_attention(q, k, bad_v, *args, return_lse=True)
+    assert torch.equal(got_l, clean_l)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(0, 9, -9), want.to(dtype).nan_to_num(0, 9, -9))
+    want, want_l, bad_k, bad_v = clean.double(), clean_l.clone(), k.clone(), v.clone()
+    a = b = 0
+    for n, m in zip(lens_q, lens_k):                      # the last third's keys and values
+        t = m - max(min(n, m) // 3, 1)
+        bad_k[b + t:b + m], bad_v[b + t:b + m] = nan, nan
+        sees = torch.arange(n, device="cuda") + m - n >= t
+        want[a:a + n] = torch.where(sees[:, None, None], nan, clean[a:a + n].double())
+        want_l[:, a:a + n] = torch.where(sees, nan, clean_l[:, a:a + n])
+        a, b = a + n, b + m
+    got, got_l = fa.prompt_attention(q, bad_k, bad_v, *args, return_lse=True)
+    for x, y in ((got, want.to(dtype)), (got_l, want_l)):
+        assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(0, 9, -9), y.nan_to_num(0, 9, -9))
+
+
 def test_nan_stays_when_keys_are_split():
     """Few queries over many keys: a NaN in one range of the keys, and one in a
     query, which meets it in every range."""
