@@ -32,6 +32,12 @@ def raw_stream(device_index):
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def current_device():
+    """Index of the calling thread's current device: where the library launches
+    (a call on another one enters its tensors' device first)."""
+    return torch._C._cuda_getDevice()
+
+
 _templates = {}
 
 

@@ -14,8 +14,8 @@ import math
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import (empty, launch_lock, raw_stream, require_cuda,
-                                       stream_workspace)
+from flagattention_b200._torch import (current_device, empty, launch_lock, raw_stream,
+                                       require_cuda, stream_workspace)
 
 
 _pack_attention, _attention_args = _lib.packer(_lib.Kv4AttentionArgs)
@@ -91,15 +91,14 @@ def _check_slots(slot_mapping, cache):
 
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(device_index, batch, hq, hk, head_size, group_size, dtype):
-    """(part_o, part_lse, merge) bytes for these sizes on this device."""
+    """(part_o, part_lse, merge) bytes for these sizes on this (the current) device."""
     a = _lib.Kv4AttentionArgs()
     a.cache = _lib.Kv4Cache(None, 0, hk, 16, head_size, group_size, dtype)
     a.batch, a.num_q_heads, a.scale = batch, hq, 1.0
     po, pl, mg = (ctypes.c_size_t(0) for _ in range(3))
-    with torch.cuda.device(device_index):
-        _lib.check(_lib.lib().fa_kv4_attention_workspace_size(
-            ctypes.byref(a), ctypes.byref(po), ctypes.byref(pl), ctypes.byref(mg)),
-            "fa_kv4_attention_workspace_size")
+    _lib.check(_lib.lib().fa_kv4_attention_workspace_size(
+        ctypes.byref(a), ctypes.byref(po), ctypes.byref(pl), ctypes.byref(mg)),
+        "fa_kv4_attention_workspace_size")
     return po.value, pl.value, mg.value
 
 
@@ -121,6 +120,9 @@ def append_kv_int4(k, v, cache, slot_mapping):
     dev = slot_mapping.get_device()
     if k.get_device() != dev or v.get_device() != dev:
         raise _lib.InvalidArgument("all tensors must be on the cache's device")
+    if dev != current_device():
+        with torch.cuda.device(dev):
+            return append_kv_int4(k, v, cache, slot_mapping)
     k, v = _rows16(k), _rows16(v)
     (k_t, k_h, _), (v_t, v_h, _) = k.stride(), v.stride()
     st = _lib.lib().fa_kv4_append(ctypes.byref(cache.struct()), k.data_ptr(), k_t, k_h,
@@ -138,6 +140,9 @@ def read_kv_int4(cache, slot_mapping):
     slot_mapping = _check_slots(slot_mapping, cache)
     n, heads, d = slot_mapping.shape[0], cache.num_kv_heads, cache.head_size
     dev = slot_mapping.get_device()
+    if dev != current_device():
+        with torch.cuda.device(dev):
+            return read_kv_int4(cache, slot_mapping)
     k, v = empty((n, heads, d), cache.dtype, dev), empty((n, heads, d), cache.dtype, dev)
     st = _lib.lib().fa_kv4_read(ctypes.byref(cache.struct()), k.data_ptr(), heads * d, d,
                                 v.data_ptr(), heads * d, d, slot_mapping.data_ptr(), n,
@@ -162,6 +167,10 @@ def paged_attention_int4(query, cache, context_lens, block_tables, attn_scale=No
             block_tables.get_device() != dev:
         require_cuda(query, context_lens, block_tables)
         raise _lib.InvalidArgument("all tensors must be on the cache's device")
+    if dev != current_device():
+        with torch.cuda.device(dev):
+            return paged_attention_int4(query, cache, context_lens, block_tables, attn_scale,
+                                        return_lse)
     if query.dim() != 3 or query.shape[2] != cache.head_size:
         raise _lib.InvalidArgument("query must be [num_seqs, num_q_heads, head_size of the cache]")
     c_dtype = cache.dtype

@@ -16,7 +16,7 @@ import math
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import (dtype_code, empty, launch_lock, raw_stream,
+from flagattention_b200._torch import (current_device, dtype_code, empty, launch_lock, raw_stream,
                                        require_cuda, status_ptr, stream_workspace)
 
 
@@ -38,13 +38,12 @@ def _rows(x):
 
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(device_index, batch, total_q, total_k, hq, hk, d_v, causal):
-    """Scratch of a call of these sizes on this device."""
+    """Scratch of a call of these sizes on this (the current) device."""
     a = _lib.PromptArgs(batch=batch, total_q=total_q, total_k=total_k, num_q_heads=hq,
                         num_kv_heads=hk, d_v=d_v, causal=causal)
     size = ctypes.c_size_t(0)
-    with torch.cuda.device(device_index):
-        _lib.check(_lib.lib().fa_prompt_workspace_size(ctypes.byref(a), ctypes.byref(size)),
-                   "fa_prompt_workspace_size")
+    _lib.check(_lib.lib().fa_prompt_workspace_size(ctypes.byref(a), ctypes.byref(size)),
+               "fa_prompt_workspace_size")
     return size.value
 
 
@@ -71,6 +70,10 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=True, sm_s
             cu_seqlens_q.get_device() != dev or cu_seqlens_k.get_device() != dev:
         require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
         raise _lib.InvalidArgument("all tensors must be on one device")
+    if dev != current_device():
+        with torch.cuda.device(dev):
+            return prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, sm_scale,
+                                    return_lse)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise _lib.InvalidArgument("q, k, v must be [tokens, heads, head size]")
     (total_q, hq, d), (total_k, hk, d_k), (total_v, hv, d_v) = q.shape, k.shape, v.shape
