@@ -1,6 +1,7 @@
 """torch helpers shared by the operator modules (device memory, streams)."""
 
 import ctypes
+import functools
 import threading
 
 import torch
@@ -36,6 +37,21 @@ def current_device():
     """Index of the calling thread's current device: where the library launches
     (a call on another one enters its tensors' device first)."""
     return torch._C._cuda_getDevice()
+
+
+def on_tensors_device(fn):
+    """fn with the device of its first argument current during the call."""
+    first = fn.__code__.co_varnames[0]
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        tensor = args[0] if args else kwargs.get(first)
+        if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda or \
+                tensor.get_device() == current_device():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(tensor.get_device()):
+            return fn(*args, **kwargs)
+    return call
 
 
 _templates = {}

@@ -12,8 +12,8 @@ import ctypes
 import torch
 
 from flagattention_b200 import _lib
-from flagattention_b200._torch import (dtype_code, ptr, require_cuda, sm_count, status_word,
-                                       stream_of)
+from flagattention_b200._torch import (dtype_code, on_tensors_device, ptr, require_cuda, sm_count,
+                                       status_word, stream_of)
 
 D_QK, D_V = 576, 512
 
@@ -26,6 +26,7 @@ def num_sm_parts(device, s_q, h_q, sparse):
     return out.value
 
 
+@on_tensors_device
 def get_mla_metadata(cache_seqlens, num_q_tokens_per_head_k, num_heads_k, num_heads_q=None,
                      is_fp8_kvcache=False, topk=None, num_sm_parts_override=None):
     """Tile-scheduler metadata for ``flash_mla_with_kvcache``.
@@ -146,6 +147,7 @@ def mla_decode(*args, **kwargs):
     MlaCall(*args, **kwargs).run()
 
 
+@on_tensors_device
 def flash_mla_with_kvcache(q, k_cache, block_table, cache_seqlens, head_dim_v,
                            tile_scheduler_metadata, num_splits, softmax_scale=None, causal=False,
                            is_fp8_kvcache=False, indices=None, out=None):
@@ -190,6 +192,7 @@ def flash_mla_with_kvcache(q, k_cache, block_table, cache_seqlens, head_dim_v,
     return out, lse
 
 
+@on_tensors_device
 def append_kv_rows(kv_rows, k_cache, slot_mapping):
     """Write new tokens' latent rows into the paged cache, in place.
 

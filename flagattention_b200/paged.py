@@ -26,7 +26,8 @@ import ctypes
 import torch
 
 from flagattention_b200 import _decode, _lib
-from flagattention_b200._torch import dtype_code, require_cuda, sm_count, status_word, stream_of
+from flagattention_b200._torch import (dtype_code, on_tensors_device, require_cuda, sm_count,
+                                       status_word, stream_of)
 
 
 def paged_num_splits(num_seqs, num_kv_heads, max_context_len, kv_block_size, num_sms,
@@ -60,6 +61,7 @@ def _mla_paged(query, key_cache, context_lens, block_tables, attn_scale):
     return out
 
 
+@on_tensors_device
 def paged_attention(query, key_cache, value_cache, context_lens, block_tables, attn_scale,
                     max_context_len, num_splits=0):
     """Drop-in for ``flag_attn.paged_attention`` (paged.py:20)."""

@@ -19,7 +19,8 @@ import math
 import torch
 
 from flagattention_b200 import _decode, _lib
-from flagattention_b200._torch import dtype_code, require_cuda, sm_count, status_word, stream_of
+from flagattention_b200._torch import (dtype_code, on_tensors_device, require_cuda, sm_count,
+                                       status_word, stream_of)
 
 BLOCK_M, BLOCK_N, MAX_SPLITS = 16, 128, 128
 
@@ -59,6 +60,7 @@ def _mla_contiguous(q, k, causal, sm_scale):
     return out, lse
 
 
+@on_tensors_device
 def _attention(q, k, v, causal, sm_scale):
     require_cuda(q, k, v)
     B, H, M, D = q.shape
