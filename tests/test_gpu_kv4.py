@@ -160,6 +160,30 @@ def test_subnormal_ranges():
         assert same(got, values(x, 64).to(x.dtype))
 
 
+@pytest.mark.parametrize("signed", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_scale(dtype, signed):
+    """Codes are those of IEEE division for every scale that the type has: a group for
+    each of its positive numbers as the largest value, beside random ones down to 0
+    or to its negative."""
+    bits = torch.arange(1, 0x7f80 if dtype is torch.bfloat16 else 0x7c00, device="cuda")
+    top = bits.to(torch.int16).view(dtype)
+    if signed:
+        top = top[top.double() <= torch.finfo(dtype).max / 2]
+    n = top.shape[0]
+    g = torch.Generator(device="cuda").manual_seed(21)
+    part = torch.rand(n, 64, generator=g, device="cuda", dtype=torch.float64)
+    x = (part * 2 - 1 if signed else part) * top.double()[:, None]
+    x[:, 17], x[:, 40] = top.double(), -top.double() if signed else 0.0
+    x = x.to(dtype)[:, None]
+    cache = fa.Int4KVCache(-(-n // 16), 1, 16, 64, dtype=dtype)
+    slots = torch.arange(n, device="cuda")
+    fa.append_kv_int4(x, x.flip(-1), cache, slots)
+    for got, rows_ in zip(fa.read_kv_int4(cache, slots), (x, x.flip(-1))):
+        want = values(rows_, 64).to(dtype)
+        assert torch.equal(got, want.clamp(max=torch.finfo(dtype).max))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_subnormal_scales(dtype):
     """Ranges of 1 .. 255 of the type's smallest steps: a scale of a few steps is
