@@ -375,6 +375,21 @@ def test_decode_values_of_very_different_sizes(kind, d, group, hq, dtype, factor
             assert (off <= bound).all(), off.max()
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e33])
+@pytest.mark.parametrize("lens", [[3000], [3000] * 300])
+def test_decode_bf16_range(size, lens):
+    """Value rows near both ends of bf16's range; the bound of
+    ``test_decode_long_context_keeps_its_accuracy``, which is relative."""
+    cache, table, q, data, n = build([3000], 8, 1, 128, 64, 16, torch.bfloat16, seed=22, size=size)
+    k, v = (_exact(x[:, 0], 64) for x in data[0])
+    want = torch.softmax(q[0].double() @ k.T * 128 ** -0.5, -1) @ v
+    batch = len(lens)
+    out = fa.paged_attention_int4(q.expand(batch, -1, -1), cache, n.expand(batch),
+                                  table.expand(batch, -1))
+    for b in {0, batch - 1}:
+        assert ((out[b].double() - want) / size).norm() / (want / size).norm() <= 3e-3
+
+
 def test_decode_nan_stays_and_does_not_spread():
     lens = [50, 70]
     cache, table, q, data, n = build(lens, 4, 2, 128, 64, 16, torch.bfloat16, seed=7)
