@@ -793,6 +793,7 @@ __global__ void __launch_bounds__(kWide ? 256 : 128)
   const int4 mg = merge[e];
   if (mg.x < 0 || in_group >= group) return;  // of all threads when wide
   RowSum<kVec> st;
+  st.init();
   st.template fold<kAtOnce>(part_o, part_lse, w, kRowWarps, 1 + mg.z, kD, lane, [&](int s) {
     return static_cast<int64_t>(s == 0 ? mg.x : mg.y + s - 1) * rows + row;
   });

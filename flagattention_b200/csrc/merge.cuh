@@ -193,9 +193,11 @@ __device__ __forceinline__ void mla_row_state(MergeState &st, const TP *__restri
 // NaN, which a maximum would drop; it makes the row and its lse NaN.
 template <int kVec>
 struct RowSum {
-  float m = -INFINITY, z = 0.f;
+  float m, z;
   float4 acc[kVec];
-  __device__ __forceinline__ RowSum() {
+  __device__ __forceinline__ void init() {
+    m = -INFINITY;
+    z = 0.f;
 #pragma unroll
     for (int c = 0; c < kVec; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
   }

@@ -1081,6 +1081,7 @@ __global__ void __launch_bounds__(128) prompt_merge_kernel(const __grid_constant
   if (tok >= __ldg(p.cu_q + p.batch)) return;  // of no sequence: not written
   const int lane = threadIdx.x & 31;
   RowSum<1> st;
+  st.init();
   st.fold<4>(p.part_o, p.part_lse, 0, 1, p.splits, p.d_v, lane,
              [&](int s) { return static_cast<int64_t>(s) * rows + row; });
   const float l = st.finish(
