@@ -26,6 +26,14 @@
 // the normal numbers 16 + c (shift, AND-OR) and bf16 operands this took 8
 // contexts of up to 65536 tokens from 147 us to 107.
 //
+// The tensor cores line products up by their operands' exponents, and that of a
+// subnormal is 2^-14 however small it is: bits more than 24 below drop out.  A
+// product of a lowest code and a query dim 2^k below the largest keeps 15 - k bits
+// so, all of a bf16 query's 8 bits up to k = 7 but an f16 query's 11 up to 4 only: scores of
+// f16 caches were 2^-21 off.  There every key code goes to bits 4 to 7 (three shifts
+// a word, where the time does not change; with bf16, 2^-23 off, they would cost
+// 4% of long contexts).
+//
 // f16 operands hold Q and P' = p * s exactly enough because both are brought
 // into its range by a power of two: Q by its row's largest magnitude (bf16 and
 // f16 queries then lose nothing above 2^-23 of it), P' by the largest product
@@ -203,6 +211,10 @@ struct Piece {
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int k) {
   return (k < 2 ? w : w8) & ((k & 1) ? 0x00f000f0u : 0x000f000fu);
 }
+// The same with every code at bits 4 to 7 of its half: 16 c * 2^-24.
+__device__ __forceinline__ uint32_t high_pair(uint32_t w, uint32_t w8, int k) {
+  return (k == 0 ? w << 4 : k == 1 ? w : k == 2 ? w >> 4 : w8) & 0x00f000f0u;
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -254,6 +266,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
   constexpr int kU = kD / 64;   // value words of a lane and token
   constexpr int kTileB = PL::kTileB, kHeads = PL::kHeads;
   constexpr bool kSplitP = std::is_same<T, __half>::value;
+  constexpr bool kHighKeys = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Control ctl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
@@ -401,20 +414,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
           x[d] = Elem<T>::to_f(el[d]) * norm;
           sum[32 * i / kG] += x[d];
         }
+        constexpr float kOdd = kHighKeys ? 1.f : 0.0625f;
         qf[t][i][0] = Elem<__half>::pack2(x[0], x[4]);
-        qf[t][i][1] = Elem<__half>::pack2(x[1] * 0.0625f, x[5] * 0.0625f);
+        qf[t][i][1] = Elem<__half>::pack2(x[1] * kOdd, x[5] * kOdd);
         qf[t][i][2] = Elem<__half>::pack2(x[2], x[6]);
-        qf[t][i][3] = Elem<__half>::pack2(x[3] * 0.0625f, x[7] * 0.0625f);
+        qf[t][i][3] = Elem<__half>::pack2(x[3] * kOdd, x[7] * kOdd);
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-        sum[g] *= 0x1p-24f;
+        sum[g] *= kHighKeys ? 0x1p-20f : 0x1p-24f;
         qs[t][g][0] = __shfl_sync(0xffffffffu, sum[g], 8 * q);
         qs[t][g][1] = __shfl_sync(0xffffffffu, sum[g], 8 * q + 4);
       }
-      const float un = p.scale_log2 * pow2(f + 12) * 4096.f;  // scale * 2^(f + 24)
+      // scale * 2^(f + 24), or 2^(f + 20)
+      const float un = p.scale_log2 * pow2(f + 12) * (kHighKeys ? 256.f : 4096.f);
       unit[t][0] = __shfl_sync(0xffffffffu, un, 8 * q);
       unit[t][1] = __shfl_sync(0xffffffffu, un, 8 * q + 4);
     }
@@ -484,9 +499,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
           const uint32_t ka8 = ka[i2] >> 8, kb8 = kb[i2] >> 8;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
-            const uint32_t a0 = code_pair(ka[i2], ka8, 2 * ks), a1 = code_pair(kb[i2], kb8, 2 * ks),
-                           a2 = code_pair(ka[i2], ka8, 2 * ks + 1),
-                           a3 = code_pair(kb[i2], kb8, 2 * ks + 1);
+            auto key_pair = [](uint32_t w, uint32_t w8, int k) {
+              return kHighKeys ? high_pair(w, w8, k) : code_pair(w, w8, k);
+            };
+            const uint32_t a0 = key_pair(ka[i2], ka8, 2 * ks), a1 = key_pair(kb[i2], kb8, 2 * ks),
+                           a2 = key_pair(ka[i2], ka8, 2 * ks + 1),
+                           a3 = key_pair(kb[i2], kb8, 2 * ks + 1);
 #pragma unroll
             for (int t = 0; t < kNT; ++t)
               mma16816(acc[t], a0, a1, a2, a3, qf[t][i2][2 * ks], qf[t][i2][2 * ks + 1]);

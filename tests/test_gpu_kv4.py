@@ -375,6 +375,24 @@ def test_decode_values_of_very_different_sizes(kind, d, group, hq, dtype, factor
             assert (off <= bound).all(), off.max()
 
 
+@pytest.mark.parametrize("dtype, bound", [(torch.bfloat16, 2.0 ** -20), (torch.float16, 2.0 ** -22)])
+@pytest.mark.parametrize("d, group, hq", [(64, 32, 16), (64, 64, 64), (128, 128, 32), (256, 64, 8)])
+def test_log_sum_exp_of_short_contexts(d, group, hq, dtype, bound):
+    """2-norm of the log-sum-exp's error against 64 bits.  A score is the small
+    difference of two sums about ten times as large, each in f32 over d products
+    (simulated with exact products, one rounding per 16 dims: 1e-7 of the scores) and the
+    logarithm adds 2^-22 of a binary unit at most: 2^-22 in all.  bf16 caches, whose codes'
+    products lose bits 24 below the largest operands' exponents: four times that."""
+    lens = [1 + b % 13 for b in range(60)]
+    cache, table, q, data, n = build(lens, hq, 4, d, group, 16, dtype, seed=23)
+    _, lse = fa.paged_attention_int4(q, cache, n, table, return_lse=True)
+    want = torch.empty_like(lse, dtype=torch.float64)
+    for b, (k, _) in enumerate(data):
+        kk = _exact(k, group).transpose(0, 1).repeat_interleave(hq // 4, 0)
+        want[b] = torch.logsumexp(d ** -0.5 * q[b].double()[:, None] @ kk.transpose(1, 2), -1)[:, 0]
+    assert (lse.double() - want).norm() / want.norm() <= bound
+
+
 @pytest.mark.parametrize("size", [1e-30, 1e33])
 @pytest.mark.parametrize("lens", [[3000], [3000] * 300])
 def test_decode_bf16_range(size, lens):
