@@ -7,12 +7,12 @@
 //   value codes  16 * D / 2 bytes
 //   scales       16 tokens x [keys: D / G x (lo, scale) | values: the same],
 //                two 16-bit numbers (bf16 or f16, the type of the rows) each
-// so any run of tokens is a run of whole tiles, fetched by one bulk copy each.
+// so any run of tokens is a run of whole tiles, each contiguous in memory.
 // A code c of a group of G dims stands for lo + scale * c.
 //
-// Codes are packed eight to a 32-bit word, and words are ordered so that
-// a lane of a warp reads what it feeds to mma.m16n8k16 with 16-byte loads and
-// without bank conflicts.  Lane l = 4 r + q (r = l / 4, q = l % 4):
+// Codes are packed eight to a 32-bit word, and words are ordered so that a lane
+// of a warp reads what it feeds to mma.m16n8k16 from global memory with wide loads (16
+// bytes; 8 for keys of 64 dims), a warp's adjacent.  Lane l = 4 r + q (r = l / 4, q = l % 4):
 //   keys (A operand, rows = tokens r and r + 8): lane q of row t owns the
 //     words j = 4 i + q (dims 8 j .. 8 j + 7, in order, nibble n = dim 8 j +
 //     n), adjacent in memory; rows of more than 128 dims are cut into planes

@@ -20,10 +20,11 @@
 // A thread takes every grid-th token and loads the next ones' rows while it
 // works on one; four blocks of 256 threads per SM.
 //
-// Measured: 16383 tokens of 8 kv heads of 128, groups of 64, bf16, written and
-// read back: 46-50 us for 172 MB (3.5 TB/s; schedulers issue in 75% / 60% of the
-// cycles of the write / the read, the integer pipe is 60% / 64% busy: the
-// instruction count binds).  64 tokens: 4.2 us for both launches.
+// Measured: 16383 tokens of 8 kv heads of 128, groups of 64, bf16: 28.7 us to write
+// (30.4 with a cold L2), 18.4 to read (20.4), 47.6 for both, 172 MB (3.6 TB/s).  Schedulers
+// issue in 76% of the write's cycles and 59% of the read's, the integer pipe is
+// 61% / 63% busy: the write is near its instruction count, the read waits.  64
+// tokens: 6.1 us for both launches.
 #include "kv4.cuh"
 #include "flagattn_b200.h"
 

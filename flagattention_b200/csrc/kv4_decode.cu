@@ -13,7 +13,7 @@
 // schedulers issue 400 warp instructions and its integer pipes 200: the
 // instruction count per tile is the second bound.  mma.sync m16n8k16 (f16)
 // fits that: tokens (S = K Q^T) or dims (O^T = V^T P) are the 16 rows, up to 8
-// heads the columns, codes come straight from 16-byte shared-memory loads into
+// heads the columns, codes come straight from 16-byte loads of global memory into
 // A fragments, and P moves between the two products in registers (movmatrix).
 // tcgen05 would need the expanded operand written to shared memory first, 4x
 // the bytes of the codes.
@@ -53,12 +53,13 @@
 // Scores, sums and the merge are f32.  The tensor cores drop bits of their own
 // f32 accumulators, so value sums leave them every 64 tiles.
 //
-// Measured at 64 query / 8 kv heads of 128, groups of 64, bf16: 8 contexts of
-// 20001 to 65536 tokens 89-92 us (390 MB read from HBM, 4.3 TB/s; schedulers
-// issue in 57% of the cycles, the integer pipe is 52% busy: the instruction count binds
-// before HBM does), 32 of 1000 to 4096 tokens 29.9 us, one of 700 tokens 9.3 us (of
-// 8000: 18.3 with a cold L2);
-// 64 of 1 to 4001 tokens, 64 / 4 heads of 64, f16: 31.3 us.
+// Measured as graphs of two calls, 64 query / 8 kv heads of 128, groups of 64, bf16: 8
+// contexts of 20001 to 65536 tokens 89 us (390 MB read from HBM, 4.4 TB/s; 96 as
+// calls), 32 of 1000 to 4096 tokens 30.8 us from L2 and 33.8 with a cold one, one of 700
+// tokens 9.3 us (of 8000: 18.3 cold); 64 of 1 to 4001 tokens, 64 / 4 heads of 64, f16: 34.9
+// us.  No pipe is full at the long ones (schedulers issue in 56% of the cycles, the
+// integer pipe is 55% busy, 64% of the copy rate): 16 warps an SM, each on one
+// tile's chain from codes to scores to weights to values, leave gaps.
 #include "kv4.cuh"
 #include "flagattn_b200.h"
 #include "merge.cuh"
@@ -352,7 +353,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kD, kNT))
     if (at >= 0 && lane == 0) bulk_prefetch_l2(tile_ptr(at), kTileB);
   };
   // a piece's loads: Q rows, block table, its first tile into registers, the
-  // next ones into L2.  Issued before the previous piece is merged.
+  // next ones into L2.  Issued after the previous piece is merged (before, the
+  // registers of both spill).
   uint4 qraw[kNT][kW];
   int at = -1;
   auto begin = [&](const Piece &pc) {

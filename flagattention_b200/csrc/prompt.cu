@@ -26,11 +26,12 @@
 // exchanged only when one has to move, and O rescaled only past a factor 2^8.
 //
 // Measured: one causal prompt of 8192 tokens, 64 query / 8 kv heads of 128,
-// bf16: 890-917 us at full clocks (1.20-1.24 PFLOP/s), 1030 us in a loop under
-// the power cap (1.07 PFLOP/s; the tensor pipe is active 51% of the cycles); 16 prompts
-// of 1 to 2048 tokens: 483 us; 2 prompts of 1000 to 2048 tokens, 128 heads of
-// 192 / 128: 322-364 us; 256 tokens over 16256 keys: 147 us (224 without split
-// keys); one prompt of 37 tokens: 12.4 us.
+// bf16: 942 us for launches 20 ms apart (SM clock 1965 MHz, 1.17 PFLOP/s), 1040 us in
+// a loop under the power cap (1605 MHz, 1.06 PFLOP/s); the tensor pipe is active 61% of
+// the cycles, 45% of those of 16 packed prompts of 1 to 2048 tokens (451 us apart, 486 in
+// a loop at 1657 MHz); 2 prompts of 1000 to 2048 tokens, 128 heads of 192 / 128: 352 and
+// 378 us; 256 tokens over 16256 keys: 152 us (about 224 without split keys);
+// one prompt of 37 tokens: 11.4 us.
 //
 //   warps 0-7 / 8-15: rows of Q tile 0 / 1 (two threads per row, S read from
 //     TMEM, P written over it as the A operand of P V)
