@@ -72,6 +72,7 @@ __device__ __forceinline__ bool find_slot(const Pool &pool, int64_t slot, int he
 // than two ulp, and adding the exact remainder times r rounds a number that is
 // off by 2^-22 ulp, while d / s is no nearer than 2^-12 ulp to a rounding boundary
 // (it is a multiple of 2^-k / s, and no boundary: that has 25 significant bits).
+// The method is Markstein's: one correction by the exact remainder.
 __device__ __forceinline__ float quotient(float d, float s, float r) {
   const float q = d * r;
   return fmaf(fmaf(-q, s, d), r, q);
